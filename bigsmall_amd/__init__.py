@@ -11,6 +11,7 @@ kernels on the GPU:
     decompress_layers(src, [i, ...])        -> only the named layers
     decompress_delta(delta, base), load_delta(delta, base) -> a fine-tune from its XOR delta
     CompressedKVCache                       -> KV entries and blocks decoded on the GPU
+    PagedKVCache, kv_append, kv_attend, kv_read -> a paged 8-bit KV cache filled, attended to and read back on the GPU
     codec_registry.register_codec / get_codec / auto_select_codec
     compress_for_hub(model_dir, out_dir), from_pretrained(path) -> multi-shard .bs models + index
     migrate.migrate(path)                   -> re-encode a container into the GPU formats where smaller
@@ -27,7 +28,14 @@ from .streaming import StreamingLoader, decompress_layers
 from .verify import verify
 
 
+_PAGED_KV = ("PagedKVCache", "KVPool", "KVBatch", "Rope", "kv_append", "kv_attend", "kv_read")
+
+
 def __getattr__(name):
+    if name in _PAGED_KV:         # imports torch, which the rest imports on first use only
+        from . import paged_kv
+        globals().update({n: getattr(paged_kv, n) for n in _PAGED_KV})
+        return globals()[name]
     # transformers/accelerate are only needed by the streaming model
     if name == "BigSmallStreamingModel":
         from .streaming_inference import BigSmallStreamingModel
@@ -40,5 +48,6 @@ def __getattr__(name):
 
 __all__ = ["compress", "decompress", "load", "info", "verify", "StreamingLoader", "BigSmallStreamingModel",
            "decompress_layers", "decompress_delta", "load_delta",
-           "CompressedKVCache", "BigSmallVersionError", "DecodeError", "compress_for_hub", "from_pretrained",
+           "CompressedKVCache", "PagedKVCache", "KVPool", "KVBatch", "Rope", "kv_append", "kv_attend", "kv_read",
+           "BigSmallVersionError", "DecodeError", "compress_for_hub", "from_pretrained",
            "__version__"]

@@ -35,7 +35,7 @@ class BsChunkInfo(ctypes.Structure):
                 ("plane_mode", ctypes.c_uint32), ("coder", ctypes.c_uint32)]
 
 
-# (restype, argtypes) of every symbol include/bigsmall_hip.h declares
+# (restype, argtypes) of every symbol include/bigsmall_hip.h and bigsmall_kv.h declare
 _P, _U8P = ctypes.c_void_p, ctypes.c_void_p
 _U32, _U64, _I32, _INT = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int32, ctypes.c_int
 SIGNATURES = {
@@ -63,7 +63,34 @@ SIGNATURES = {
     "bs_refcodec_encode": (_INT, [_I32, _P, _U64, _U32, _P, _U64, ctypes.POINTER(_U64), _INT]),
     "bs_refcodec_decode_serial_batch": (_INT, [_P, _U32, _U32, _U32, _U32, _U32, _P, _U64, _P, _P]),
     "bs_refcodec_serial_chains_per_group": (_U32, []),
+    "bs_kv_append": (_INT, [_P, _P, _P, _P, _P]),
+    "bs_kv_attend_work_bytes": (_U64, [_P, _P, _U32]),
+    "bs_kv_attend": (_INT, [_P, _P, _P, _P, _U64, _P, _P]),
+    "bs_kv_read": (_INT, [_P, _P, _U32, _P, _U32, _P, _P, _P, _P]),
 }
+
+
+# include/bigsmall_kv.h
+class BsKvPool(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")] + \
+               [(n, _U32) for n in ("n_pages", "n_tails", "n_kv_heads", "head_dim", "kind")]
+
+
+class BsKvBatch(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("start", "cu", "table", "tails")] + \
+               [(n, _U32) for n in ("n_seqs", "table_stride", "table_cols", "n_rows", "max_new", "max_len")]
+
+
+class BsKvRows(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("q", "k", "v", "q_out", "cos", "sin")] + \
+               [(n, ctypes.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head")] + \
+               [(n, _U32) for n in ("n_q_heads", "rot", "interleaved", "n_pos")]
+
+
+class BsKvQuery(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("q", "out", "lse", "slopes", "prefix", "first")] + \
+               [("q_token", ctypes.c_int64), ("q_head", ctypes.c_int64), ("n_q_heads", _U32), ("window", _U32),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
 
 _lib = None
 

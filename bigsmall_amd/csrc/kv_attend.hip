@@ -1,0 +1,478 @@
+// Attention over the paged 8-bit KV cache.
+//
+// The rows of a sequence and kv head are its new tokens times the q heads of
+// the group, row r = token r / G, head r % G, in tiles of 16. A wave takes one
+// page at a time:
+//   S^T = K Q^T   (64 keys x 16 rows; K's codes as f16, exactly)
+//   softmax over keys with a running maximum and sum
+//   O^T += V^T P^T
+// in 16x16x32 products. Keys are numbered so that the 16 keys of a lane in S^T
+// (4 products of 16 keys, 4 accumulators each) are the 16 consecutive ones
+// 16g..16g+15 of its lane group g = lane / 16; that is what the lane needs as
+// the right operand of the second product, and 16 consecutive tokens of a
+// channel of V are 16 bytes of the page. So P stays in registers and K and V
+// go from memory to the matrix unit without LDS.
+//
+// Scales: a page's K scale multiplies the scores; its V scale goes into the
+// exponent, p' = 2^(s + log2(vs) - m) with m the running maximum of s +
+// log2(vs), so that O adds up codes * p' over pages of different scales, and
+// the denominator adds up (sum of p' in the page) / vs. Scores and log2 in base
+// 2, all in f32; p' goes to the product as f16 (11 bits), multiplied by 2^12 so
+// that weights down to 2^-26 of the largest keep them all.
+//
+// A row sees one interval of keys [lo, hi), whatever masks are set. A page that
+// lies inside the interval of all rows needs no comparison.
+#include "kv_common.h"
+
+#include <algorithm>
+
+#include "lds_limit.h"
+
+namespace bs_kv {
+bool check_pool(const bs_kv_pool* p);
+bool check_batch(const bs_kv_batch* b);
+}  // namespace bs_kv
+
+namespace {
+
+using namespace bs_kv;
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN2 = 0.69314718055994530942f;
+constexpr float P_SHIFT = 12.0f;
+constexpr float NEG_INF = -__builtin_inff();
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+struct Work {          // a launch's split results: per split and row O (f32, not divided), m, l
+  float* o;
+  float2* ml;
+  uint32_t splits;
+};
+
+// Interval of keys that row (token i of the sequence) sees.
+__device__ __forceinline__ int2 seen_by(const bs_kv_query& A, const SeqStep& s, uint32_t b, int i) {
+  const int pos = s.start + i;
+  int lo = 0, hi = pos + 1;
+  if (A.prefix) hi = max(hi, min(A.prefix[b], s.len));
+  if (A.first) lo = max(lo, A.first[s.t0 + i]);
+  if (A.window && (uint32_t)pos >= A.window) lo = max(lo, pos - (int)A.window + 1);
+  return make_int2(min(lo, hi), hi);
+}
+
+// What turns products into scores (base 2) besides the per-row and per-page scales.
+struct Score {
+  float scale;    // of q.k: times log2 e without a cap, divided by the cap with one
+  float cap;      // softcap * log2 e, 0: none
+};
+
+__device__ __forceinline__ float capped(float x, float cap) {      // cap * tanh(x)
+  const float e = exp2_fast(x * (2.0f * LOG2E));
+  return cap - cap * 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+}
+
+template <int D>
+struct Dims {
+  static constexpr int PAIRS = D / 64;              // 64 channels: two products of 32
+  static constexpr bool REST = D % 64 != 0;         // 16 or 32 more: one product
+  static constexpr int REST_GROUPS = (D % 64) / 8;  // lane groups that hold channels of it
+  static constexpr int STEPS = 2 * PAIRS + (REST ? 1 : 0);
+  static constexpr int TILES = D / 16;              // of 16 channels of O^T
+};
+
+// Channel that element 0 of product `step` holds in lane group g.
+template <int D>
+__device__ __forceinline__ int channel_of(int step, int g) {
+  return step < 2 * Dims<D>::PAIRS ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 64 * Dims<D>::PAIRS + 8 * g;
+}
+
+template <int D, int KIND>
+struct PageK {       // a lane's part of a K page: 4 keys
+  uint4 w[4][Dims<D>::PAIRS];
+  uint2 r[4];
+  __device__ __forceinline__ void load(const uint8_t* page, int lane) {
+    const int g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint8_t* row = page + (16 * ((lane & 15) >> 2) + 4 * t + (lane & 3)) * D;
+#pragma unroll
+      for (int c = 0; c < Dims<D>::PAIRS; ++c) w[t][c] = *(const uint4*)(row + 64 * c + 16 * g);
+      if constexpr (Dims<D>::REST) r[t] = g < Dims<D>::REST_GROUPS ? *(const uint2*)(row + 64 * Dims<D>::PAIRS + 8 * g) : make_uint2(0, 0);
+    }
+  }
+  __device__ __forceinline__ half8v operand(int t, int step) const {
+    if (step >= 2 * Dims<D>::PAIRS) {
+      half8v x = codes8_to_f16<KIND>(r[t].x, r[t].y);
+      return x;
+    }
+    const uint4 x = w[t][step / 2];
+    return step % 2 ? codes8_to_f16<KIND>(x.z, x.w) : codes8_to_f16<KIND>(x.x, x.y);
+  }
+};
+
+template <int D, int KIND>
+struct PageV {
+  uint4 w[Dims<D>::TILES];
+  __device__ __forceinline__ void load(const uint8_t* page, int lane) {
+#pragma unroll
+    for (int d = 0; d < Dims<D>::TILES; ++d) w[d] = *(const uint4*)(page + (16 * d + (lane & 15)) * PAGE + 16 * (lane >> 4));
+  }
+  __device__ __forceinline__ half8v operand(int d, int u) const {
+    return u ? codes8_to_f16<KIND>(w[d].z, w[d].w) : codes8_to_f16<KIND>(w[d].x, w[d].y);
+  }
+};
+
+// Running softmax of one row tile in a wave: this lane's row is lane & 15.
+template <int D>
+struct State {
+  f32x4 o[Dims<D>::TILES];
+  float m, l;        // m: over all keys so far; l: of this lane's keys
+};
+
+// Scores of a page from its products: s[t][i] belongs to key j0 + 4 t + i (j0: the lane group's first).
+template <int D>
+__device__ __forceinline__ void scores(f32x4 (&s)[4], const Score& sc, float row_scale, float page_scale, float shift,
+                                       int j0, int2 see, bool inside, float slope, int pos) {
+  const float c = row_scale * (page_scale * sc.scale);
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = s[t][i] * c;
+      if (sc.cap != 0.0f) x = capped(x, sc.cap);
+      const int j = j0 + 4 * t + i;
+      if (slope != 0.0f) x -= slope * fabsf((float)(pos - j));
+      x += shift;
+      if (!inside) x = (j >= see.x && j < see.y) ? x : NEG_INF;
+      s[t][i] = x;
+    }
+}
+
+// Weights from scores; rescales what is already there.
+template <int D>
+__device__ __forceinline__ void weights(f32x4 (&s)[4], State<D>& st, float inv_vs) {
+  float top = NEG_INF;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+  top = fmaxf(top, __shfl_xor(top, 16));
+  top = fmaxf(top, __shfl_xor(top, 32));
+  const float m = fmaxf(st.m, top);
+  const float base = (m == NEG_INF ? 0.0f : m) - P_SHIFT;
+  const float alpha = exp2_fast(st.m - (m == NEG_INF ? 0.0f : m));
+  st.m = m;
+  float sum = 0;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[t][i] = exp2_fast(s[t][i] - base);
+      sum += s[t][i];
+    }
+  // a page that the row does not see adds nothing, whatever its scale
+  st.l = st.l * alpha + (sum == 0.0f ? 0.0f : sum * inv_vs);
+#pragma unroll
+  for (int d = 0; d < Dims<D>::TILES; ++d) st.o[d] *= alpha;
+}
+
+constexpr int WAVES = 4;
+
+template <int D, int KIND>
+__global__ __launch_bounds__(64 * WAVES) void attend_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, int32_t* status) {
+  constexpr int STEPS = Dims<D>::STEPS, TILES = Dims<D>::TILES;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  const uint32_t h = blockIdx.y % P.n_kv_heads, b = blockIdx.z;
+  const uint32_t group = A.n_q_heads / P.n_kv_heads;
+  const uint32_t row_tiles = gridDim.y / P.n_kv_heads;
+  __shared__ float part_o[WAVES][16][17];
+  __shared__ float part_m[WAVES][16], part_l[WAVES][16];
+
+  SeqStep s;
+  if (!seq_step(B, b, s)) {
+    if (threadIdx.x == 0) report(status, BS_DEV_ERR_BOUNDS);
+    return;
+  }
+  const int rows = s.n * (int)group;
+  const Score sc = {A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E, A.softcap * LOG2E};
+  const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
+
+  for (int tile = blockIdx.y / P.n_kv_heads; tile * 16 < rows; tile += row_tiles) {
+    const int r = tile * 16 + (lane & 15);
+    const bool real = r < rows;
+    const int i = real ? r / (int)group : 0;
+    const uint32_t hq = h * group + (uint32_t)(real ? r % (int)group : 0);
+    const int pos = s.start + i;
+    const int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
+    const float slope = A.slopes ? A.slopes[hq] * LOG2E : 0.0f;
+
+    // the row of q as f16, scaled by a power of two to lie below 2 (exact for what is within 2^-14 of the largest)
+    const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
+    half8v q16[STEPS];
+    float row_scale;
+    {
+      uint16_t x[STEPS][8];
+      float top = 0;
+      bool fine = true;
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c) {
+        const int ch = channel_of<D>(c, g);
+        const uint4 w = (real && ch < D) ? *(const uint4*)(q + ch) : make_uint4(0, 0, 0, 0);
+        __builtin_memcpy(x[c], &w, 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          fine = fine && bf16_finite(x[c][e]);
+          top = fmaxf(top, fabsf(bf16_to_f32(x[c][e])));
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      int ok = fine;
+      ok &= __shfl_xor(ok, 16);
+      ok &= __shfl_xor(ok, 32);
+      const int e2 = (top == 0.0f || !ok) ? 0 : max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
+      row_scale = ok ? ldexpf(1.0f, e2) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)ldexpf(bf16_to_f32(x[c][e]), -e2) : (_Float16)0.0f;
+    }
+
+    // pages that any row of the tile sees, cut into splits
+    int lo = real ? see.x : 0x7FFFFFFF, hi = see.y;
+    if (real && see.x >= see.y) lo = 0x7FFFFFFF, hi = 0;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      lo = min(lo, __shfl_xor(lo, d));
+      hi = max(hi, __shfl_xor(hi, d));
+    }
+    const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
+    const int per = (page_hi - page_lo + (int)W.splits - 1) / (int)W.splits;
+    const int mine = page_lo + per * (int)blockIdx.x, end = min(mine + per, page_hi);
+    const int full_pages = s.len / (int)PAGE;      // pages from here on are the tail
+
+    State<D> st;
+#pragma unroll
+    for (int d = 0; d < TILES; ++d) st.o[d] = f32x4{0, 0, 0, 0};
+    st.m = NEG_INF;
+    st.l = 0;
+
+    for (int page = mine + wave; page < min(end, full_pages); page += WAVES) {
+      const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(B.table[(size_t)b * B.table_stride + page]);
+      if (id >= P.n_pages) {
+        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
+        continue;
+      }
+      PageK<D, KIND> k;
+      PageV<D, KIND> v;
+      k.load((const uint8_t*)P.k + id * unit + head, lane);
+      v.load((const uint8_t*)P.v + id * unit + head, lane);
+      const float ks = P.k_scale[(size_t)id * P.n_kv_heads + h], vs = P.v_scale[(size_t)id * P.n_kv_heads + h];
+      const float shift = __builtin_amdgcn_logf(vs);
+      f32x4 acc[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        acc[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.operand(t, c), q16[c], acc[t], 0, 0, 0);
+      }
+      const int j0 = page * (int)PAGE;
+      const bool inside = __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
+      scores<D>(acc, sc, row_scale, ks, shift, j0 + 16 * g, see, inside, slope, pos);
+      weights<D>(acc, st, exp2_fast(-shift));
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        half8v p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = (_Float16)acc[2 * u + e / 4][e % 4];
+#pragma unroll
+        for (int d = 0; d < TILES; ++d) st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.operand(d, u), p, st.o[d], 0, 0, 0);
+      }
+    }
+
+    // the tail: bf16 as it is; p' in two bf16 parts keeps 16 bits of it. Slots after the sequence's end hold anything.
+    if (mine < end && end > full_pages && wave == (end - 1 - mine) % WAVES) {
+      const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(B.tails[2 * b + 1]);
+      if (id >= P.n_tails) {
+        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
+      } else {
+        const uint16_t* kt = P.k_tail + id * unit + head;
+        const uint16_t* vt = P.v_tail + id * unit + head;
+        const int used = s.len - full_pages * (int)PAGE;
+        f32x4 acc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+          const int ch = channel_of<D>(c, g);
+          const uint4 none = make_uint4(0, 0, 0, 0);
+          const bf16x8 qb = __builtin_bit_cast(bf16x8, (real && ch < D) ? *(const uint4*)(q + ch) : none);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int key = 16 * ((lane & 15) >> 2) + 4 * t + (lane & 3);
+            const bf16x8 kb = __builtin_bit_cast(bf16x8, (key < used && ch < D) ? *(const uint4*)(kt + key * D + ch) : none);
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, qb, acc[t], 0, 0, 0);
+          }
+        }
+        scores<D>(acc, sc, row_scale == row_scale ? 1.0f : row_scale, 1.0f, 0.0f, full_pages * (int)PAGE + 16 * g, see, false, slope, pos);
+        weights<D>(acc, st, 1.0f);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          bf16x8 p_hi, p_lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = acc[2 * u + e / 4][e % 4];
+            p_hi[e] = (__bf16)x;
+            p_lo[e] = (__bf16)(x - (float)p_hi[e]);
+          }
+          const int key = 16 * g + 8 * u;
+#pragma unroll
+          for (int d = 0; d < TILES; ++d) {
+            uint16_t x[8];
+            const uint4 w = *(const uint4*)(vt + (16 * d + (lane & 15)) * PAGE + key);
+            __builtin_memcpy(x, &w, 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (key + e >= used) x[e] = 0;
+            bf16x8 vb;
+            __builtin_memcpy(&vb, x, 16);
+            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_hi, st.o[d], 0, 0, 0);
+            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_lo, st.o[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+
+    // join the waves: rows' m and l first, then O in pieces of 16 channels
+    st.l += __shfl_xor(st.l, 16);
+    st.l += __shfl_xor(st.l, 32);
+    __syncthreads();
+    if (lane < 16) part_m[wave][lane] = st.m, part_l[wave][lane] = st.l;
+    __syncthreads();
+    float m = NEG_INF;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, part_m[w][lane & 15]);
+    const float ref = m == NEG_INF ? 0.0f : m;
+    const float mine_scale = exp2_fast(st.m - ref);
+    // this thread's part of a piece: row tid / 16, channel tid % 16
+    const int wr = (int)threadIdx.x >> 4, wc = (int)threadIdx.x & 15;
+    const int wrow = tile * 16 + wr;
+    float row_l = 0, row_m = NEG_INF;
+    {
+      float ws = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) row_m = fmaxf(row_m, part_m[w][wr]);
+      const float rr = row_m == NEG_INF ? 0.0f : row_m;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) ws += part_l[w][wr] * exp2_fast(part_m[w][wr] - rr);
+      row_l = ws;
+    }
+    const float inv = row_l == 0.0f ? 0.0f : 1.0f / row_l;
+    const size_t out_row = (size_t)(s.t0 + (wrow < rows ? wrow / (int)group : 0)) * A.n_q_heads + h * group + (uint32_t)(wrow < rows ? wrow % (int)group : 0);
+    const size_t split_row = (size_t)blockIdx.x * B.n_rows * A.n_q_heads + out_row;
+    if (wrow < rows && wc == 0) {
+      if (W.splits > 1) W.ml[split_row] = make_float2(row_m, row_l);
+      else if (A.lse) A.lse[out_row] = row_l == 0.0f ? NEG_INF : (row_m - P_SHIFT + __builtin_amdgcn_logf(row_l)) * LN2;
+    }
+    if (W.splits > 1 && mine >= end) continue;      // nothing here: the joining kernel sees m = -inf and reads no O
+#pragma unroll
+    for (int d = 0; d < TILES; ++d) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part_o[wave][lane & 15][4 * g + e] = st.o[d][e] * mine_scale;
+      __syncthreads();
+      float x = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) x += part_o[w][wr][wc];
+      if (wrow < rows) {
+        if (W.splits > 1) W.o[split_row * D + 16 * d + wc] = x;
+        else A.out[out_row * D + 16 * d + wc] = f32_to_bf16(x * inv);
+      }
+    }
+  }
+}
+
+// Rows' parts from all splits into the output: one wave a row.
+template <int D>
+__global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32_t n) {
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= n) return;
+  float m = NEG_INF;
+  for (uint32_t k = 0; k < W.splits; ++k) m = fmaxf(m, W.ml[(size_t)k * n + row].x);
+  const float ref = m == NEG_INF ? 0.0f : m;
+  float l = 0, x[(D + 63) / 64] = {};
+  for (uint32_t k = 0; k < W.splits; ++k) {
+    const float2 ml = W.ml[(size_t)k * n + row];
+    if (ml.x == NEG_INF && ml.y == 0.0f) continue;
+    const float f = exp2_fast(ml.x - ref);
+    l += ml.y * f;
+    const float* o = W.o + ((size_t)k * n + row) * D;
+#pragma unroll
+    for (int c = 0; c < (D + 63) / 64; ++c)
+      if ((int)lane + 64 * c < D) x[c] += o[lane + 64 * c] * f;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int c = 0; c < (D + 63) / 64; ++c)
+    if ((int)lane + 64 * c < D) A.out[(size_t)row * D + lane + 64 * c] = f32_to_bf16(x[c] * inv);
+  if (A.lse && lane == 0) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+struct Plan {
+  uint32_t row_tiles, splits;
+};
+
+Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
+  const uint64_t group = n_q_heads / P->n_kv_heads;
+  const uint64_t tiles = std::min<uint64_t>(std::max<uint64_t>((B->max_new * group + 15) / 16, 1), 65535 / P->n_kv_heads);
+  const uint64_t blocks = tiles * P->n_kv_heads * B->n_seqs;
+  const uint64_t pages = (B->max_len + PAGE - 1) / PAGE;
+  uint64_t splits = blocks >= 1024 ? 1 : (1024 + blocks - 1) / blocks;
+  splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, pages / 8));
+  return {(uint32_t)tiles, (uint32_t)splits};
+}
+
+uint64_t split_rows(const bs_kv_batch* B, uint32_t n_q_heads, const Plan& p) {
+  return p.splits > 1 ? (uint64_t)p.splits * B->n_rows * n_q_heads : 0;
+}
+
+template <int D, int KIND>
+int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
+  const Plan p = make_plan(P, B, Q->n_q_heads);
+  const uint64_t rows = split_rows(B, Q->n_q_heads, p);
+  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.splits};
+  attend_kernel<D, KIND><<<dim3(p.splits, p.row_tiles * P->n_kv_heads, B->n_seqs), 64 * WAVES, 0, stream>>>(*P, *B, *Q, w, status);
+  if (p.splits > 1) {
+    const uint32_t n = B->n_rows * Q->n_q_heads;
+    join_kernel<D><<<(n + 3) / 4, 256, 0, stream>>>(*Q, w, n);
+  }
+  return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
+}
+
+bool heads_ok(const bs_kv_pool* P, uint32_t n_q_heads) { return n_q_heads > 0 && n_q_heads % P->n_kv_heads == 0; }
+
+}  // namespace
+
+extern "C" uint64_t bs_kv_attend_work_bytes(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
+  if (!check_pool(P) || !check_batch(B) || !heads_ok(P, n_q_heads) || B->n_rows == 0 || B->n_seqs == 0) return 0;
+  return split_rows(B, n_q_heads, make_plan(P, B, n_q_heads)) * (P->head_dim * 4ull + 8);
+}
+
+extern "C" int bs_kv_attend(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* d_work, uint64_t work_bytes,
+                            int32_t* d_status, void* stream) {
+  if (!check_pool(P) || !check_batch(B) || !Q || !heads_ok(P, Q->n_q_heads)) return BS_ERR_ARG;
+  if (B->n_rows == 0 || B->n_seqs == 0) return BS_OK;
+  if (!Q->q || !Q->out || (((uintptr_t)Q->q | (uintptr_t)Q->out) & 15) || (Q->q_token & 7) || (Q->q_head & 7)) return BS_ERR_ARG;
+  if (!(Q->softcap >= 0.0f) || B->n_seqs > 65535) return BS_ERR_ARG;
+  if (bs_kv_attend_work_bytes(P, B, Q->n_q_heads) > work_bytes || (work_bytes && (!d_work || ((uintptr_t)d_work & 15)))) return BS_ERR_CAP;
+  hipStream_t s = (hipStream_t)stream;
+#define BS_KV_GO(D)                                                                     \
+  return P->kind == BS_KV_FP8 ? launch<D, BS_KV_FP8>(P, B, Q, d_work, d_status, s)      \
+                              : launch<D, BS_KV_INT8>(P, B, Q, d_work, d_status, s)
+  switch (P->head_dim) {
+    case 64: BS_KV_GO(64);
+    case 80: BS_KV_GO(80);
+    case 96: BS_KV_GO(96);
+    case 128: BS_KV_GO(128);
+    default: BS_KV_GO(256);
+  }
+#undef BS_KV_GO
+}
