@@ -1,8 +1,11 @@
 // Attention over the paged 8-bit KV cache.
 //
 // The rows of a sequence and kv head are its new tokens times the q heads of
-// the group, row r = token r / G, head r % G, in tiles of 16. A wave takes one
-// page at a time:
+// the group, row r = token r / G, head r % G. Sequences with few rows go to
+// rows_kernel, with many to prompt_kernel; join_kernel puts together what was
+// split over the cache's length.
+//
+// rows_kernel: tiles of 16 rows. A wave takes one page at a time:
 //   S^T = K Q^T   (64 keys x 16 rows; K's codes as f16, exactly)
 //   softmax over keys with a running maximum and sum
 //   O^T += V^T P^T
@@ -44,11 +47,20 @@ constexpr float NEG_INF = -__builtin_inff();
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-struct Work {          // a launch's split results: per split and row O (f32, not divided), m, l
+// Split results: per slot and row O (f32, not divided), m, l. The kernels of a
+// call may split differently: `splits` is the kernel's own number, `slots` the
+// largest, 1 if nothing is split. A row has all its slots marked: parts without
+// keys with m = -inf and l = 0; a kernel that does not split while another does
+// writes the output itself and leaves l = -1.
+struct Work {
   float* o;
   float2* ml;
-  uint32_t splits;
+  uint32_t splits, slots;
 };
+
+// Which sequences a kernel takes: those with few rows, with many, or all.
+enum Take { FEW, MANY, ALL };
+__device__ __forceinline__ bool takes(Take take, int rows, int few) { return take == ALL || (rows <= few) == (take == FEW); }
 
 // Interval of keys that row (token i of the sequence) sees.
 __device__ __forceinline__ int2 seen_by(const bs_kv_query& A, const SeqStep& s, uint32_t b, int i) {
@@ -174,10 +186,24 @@ __device__ __forceinline__ void weights(f32x4 (&s)[4], State<D>& st, float inv_v
   for (int d = 0; d < Dims<D>::TILES; ++d) st.o[d] *= alpha;
 }
 
+// One row's m and l after all its keys of a split; without splits, its lse.
+__device__ __forceinline__ void mark_row(const bs_kv_query& A, const bs_kv_batch& B, const Work& W, uint32_t split, size_t row, float m,
+                                         float l) {
+  const size_t n = (size_t)B.n_rows * A.n_q_heads;
+  if (W.splits > 1) {
+    W.ml[split * n + row] = make_float2(m, l);
+    if (split == 0)
+      for (uint32_t k = W.splits; k < W.slots; ++k) W.ml[k * n + row] = make_float2(NEG_INF, 0.0f);
+  } else {
+    if (A.lse) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
+    if (W.slots > 1) W.ml[row] = make_float2(NEG_INF, -1.0f);
+  }
+}
+
 constexpr int WAVES = 4;
 
 template <int D, int KIND>
-__global__ __launch_bounds__(64 * WAVES) void attend_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, int32_t* status) {
+__global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few, int32_t* status) {
   constexpr int STEPS = Dims<D>::STEPS, TILES = Dims<D>::TILES;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
   const uint32_t h = blockIdx.y % P.n_kv_heads, b = blockIdx.z;
@@ -192,6 +218,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(bs_kv_pool P, bs_kv_
     return;
   }
   const int rows = s.n * (int)group;
+  if (!takes(take, rows, few)) return;
   const Score sc = {A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E, A.softcap * LOG2E};
   const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
 
@@ -368,10 +395,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(bs_kv_pool P, bs_kv_
     const float inv = row_l == 0.0f ? 0.0f : 1.0f / row_l;
     const size_t out_row = (size_t)(s.t0 + (wrow < rows ? wrow / (int)group : 0)) * A.n_q_heads + h * group + (uint32_t)(wrow < rows ? wrow % (int)group : 0);
     const size_t split_row = (size_t)blockIdx.x * B.n_rows * A.n_q_heads + out_row;
-    if (wrow < rows && wc == 0) {
-      if (W.splits > 1) W.ml[split_row] = make_float2(row_m, row_l);
-      else if (A.lse) A.lse[out_row] = row_l == 0.0f ? NEG_INF : (row_m - P_SHIFT + __builtin_amdgcn_logf(row_l)) * LN2;
-    }
+    if (wrow < rows && wc == 0) mark_row(A, B, W, blockIdx.x, out_row, row_m, row_l);
     if (W.splits > 1 && mine >= end) continue;      // nothing here: the joining kernel sees m = -inf and reads no O
 #pragma unroll
     for (int d = 0; d < TILES; ++d) {
@@ -390,16 +414,339 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(bs_kv_pool P, bs_kv_
   }
 }
 
+
+// Many rows: a workgroup of four waves takes 128 rows of a sequence and kv head,
+// 32 a wave, and goes through their pages together. Each page is converted to
+// f16 once, on its way into LDS (two buffers, one barrier a page, the next
+// page's loads in flight meanwhile), and read from there by all four waves as
+// the left operand of 32x32x16 products. Keys are numbered so that the 16 keys
+// of a lane in a 32-key S^T tile are two runs of 8, which are its part of the
+// right operand of two products with V^T: key bits 2 and 3 change places
+// between a tile's row and the key in it. LDS rows have an odd number of 16-byte
+// pieces, so that the 8 lanes of one LDS cycle hit different banks.
+constexpr int PROMPT_ROWS = 128;
+
+// The maximum of x over the two lanes that share a row (32 apart).
+__device__ __forceinline__ float pair_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+template <int D>
+struct Tile {
+  static constexpr int STEPS = D / 16;            // products over channels
+  static constexpr int TILES = (D + 31) / 32;     // of 32 channels of O^T (the last may be half empty)
+  static constexpr int K_ROW = D * 2 + 16;        // bytes
+  static constexpr int V_ROW = PAGE * 2 + 16;
+  static constexpr int K_BYTES = PAGE * K_ROW, V_BYTES = TILES * 32 * V_ROW;
+  static constexpr int BYTES = K_BYTES + V_BYTES;
+  static constexpr int LOADS = (PAGE * D / 16 + 255) / 256;   // 16-byte loads of a thread, for K and for V
+};
+
+template <int D, int KIND>
+struct Staged {      // a thread's part of a page on its way to LDS
+  uint4 k[Tile<D>::LOADS], v[Tile<D>::LOADS];
+  __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int tid) {
+#pragma unroll
+    for (int i = 0; i < Tile<D>::LOADS; ++i) {
+      const int at = (tid + 256 * i) * 16;
+      if (at < (int)PAGE * D) {
+        k[i] = *(const uint4*)(kp + at);
+        v[i] = *(const uint4*)(vp + at);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t* lds, int tid) const {
+#pragma unroll
+    for (int i = 0; i < Tile<D>::LOADS; ++i) {
+      const int at = (tid + 256 * i) * 16;
+      if (at < (int)PAGE * D) {
+        const int key = at / D, ch = at % D;
+        const int row = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
+        uint8_t* to = lds + row * Tile<D>::K_ROW + ch * 2;
+        *(half8v*)to = codes8_to_f16<KIND>(k[i].x, k[i].y);
+        *(half8v*)(to + 16) = codes8_to_f16<KIND>(k[i].z, k[i].w);
+        to = lds + Tile<D>::K_BYTES + at / (int)PAGE * Tile<D>::V_ROW + at % (int)PAGE * 2;
+        *(half8v*)to = codes8_to_f16<KIND>(v[i].x, v[i].y);
+        *(half8v*)(to + 16) = codes8_to_f16<KIND>(v[i].z, v[i].w);
+      }
+    }
+  }
+};
+
+// Scores s of 64 keys (two S^T tiles) into weights; m, l and o move on. j0: the page's first key.
+// The maximum only moves when some row's has grown by more than 8 times, so that
+// o is rescaled a few times and not at every page; weights then reach 2^(P_SHIFT
+// + 3), inside f16.
+template <int D>
+__device__ __forceinline__ void prompt_softmax(f32x16 (&s)[2], f32x16 (&o)[Tile<D>::TILES], float& m, float& l, const Score& sc, float row_scale,
+                                               float page_scale, float shift, float inv_vs, int j0, int half, int2 see, bool plain,
+                                               bool inside, float slope, int pos) {
+  float c = row_scale * (page_scale * sc.scale), add = shift;
+  if (!(plain && inside)) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int j = j0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
+        float x = s[t][i] * c;
+        if (sc.cap != 0.0f) x = capped(x, sc.cap);
+        if (slope != 0.0f) x -= slope * fabsf((float)(pos - j));
+        x += shift;
+        s[t][i] = (j >= see.x && j < see.y) ? x : NEG_INF;
+      }
+    c = 1.0f;
+    add = 0.0f;
+  }
+  float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+  top = pair_max(fmaf(top, c, add));
+  if (__ballot(top > m + 3.0f)) {
+    const float now = fmaxf(m, top);
+    const float alpha = exp2_fast(m - (now == NEG_INF ? 0.0f : now));
+    m = now;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < Tile<D>::TILES; ++d) o[d] *= alpha;
+  }
+  const float base = add - ((m == NEG_INF ? 0.0f : m) - P_SHIFT);
+  float sum = 0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[t][i] = exp2_fast(fmaf(s[t][i], c, base));
+      sum += s[t][i];
+    }
+  l += sum == 0.0f ? 0.0f : sum * inv_vs;
+}
+
+template <int D, int KIND>
+__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
+                                                                      int32_t* status) {
+  constexpr int STEPS = Tile<D>::STEPS, TILES = Tile<D>::TILES;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  __shared__ int bounds[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const uint32_t h = blockIdx.x % P.n_kv_heads, split = blockIdx.x / P.n_kv_heads, b = blockIdx.z;
+  const uint32_t group = A.n_q_heads / P.n_kv_heads;
+  SeqStep s;
+  if (!seq_step(B, b, s)) {
+    if (tid == 0) report(status, BS_DEV_ERR_BOUNDS);
+    return;
+  }
+  const int rows = s.n * (int)group;
+  if (!takes(take, rows, few)) return;
+  const Score sc = {A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E, A.softcap * LOG2E};
+  const bool plain = A.softcap == 0.0f && !A.slopes && A.scale > 0.0f;
+  const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
+  const int full_pages = s.len / (int)PAGE, row_tiles = (rows + PROMPT_ROWS - 1) / PROMPT_ROWS;
+
+  // the last tiles, which see most under a causal mask, come first
+  for (int tile = row_tiles - 1 - (int)blockIdx.y; tile >= 0; tile -= (int)gridDim.y) {
+    const int r = tile * PROMPT_ROWS + wave * 32 + (lane & 31);
+    const bool real = r < rows;
+    const int i = real ? r / (int)group : 0;
+    const uint32_t hq = h * group + (uint32_t)(real ? r % (int)group : 0);
+    const int pos = s.start + i;
+    int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
+    const float slope = A.slopes ? A.slopes[hq] * LOG2E : 0.0f;
+
+    const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
+    half8v q16[STEPS];
+    float row_scale;
+    {
+      uint16_t x[STEPS][8];
+      float top = 0;
+      bool fine = true;
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c) {
+        const uint4 w = real ? *(const uint4*)(q + 16 * c + 8 * half) : make_uint4(0, 0, 0, 0);
+        __builtin_memcpy(x[c], &w, 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          fine = fine && bf16_finite(x[c][e]);
+          top = fmaxf(top, fabsf(bf16_to_f32(x[c][e])));
+        }
+      }
+      top = pair_max(top);
+      const bool ok = pair_max(fine ? 0.0f : 1.0f) == 0.0f;
+      const int e2 = (top == 0.0f || !ok) ? 0 : max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
+      row_scale = ok ? ldexpf(1.0f, e2) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)ldexpf(bf16_to_f32(x[c][e]), -e2) : (_Float16)0.0f;
+    }
+
+    // keys that any row of the wave, and of the workgroup, sees
+    int lo = see.x < see.y ? see.x : 0x7FFFFFFF, hi = see.x < see.y ? see.y : 0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      lo = min(lo, __shfl_xor(lo, d));
+      hi = max(hi, __shfl_xor(hi, d));
+    }
+    const int wave_lo = __builtin_amdgcn_readfirstlane(lo), wave_hi = __builtin_amdgcn_readfirstlane(hi);
+    __syncthreads();
+    if (lane == 0) bounds[0][wave] = lo, bounds[1][wave] = hi;
+    __syncthreads();
+    lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
+    hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
+    const int per = (page_hi - page_lo + (int)W.splits - 1) / (int)W.splits;
+    const int begin = __builtin_amdgcn_readfirstlane(page_lo + per * (int)split);
+    const int end = __builtin_amdgcn_readfirstlane(min(begin + per, page_hi));
+    const int full_end = min(end, full_pages);
+
+    f32x16 o[TILES];
+#pragma unroll
+    for (int d = 0; d < TILES; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0;
+    float m = NEG_INF, l = 0;
+
+    const int32_t* table = B.table + (size_t)b * B.table_stride;
+    Staged<D, KIND> st;
+    bool next_ok = false;
+    float next_ks = 0, next_vs = 1;
+    const auto fetch = [&](int page) {
+      uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(table[page]);
+      next_ok = id < P.n_pages;
+      if (!next_ok) {
+        if (tid == 0) report(status, BS_DEV_ERR_BOUNDS);
+        id = 0;
+      }
+      st.load((const uint8_t*)P.k + id * unit + head, (const uint8_t*)P.v + id * unit + head, tid);
+      next_ks = P.k_scale[(size_t)id * P.n_kv_heads + h];
+      next_vs = P.v_scale[(size_t)id * P.n_kv_heads + h];
+    };
+    if (begin < full_end) fetch(begin);
+    for (int page = begin; page < full_end; ++page) {
+      uint8_t* buf = lds + ((page - begin) & 1) * Tile<D>::BYTES;
+      st.store(buf, tid);
+      const bool ok = next_ok;
+      const float ks = next_ks, shift = __builtin_amdgcn_logf(next_vs);
+      if (page + 1 < full_end) fetch(page + 1);
+      __syncthreads();
+      const int j0 = page * (int)PAGE;
+      if (!ok || j0 >= wave_hi || j0 + (int)PAGE <= wave_lo) continue;
+      f32x16 acc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[t][e] = 0;
+        const uint8_t* row = buf + (32 * t + (lane & 31)) * Tile<D>::K_ROW + 16 * half;
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(row + 32 * c), q16[c], acc[t], 0, 0, 0);
+      }
+      const bool inside = __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
+      prompt_softmax<D>(acc, o, m, l, sc, row_scale, ks, shift, exp2_fast(-shift), j0, half, see, plain, inside, slope, pos);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        half8v p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = (_Float16)acc[u >> 1][8 * (u & 1) + e];
+        const uint8_t* row = buf + Tile<D>::K_BYTES + (lane & 31) * Tile<D>::V_ROW + 32 * u + 16 * half;
+#pragma unroll
+        for (int d = 0; d < TILES; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(row + 32 * d * Tile<D>::V_ROW), p, o[d], 0, 0, 0);
+      }
+    }
+
+    // the tail, as in rows_kernel
+    if (begin < end && end > full_pages && full_pages * (int)PAGE < wave_hi) {
+      const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(B.tails[2 * b + 1]);
+      if (id >= P.n_tails) {
+        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
+      } else {
+        const uint16_t* kt = P.k_tail + id * unit + head;
+        const uint16_t* vt = P.v_tail + id * unit + head;
+        const int used = s.len - full_pages * (int)PAGE;
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        f32x16 acc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[t][e] = 0;
+        const int row = lane & 31, key0 = (row & 0x13) | ((row & 4) << 1) | ((row & 8) >> 1);
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) {
+          const bf16x8 qb = __builtin_bit_cast(bf16x8, real ? *(const uint4*)(q + 16 * c + 8 * half) : none);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int key = 32 * t + key0;
+            const bf16x8 kb = __builtin_bit_cast(bf16x8, key < used ? *(const uint4*)(kt + key * D + 16 * c + 8 * half) : none);
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb, qb, acc[t], 0, 0, 0);
+          }
+        }
+        prompt_softmax<D>(acc, o, m, l, sc, row_scale == row_scale ? 1.0f : row_scale, 1.0f, 0.0f, 1.0f, full_pages * (int)PAGE, half, see, plain,
+                          false, slope, pos);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          bf16x8 p_hi, p_lo;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float x = acc[u >> 1][8 * (u & 1) + e];
+            p_hi[e] = (__bf16)x;
+            p_lo[e] = (__bf16)(x - (float)p_hi[e]);
+          }
+          const int key = 16 * u + 8 * half;
+#pragma unroll
+          for (int d = 0; d < TILES; ++d) {
+            const int ch = 32 * d + (lane & 31);
+            bf16x8 vb = __builtin_bit_cast(bf16x8, ch < D ? *(const uint4*)(vt + ch * PAGE + key) : none);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (key + e >= used) vb[e] = (__bf16)0.0f;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, p_hi, o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb, p_lo, o[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+
+    l = pair_sum(l);
+    if (real) {
+      const size_t out_row = (size_t)(s.t0 + i) * A.n_q_heads + hq;
+      if (half == 0) mark_row(A, B, W, split, out_row, m, l);
+      if (W.splits == 1 || begin < end) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        float* part = W.o + ((size_t)split * B.n_rows * A.n_q_heads + out_row) * D;
+#pragma unroll
+        for (int d = 0; d < TILES; ++d)
+#pragma unroll
+          for (int a = 0; a < 4; ++a) {
+            const int ch = 32 * d + 8 * a + 4 * half;
+            if (ch >= D) continue;
+            if (W.splits > 1) {
+              *(float4*)(part + ch) = make_float4(o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]);
+            } else {
+              uint2 w;
+              w.x = f32_to_bf16(o[d][4 * a] * inv) | ((uint32_t)f32_to_bf16(o[d][4 * a + 1] * inv) << 16);
+              w.y = f32_to_bf16(o[d][4 * a + 2] * inv) | ((uint32_t)f32_to_bf16(o[d][4 * a + 3] * inv) << 16);
+              *(uint2*)(A.out + out_row * D + ch) = w;
+            }
+          }
+      }
+    }
+  }
+}
+
 // Rows' parts from all splits into the output: one wave a row.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32_t n) {
   const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= n) return;
+  if (W.ml[row].y < 0.0f) return;
   float m = NEG_INF;
-  for (uint32_t k = 0; k < W.splits; ++k) m = fmaxf(m, W.ml[(size_t)k * n + row].x);
+  for (uint32_t k = 0; k < W.slots; ++k) m = fmaxf(m, W.ml[(size_t)k * n + row].x);
   const float ref = m == NEG_INF ? 0.0f : m;
   float l = 0, x[(D + 63) / 64] = {};
-  for (uint32_t k = 0; k < W.splits; ++k) {
+  for (uint32_t k = 0; k < W.slots; ++k) {
     const float2 ml = W.ml[(size_t)k * n + row];
     if (ml.x == NEG_INF && ml.y == 0.0f) continue;
     const float f = exp2_fast(ml.x - ref);
@@ -416,31 +763,63 @@ __global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32
   if (A.lse && lane == 0) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
 }
 
+// Launch shapes of a call. FEW_ROWS: rows of a sequence and kv head up to which rows_kernel takes it.
+constexpr uint32_t FEW_ROWS = 32;
+
 struct Plan {
-  uint32_t row_tiles, splits;
+  Take rows_take, prompt_take;
+  uint32_t row_tiles, row_splits;        // rows_kernel; 0 tiles: not launched
+  uint32_t prompt_tiles, prompt_splits;  // prompt_kernel
+  uint32_t slots;
 };
 
+uint32_t split_for(uint64_t blocks, uint64_t want, uint64_t pages, uint64_t least) {
+  const uint64_t n = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(n, pages / least));
+}
+
 Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
-  const uint64_t group = n_q_heads / P->n_kv_heads;
-  const uint64_t tiles = std::min<uint64_t>(std::max<uint64_t>((B->max_new * group + 15) / 16, 1), 65535 / P->n_kv_heads);
-  const uint64_t blocks = tiles * P->n_kv_heads * B->n_seqs;
-  const uint64_t pages = (B->max_len + PAGE - 1) / PAGE;
-  uint64_t splits = blocks >= 1024 ? 1 : (1024 + blocks - 1) / blocks;
-  splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, pages / 8));
-  return {(uint32_t)tiles, (uint32_t)splits};
+  const uint64_t group = n_q_heads / P->n_kv_heads, heads = P->n_kv_heads;
+  const uint64_t rows = std::max<uint64_t>(B->max_new * group, 1), pages = (B->max_len + PAGE - 1) / PAGE;
+  Plan p = {ALL, ALL, 0, 1, 0, 1, 1};
+  if (rows > FEW_ROWS) {
+    p.prompt_tiles = (uint32_t)std::min<uint64_t>((rows + PROMPT_ROWS - 1) / PROMPT_ROWS, 65535);
+    // tiles that the sequences can have in all, if max_new is what it says
+    const uint64_t tiles = std::min<uint64_t>(p.prompt_tiles * (uint64_t)B->n_seqs, B->n_rows * group / PROMPT_ROWS + B->n_seqs);
+    p.prompt_splits = split_for(tiles * heads, 512, pages, 8);
+  }
+  if (rows <= FEW_ROWS || B->n_seqs > 1) {
+    const uint64_t most = std::min<uint64_t>(rows, FEW_ROWS);
+    p.row_tiles = (uint32_t)std::min<uint64_t>((most + 15) / 16, 65535 / heads);
+    p.row_splits = split_for(p.row_tiles * heads * B->n_seqs, 1024, pages, 8);
+  }
+  if (p.prompt_tiles && p.row_tiles) p.rows_take = FEW, p.prompt_take = MANY;
+  p.slots = std::max(p.row_splits, p.prompt_splits);
+  return p;
 }
 
 uint64_t split_rows(const bs_kv_batch* B, uint32_t n_q_heads, const Plan& p) {
-  return p.splits > 1 ? (uint64_t)p.splits * B->n_rows * n_q_heads : 0;
+  return p.slots > 1 ? (uint64_t)p.slots * B->n_rows * n_q_heads : 0;
 }
 
 template <int D, int KIND>
 int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
-  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.splits};
-  attend_kernel<D, KIND><<<dim3(p.splits, p.row_tiles * P->n_kv_heads, B->n_seqs), 64 * WAVES, 0, stream>>>(*P, *B, *Q, w, status);
-  if (p.splits > 1) {
+  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), 1, p.slots};
+  if (p.prompt_tiles) {
+    static std::atomic<uint64_t> done{0};
+    bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND>, 2 * Tile<D>::BYTES, done);
+    w.splits = p.prompt_splits;
+    prompt_kernel<D, KIND><<<dim3(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs), 256, 2 * Tile<D>::BYTES, stream>>>(
+        *P, *B, *Q, w, p.prompt_take, (int)FEW_ROWS, status);
+  }
+  if (p.row_tiles) {
+    w.splits = p.row_splits;
+    rows_kernel<D, KIND><<<dim3(p.row_splits, p.row_tiles * P->n_kv_heads, B->n_seqs), 64 * WAVES, 0, stream>>>(
+        *P, *B, *Q, w, p.rows_take, (int)FEW_ROWS, status);
+  }
+  if (p.slots > 1) {
     const uint32_t n = B->n_rows * Q->n_q_heads;
     join_kernel<D><<<(n + 3) / 4, 256, 0, stream>>>(*Q, w, n);
   }
