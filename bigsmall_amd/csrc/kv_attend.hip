@@ -144,18 +144,23 @@ struct State {
 // Scores of a page from its products: s[t][i] belongs to key j0 + 4 t + i (j0: the lane group's first).
 template <int D>
 __device__ __forceinline__ void scores(f32x4 (&s)[4], const Score& sc, float row_scale, float page_scale, float shift,
-                                       int j0, int2 see, bool inside, float slope, int pos) {
+                                       int j0, int2 see, bool inside, bool biased, float slope, int pos) {
   const float c = row_scale * (page_scale * sc.scale);
+  int lo = see.x - j0, hi = see.y - j0;
+  float d = (float)(pos - j0);
+  BS_OPAQUE(lo);
+  BS_OPAQUE(hi);
+  BS_OPAQUE(d);
 #pragma unroll
   for (int t = 0; t < 4; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float x = s[t][i] * c;
       if (sc.cap != 0.0f) x = capped(x, sc.cap);
-      const int j = j0 + 4 * t + i;
-      if (slope != 0.0f) x -= slope * fabsf((float)(pos - j));
+      const int j = 4 * t + i;
+      if (biased) x -= slope * fabsf(d - (float)j);
       x += shift;
-      if (!inside) x = (j >= see.x && j < see.y) ? x : NEG_INF;
+      if (!inside) x = (j >= lo && j < hi) ? x : NEG_INF;
       s[t][i] = x;
     }
 }
@@ -219,7 +224,8 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
   }
   const int rows = s.n * (int)group;
   if (!takes(take, rows, few)) return;
-  const Score sc = {A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E, A.softcap * LOG2E};
+  const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
+  const Score sc = {fabsf(A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E), A.softcap * LOG2E};
   const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
 
   for (int tile = blockIdx.y / P.n_kv_heads; tile * 16 < rows; tile += row_tiles) {
@@ -229,7 +235,8 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
     const uint32_t hq = h * group + (uint32_t)(real ? r % (int)group : 0);
     const int pos = s.start + i;
     const int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
-    const float slope = A.slopes ? A.slopes[hq] * LOG2E : 0.0f;
+    const bool biased = A.slopes != nullptr;
+    const float slope = biased ? A.slopes[hq] * LOG2E : 0.0f;
 
     // the row of q as f16, scaled by a power of two to lie below 2 (exact for what is within 2^-14 of the largest)
     const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
@@ -260,7 +267,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
 #pragma unroll
       for (int c = 0; c < STEPS; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)ldexpf(bf16_to_f32(x[c][e]), -e2) : (_Float16)0.0f;
+        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[c][e]), -e2)) : (_Float16)0.0f;
     }
 
     // pages that any row of the tile sees, cut into splits
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
       }
       const int j0 = page * (int)PAGE;
       const bool inside = __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
-      scores<D>(acc, sc, row_scale, ks, shift, j0 + 16 * g, see, inside, slope, pos);
+      scores<D>(acc, sc, row_scale, ks, shift, j0 + 16 * g, see, inside, biased, slope, pos);
       weights<D>(acc, st, exp2_fast(-shift));
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -339,7 +346,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
             acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, qb, acc[t], 0, 0, 0);
           }
         }
-        scores<D>(acc, sc, row_scale == row_scale ? 1.0f : row_scale, 1.0f, 0.0f, full_pages * (int)PAGE + 16 * g, see, false, slope, pos);
+        scores<D>(acc, sc, row_scale == row_scale ? sign : row_scale, 1.0f, 0.0f, full_pages * (int)PAGE + 16 * g, see, false, biased, slope, pos);
         weights<D>(acc, st, 1.0f);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -454,7 +461,7 @@ struct Staged {      // a thread's part of a page on its way to LDS
 #pragma unroll
     for (int i = 0; i < Tile<D>::LOADS; ++i) {
       const int at = (tid + 256 * i) * 16;
-      if (at < (int)PAGE * D) {
+      if (PAGE * D % 4096 == 0 || at < (int)PAGE * D) {
         k[i] = *(const uint4*)(kp + at);
         v[i] = *(const uint4*)(vp + at);
       }
@@ -464,7 +471,7 @@ struct Staged {      // a thread's part of a page on its way to LDS
 #pragma unroll
     for (int i = 0; i < Tile<D>::LOADS; ++i) {
       const int at = (tid + 256 * i) * 16;
-      if (at < (int)PAGE * D) {
+      if (PAGE * D % 4096 == 0 || at < (int)PAGE * D) {
         const int key = at / D, ch = at % D;
         const int row = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
         uint8_t* to = lds + row * Tile<D>::K_ROW + ch * 2;
@@ -478,33 +485,74 @@ struct Staged {      // a thread's part of a page on its way to LDS
   }
 };
 
-// Scores s of 64 keys (two S^T tiles) into weights; m, l and o move on. j0: the page's first key.
-// The maximum only moves when some row's has grown by more than 8 times, so that
-// o is rescaled a few times and not at every page; weights then reach 2^(P_SHIFT
-// + 3), inside f16.
-template <int D>
-__device__ __forceinline__ void prompt_softmax(f32x16 (&s)[2], f32x16 (&o)[Tile<D>::TILES], float& m, float& l, const Score& sc, float row_scale,
-                                               float page_scale, float shift, float inv_vs, int j0, int half, int2 see, bool plain,
-                                               bool inside, float slope, int pos) {
-  float c = row_scale * (page_scale * sc.scale), add = shift;
-  if (!(plain && inside)) {
+// N products whose left operands come from LDS, in groups of four: the next group's reads are under way while one
+// group is multiplied. Left alone the compiler waits for every read right before its product.
+template <int N, class Read, class Multiply>
+__device__ __forceinline__ void products(Read read, Multiply multiply) {
+  constexpr int G = 4;
+  half8v a[2][G];
+#pragma unroll
+  for (int i = 0; i < G && i < N; ++i) a[0][i] = read(i);
+#pragma unroll
+  for (int g = 0; g * G < N; ++g) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      if ((g + 1) * G + i < N) a[(g + 1) & 1][i] = read((g + 1) * G + i);
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      if (g * G + i < N) multiply(g * G + i, a[g & 1][i]);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Scores of 64 keys (two S^T tiles) as they come from the products, into what is left to multiply by c and add to:
+// caps, biases and masks where there are any. j0: this lane's first key.
+template <bool PLAIN>
+__device__ __forceinline__ void prompt_scores(f32x16 (&s)[2], float& c, const Score& sc, bool inside, int j0, int2 see, bool biased,
+                                              float slope, int pos) {
+  if constexpr (!PLAIN) {
+    if (sc.cap != 0.0f) {          // cap * tanh(x) = cap - 2 cap / (e^2x + 1): the quotient here, cap in the last step
+      const float k = c * (2.0f * LOG2E);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = __builtin_amdgcn_rcpf(-1.0f - exp2_fast(s[t][i] * k));
+      c = 2.0f * sc.cap;
+    }
+    if (biased) {
+      float d = (float)(pos - j0);
+      BS_OPAQUE(d);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = s[t][i] * c - slope * fabsf(d - (float)(32 * t + 16 * (i >> 3) + (i & 7)));
+      c = 1.0f;
+    }
+  }
+  if (!inside) {
+    // made here and nowhere earlier: left to itself the compiler keeps 64 bounds in registers through the whole loop
+    int lo = see.x - j0, hi = see.y - j0;
+    BS_OPAQUE(lo);
+    BS_OPAQUE(hi);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int j = j0 + 32 * t + 16 * (i >> 3) + 8 * half + (i & 7);
-        float x = s[t][i] * c;
-        if (sc.cap != 0.0f) x = capped(x, sc.cap);
-        if (slope != 0.0f) x -= slope * fabsf((float)(pos - j));
-        x += shift;
-        s[t][i] = (j >= see.x && j < see.y) ? x : NEG_INF;
+        const int j = 32 * t + 16 * (i >> 3) + (i & 7);
+        s[t][i] = (j >= lo && j < hi) ? s[t][i] * c : NEG_INF;
       }
     c = 1.0f;
-    add = 0.0f;
   }
-  float top = fmaxf(s[0][0], s[1][0]);
+}
+
+// Weights 2^(s c + add - m) from scores; m, l and o move on. The maximum only moves when some row's has grown by more
+// than 8 times, so that o is rescaled a few times and not at every page; weights then reach 2^(P_SHIFT + 3), inside f16.
+template <int D>
+__device__ __forceinline__ void prompt_weights(f32x16 (&s)[2], f32x16 (&o)[Tile<D>::TILES], float& m, float& l, float c, float add, float inv_vs) {
+  float top = NEG_INF;               // c is not negative: q carries the sign of the call's scale
 #pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
   top = pair_max(fmaf(top, c, add));
   if (__ballot(top > m + 3.0f)) {
     const float now = fmaxf(m, top);
@@ -515,18 +563,20 @@ __device__ __forceinline__ void prompt_softmax(f32x16 (&s)[2], f32x16 (&o)[Tile<
     for (int d = 0; d < Tile<D>::TILES; ++d) o[d] *= alpha;
   }
   const float base = add - ((m == NEG_INF ? 0.0f : m) - P_SHIFT);
-  float sum = 0;
+  float sum[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[t][i] = exp2_fast(fmaf(s[t][i], c, base));
-      sum += s[t][i];
+      sum[i & 3] += s[t][i];
     }
-  l += sum == 0.0f ? 0.0f : sum * inv_vs;
+  const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  l += all == 0.0f ? 0.0f : all * inv_vs;
 }
 
-template <int D, int KIND>
+// PLAIN: no cap, no bias.
+template <int D, int KIND, bool PLAIN>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
                                                                       int32_t* status) {
   constexpr int STEPS = Tile<D>::STEPS, TILES = Tile<D>::TILES;
@@ -542,8 +592,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
   }
   const int rows = s.n * (int)group;
   if (!takes(take, rows, few)) return;
-  const Score sc = {A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E, A.softcap * LOG2E};
-  const bool plain = A.softcap == 0.0f && !A.slopes && A.scale > 0.0f;
+  const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
+  const Score sc = {fabsf(A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E), A.softcap * LOG2E};
+  const bool biased = A.slopes != nullptr;
   const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
   const int full_pages = s.len / (int)PAGE, row_tiles = (rows + PROMPT_ROWS - 1) / PROMPT_ROWS;
 
@@ -555,7 +606,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
     const uint32_t hq = h * group + (uint32_t)(real ? r % (int)group : 0);
     const int pos = s.start + i;
     int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
-    const float slope = A.slopes ? A.slopes[hq] * LOG2E : 0.0f;
+    const float slope = !PLAIN && biased ? A.slopes[hq] * LOG2E : 0.0f;
 
     const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
     half8v q16[STEPS];
@@ -581,7 +632,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
 #pragma unroll
       for (int c = 0; c < STEPS; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)ldexpf(bf16_to_f32(x[c][e]), -e2) : (_Float16)0.0f;
+        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[c][e]), -e2)) : (_Float16)0.0f;
     }
 
     // keys that any row of the wave, and of the workgroup, sees
@@ -637,24 +688,24 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
       if (!ok || j0 >= wave_hi || j0 + (int)PAGE <= wave_lo) continue;
       f32x16 acc[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[t][e] = 0;
-        const uint8_t* row = buf + (32 * t + (lane & 31)) * Tile<D>::K_ROW + 16 * half;
-#pragma unroll
-        for (int c = 0; c < STEPS; ++c) acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(row + 32 * c), q16[c], acc[t], 0, 0, 0);
-      }
+      const uint8_t* kr = buf + (lane & 31) * Tile<D>::K_ROW + 16 * half;
+      products<2 * STEPS>([&](int n) { return *(const half8v*)(kr + n % 2 * 32 * Tile<D>::K_ROW + n / 2 * 32); },
+                          [&](int n, half8v a) { acc[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q16[n / 2], acc[n % 2], 0, 0, 0); });
       const bool inside = __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
-      prompt_softmax<D>(acc, o, m, l, sc, row_scale, ks, shift, exp2_fast(-shift), j0, half, see, plain, inside, slope, pos);
+      float c = row_scale * (ks * sc.scale);
+      prompt_scores<PLAIN>(acc, c, sc, inside, j0 + 8 * half, see, biased, slope, pos);
+      prompt_weights<D>(acc, o, m, l, c, shift + sc.cap, exp2_fast(-shift));
+      half8v p[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        half8v p;
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = (_Float16)acc[u >> 1][8 * (u & 1) + e];
-        const uint8_t* row = buf + Tile<D>::K_BYTES + (lane & 31) * Tile<D>::V_ROW + 32 * u + 16 * half;
-#pragma unroll
-        for (int d = 0; d < TILES; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8v*)(row + 32 * d * Tile<D>::V_ROW), p, o[d], 0, 0, 0);
-      }
+        for (int e = 0; e < 8; ++e) p[u][e] = (_Float16)acc[u >> 1][8 * (u & 1) + e];
+      const uint8_t* vr = buf + Tile<D>::K_BYTES + (lane & 31) * Tile<D>::V_ROW + 16 * half;
+      products<4 * TILES>([&](int n) { return *(const half8v*)(vr + n % TILES * 32 * Tile<D>::V_ROW + n / TILES * 32); },
+                          [&](int n, half8v a) { o[n % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[n / TILES], o[n % TILES], 0, 0, 0); });
     }
 
     // the tail, as in rows_kernel
@@ -683,8 +734,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
             acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb, qb, acc[t], 0, 0, 0);
           }
         }
-        prompt_softmax<D>(acc, o, m, l, sc, row_scale == row_scale ? 1.0f : row_scale, 1.0f, 0.0f, 1.0f, full_pages * (int)PAGE, half, see, plain,
-                          false, slope, pos);
+        if (sign < 0.0f)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) acc[t] = -acc[t];
+        float c = row_scale == row_scale ? sc.scale : row_scale;
+        prompt_scores<PLAIN>(acc, c, sc, false, full_pages * (int)PAGE + 8 * half, see, biased, slope, pos);
+        prompt_weights<D>(acc, o, m, l, c, sc.cap, 1.0f);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           bf16x8 p_hi, p_lo;
@@ -802,17 +857,24 @@ uint64_t split_rows(const bs_kv_batch* B, uint32_t n_q_heads, const Plan& p) {
   return p.slots > 1 ? (uint64_t)p.slots * B->n_rows * n_q_heads : 0;
 }
 
+template <int D, int KIND, bool PLAIN>
+void prompt_launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, const Work& w, Take take, int32_t* status,
+                   hipStream_t stream, dim3 grid) {
+  static std::atomic<uint64_t> done{0};
+  bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND, PLAIN>, 2 * Tile<D>::BYTES, done);
+  prompt_kernel<D, KIND, PLAIN><<<grid, 256, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, take, (int)FEW_ROWS, status);
+}
+
 template <int D, int KIND>
 int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
   Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), 1, p.slots};
   if (p.prompt_tiles) {
-    static std::atomic<uint64_t> done{0};
-    bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND>, 2 * Tile<D>::BYTES, done);
     w.splits = p.prompt_splits;
-    prompt_kernel<D, KIND><<<dim3(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs), 256, 2 * Tile<D>::BYTES, stream>>>(
-        *P, *B, *Q, w, p.prompt_take, (int)FEW_ROWS, status);
+    const dim3 grid(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs);
+    if (Q->softcap == 0.0f && !Q->slopes) prompt_launch<D, KIND, true>(P, B, Q, w, p.prompt_take, status, stream, grid);
+    else prompt_launch<D, KIND, false>(P, B, Q, w, p.prompt_take, status, stream, grid);
   }
   if (p.row_tiles) {
     w.splits = p.row_splits;
