@@ -290,7 +290,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
     st.l = 0;
 
     for (int page = mine + wave; page < min(end, full_pages); page += WAVES) {
-      const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(B.table[(size_t)b * B.table_stride + page]);
+      const uint32_t id = (uint32_t)uniform_load(B.table, (size_t)b * B.table_stride + page);
       if (id >= P.n_pages) {
         if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
         continue;
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
       PageV<D, KIND> v;
       k.load((const uint8_t*)P.k + id * unit + head, lane);
       v.load((const uint8_t*)P.v + id * unit + head, lane);
-      const float ks = P.k_scale[(size_t)id * P.n_kv_heads + h], vs = P.v_scale[(size_t)id * P.n_kv_heads + h];
+      const float ks = uniform_load(P.k_scale, (size_t)id * P.n_kv_heads + h), vs = uniform_load(P.v_scale, (size_t)id * P.n_kv_heads + h);
       const float shift = __builtin_amdgcn_logf(vs);
       f32x4 acc[4];
 #pragma unroll
@@ -324,7 +324,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
 
     // the tail: bf16 as it is; p' in two bf16 parts keeps 16 bits of it. Slots after the sequence's end hold anything.
     if (mine < end && end > full_pages && wave == (end - 1 - mine) % WAVES) {
-      const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(B.tails[2 * b + 1]);
+      const uint32_t id = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
       if (id >= P.n_tails) {
         if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
       } else {
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
 // right operand of two products with V^T: key bits 2 and 3 change places
 // between a tile's row and the key in it. LDS rows have an odd number of 16-byte
 // pieces, so that the 8 lanes of one LDS cycle hit different banks.
-constexpr int PROMPT_ROWS = 128;
+constexpr int PROMPT_WAVES = 4, PROMPT_ROWS = 32 * PROMPT_WAVES, PROMPT_THREADS = 64 * PROMPT_WAVES;
 
 // The maximum of x over the two lanes that share a row (32 apart).
 __device__ __forceinline__ float pair_max(float x) {
@@ -451,7 +451,7 @@ struct Tile {
   static constexpr int V_ROW = PAGE * 2 + 16;
   static constexpr int K_BYTES = PAGE * K_ROW, V_BYTES = TILES * 32 * V_ROW;
   static constexpr int BYTES = K_BYTES + V_BYTES;
-  static constexpr int LOADS = (PAGE * D / 16 + 255) / 256;   // 16-byte loads of a thread, for K and for V
+  static constexpr int LOADS = (PAGE * D / 16 + PROMPT_THREADS - 1) / PROMPT_THREADS;   // 16-byte loads of a thread, for K and for V
 };
 
 template <int D, int KIND>
@@ -460,8 +460,8 @@ struct Staged {      // a thread's part of a page on its way to LDS
   __device__ __forceinline__ void load(const uint8_t* kp, const uint8_t* vp, int tid) {
 #pragma unroll
     for (int i = 0; i < Tile<D>::LOADS; ++i) {
-      const int at = (tid + 256 * i) * 16;
-      if (PAGE * D % 4096 == 0 || at < (int)PAGE * D) {
+      const int at = (tid + PROMPT_THREADS * i) * 16;
+      if (PAGE * D % (16 * PROMPT_THREADS) == 0 || at < (int)PAGE * D) {
         k[i] = *(const uint4*)(kp + at);
         v[i] = *(const uint4*)(vp + at);
       }
@@ -470,8 +470,8 @@ struct Staged {      // a thread's part of a page on its way to LDS
   __device__ __forceinline__ void store(uint8_t* lds, int tid) const {
 #pragma unroll
     for (int i = 0; i < Tile<D>::LOADS; ++i) {
-      const int at = (tid + 256 * i) * 16;
-      if (PAGE * D % 4096 == 0 || at < (int)PAGE * D) {
+      const int at = (tid + PROMPT_THREADS * i) * 16;
+      if (PAGE * D % (16 * PROMPT_THREADS) == 0 || at < (int)PAGE * D) {
         const int key = at / D, ch = at % D;
         const int row = (key & 0x33) | ((key & 4) << 1) | ((key & 8) >> 1);
         uint8_t* to = lds + row * Tile<D>::K_ROW + ch * 2;
@@ -546,29 +546,42 @@ __device__ __forceinline__ void prompt_scores(f32x16 (&s)[2], float& c, const Sc
   }
 }
 
-// Weights 2^(s c + add - m) from scores; m, l and o move on. The maximum only moves when some row's has grown by more
-// than 8 times, so that o is rescaled a few times and not at every page; weights then reach 2^(P_SHIFT + 3), inside f16.
+// Weights 2^(s c + add - m + SHIFT) from scores; m, l and o move on. The exponents are made with the maximum of the
+// pages before, and only if some row's largest is over 2^SLACK times that (or the row had seen nothing) does the
+// maximum move and o get rescaled: hardly ever. Weights then reach 2^(SHIFT + SLACK), inside f16, and those down to
+// 2^-(SHIFT + 14) of the largest keep all 11 bits.
+constexpr float SLACK = 8.0f, SHIFT = 7.0f;
 template <int D>
 __device__ __forceinline__ void prompt_weights(f32x16 (&s)[2], f32x16 (&o)[Tile<D>::TILES], float& m, float& l, float c, float add, float inv_vs) {
-  float top = NEG_INF;               // c is not negative: q carries the sign of the call's scale
+  const float base = add + SHIFT - (m == NEG_INF ? 0.0f : m);
+  float top = NEG_INF;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[t][i] = fmaf(s[t][i], c, base);
 #pragma unroll
   for (int i = 0; i < 16; ++i) top = fmaxf(top, fmaxf(s[0][i], s[1][i]));
-  top = pair_max(fmaf(top, c, add));
-  if (__ballot(top > m + 3.0f)) {
-    const float now = fmaxf(m, top);
+  top = pair_max(top);
+  if (__ballot(top > (m == NEG_INF ? NEG_INF : SHIFT + SLACK))) {
+    const float was = m == NEG_INF ? 0.0f : m, grown = top - SHIFT + was;      // the row's largest score
+    const float now = fmaxf(m, grown);
     const float alpha = exp2_fast(m - (now == NEG_INF ? 0.0f : now));
+    const float down = was - (now == NEG_INF ? 0.0f : now);
     m = now;
     l *= alpha;
 #pragma unroll
     for (int d = 0; d < Tile<D>::TILES; ++d) o[d] *= alpha;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] += down;
   }
-  const float base = add - ((m == NEG_INF ? 0.0f : m) - P_SHIFT);
   float sum[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[t][i] = exp2_fast(fmaf(s[t][i], c, base));
+      s[t][i] = exp2_fast(s[t][i]);
       sum[i & 3] += s[t][i];
     }
   const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -577,11 +590,11 @@ __device__ __forceinline__ void prompt_weights(f32x16 (&s)[2], f32x16 (&o)[Tile<
 
 // PLAIN: no cap, no bias.
 template <int D, int KIND, bool PLAIN>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
+__global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
                                                                       int32_t* status) {
   constexpr int STEPS = Tile<D>::STEPS, TILES = Tile<D>::TILES;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-  __shared__ int bounds[2][4];
+  __shared__ int bounds[2][PROMPT_WAVES];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const uint32_t h = blockIdx.x % P.n_kv_heads, split = blockIdx.x / P.n_kv_heads, b = blockIdx.z;
   const uint32_t group = A.n_q_heads / P.n_kv_heads;
@@ -643,11 +656,11 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
       hi = max(hi, __shfl_xor(hi, d));
     }
     const int wave_lo = __builtin_amdgcn_readfirstlane(lo), wave_hi = __builtin_amdgcn_readfirstlane(hi);
-    __syncthreads();
+    lds_barrier();
     if (lane == 0) bounds[0][wave] = lo, bounds[1][wave] = hi;
-    __syncthreads();
-    lo = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
-    hi = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    lds_barrier();
+#pragma unroll
+    for (int w = 0; w < PROMPT_WAVES; ++w) lo = min(lo, bounds[0][w]), hi = max(hi, bounds[1][w]);
     const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
     const int per = (page_hi - page_lo + (int)W.splits - 1) / (int)W.splits;
     const int begin = __builtin_amdgcn_readfirstlane(page_lo + per * (int)split);
@@ -661,29 +674,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
       for (int e = 0; e < 16; ++e) o[d][e] = 0;
     float m = NEG_INF, l = 0;
 
+    // Page numbers and scales come through vector loads, in line with the pages' own: number n is asked for with page
+    // n - 1, scales with their page, so that nothing waits for them. Past the end: the last page again.
     const int32_t* table = B.table + (size_t)b * B.table_stride;
+    int zero = 0;
+    BS_OPAQUE(zero);                          // (an index of the lanes' own keeps the loads out of the scalar cache)
+    const auto number = [&](int page) { return table[min(page, full_end - 1) + zero]; };
     Staged<D, KIND> st;
-    bool next_ok = false;
+    uint32_t id = 0;
+    int coming = 0;
     float next_ks = 0, next_vs = 1;
     const auto fetch = [&](int page) {
-      uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(table[page]);
-      next_ok = id < P.n_pages;
-      if (!next_ok) {
-        if (tid == 0) report(status, BS_DEV_ERR_BOUNDS);
-        id = 0;
-      }
-      st.load((const uint8_t*)P.k + id * unit + head, (const uint8_t*)P.v + id * unit + head, tid);
-      next_ks = P.k_scale[(size_t)id * P.n_kv_heads + h];
-      next_vs = P.v_scale[(size_t)id * P.n_kv_heads + h];
+      id = (uint32_t)__builtin_amdgcn_readfirstlane(coming);
+      const uint32_t real_id = id < P.n_pages ? id : 0;
+      next_ks = P.k_scale[(size_t)real_id * P.n_kv_heads + h + zero];
+      next_vs = P.v_scale[(size_t)real_id * P.n_kv_heads + h + zero];
+      coming = number(page + 1);
+      st.load((const uint8_t*)P.k + real_id * unit + head, (const uint8_t*)P.v + real_id * unit + head, tid);
     };
-    if (begin < full_end) fetch(begin);
+    if (begin < full_end) {
+      coming = number(begin);
+      fetch(begin);
+    }
     for (int page = begin; page < full_end; ++page) {
       uint8_t* buf = lds + ((page - begin) & 1) * Tile<D>::BYTES;
       st.store(buf, tid);
-      const bool ok = next_ok;
+      const bool ok = id < P.n_pages;
+      if (!ok && tid == 0) report(status, BS_DEV_ERR_BOUNDS);
       const float ks = next_ks, shift = __builtin_amdgcn_logf(next_vs);
-      if (page + 1 < full_end) fetch(page + 1);
-      __syncthreads();
+      fetch(page + 1);
+      lds_barrier();
       const int j0 = page * (int)PAGE;
       if (!ok || j0 >= wave_hi || j0 + (int)PAGE <= wave_lo) continue;
       f32x16 acc[2];
@@ -710,7 +730,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
 
     // the tail, as in rows_kernel
     if (begin < end && end > full_pages && full_pages * (int)PAGE < wave_hi) {
-      const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(B.tails[2 * b + 1]);
+      const uint32_t id = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
       if (id >= P.n_tails) {
         if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
       } else {
@@ -767,7 +787,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void prompt_kernel(bs_kv_poo
     l = pair_sum(l);
     if (real) {
       const size_t out_row = (size_t)(s.t0 + i) * A.n_q_heads + hq;
-      if (half == 0) mark_row(A, B, W, split, out_row, m, l);
+      if (half == 0) mark_row(A, B, W, split, out_row, m + (P_SHIFT - SHIFT), l);
       if (W.splits == 1 || begin < end) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         float* part = W.o + ((size_t)split * B.n_rows * A.n_q_heads + out_row) * D;
@@ -862,7 +882,7 @@ void prompt_launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query*
                    hipStream_t stream, dim3 grid) {
   static std::atomic<uint64_t> done{0};
   bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND, PLAIN>, 2 * Tile<D>::BYTES, done);
-  prompt_kernel<D, KIND, PLAIN><<<grid, 256, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, take, (int)FEW_ROWS, status);
+  prompt_kernel<D, KIND, PLAIN><<<grid, PROMPT_THREADS, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, take, (int)FEW_ROWS, status);
 }
 
 template <int D, int KIND>

@@ -2,10 +2,10 @@
 // stored 8-bit types, f16 and bf16, wave reductions, and a step's bounds.
 #pragma once
 
-#include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "bigsmall_kv.h"
+#include "simt.h"
 
 namespace bs_kv {
 
@@ -52,10 +52,24 @@ __device__ __forceinline__ half8v codes8_to_f16(uint32_t w0, uint32_t w1) {
   return half8v{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// A workgroup barrier for LDS only: loads from memory that are under way stay so (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
   return x;
+}
+
+// p[i] of an array that no kernel of the call writes, at an index that is the same in all lanes: a load through the
+// scalar cache, which does not stand in line with the vector loads under way.
+template <class T>
+__device__ __forceinline__ T uniform_load(const T* p, size_t i) {
+  return ((const CST T*)(uintptr_t)p)[i];
 }
 
 // The bounds of sequence b in a step, held to what the batch's arrays can hold;
