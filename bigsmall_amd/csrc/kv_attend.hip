@@ -56,6 +56,7 @@ struct Work {
   float* o;
   float2* ml;
   uint32_t splits, slots;
+  int piece;           // rows_kernel: pages of a split
 };
 
 // Which sequences a kernel takes: those with few rows, with many, or all.
@@ -207,14 +208,39 @@ __device__ __forceinline__ void mark_row(const bs_kv_query& A, const bs_kv_batch
 
 constexpr int WAVES = 4;
 
+// 64 of a wave's pages at a time, one a lane: number (or ~0: no such page) and scales.
+struct PageList {
+  uint32_t id;
+  float ks, vs;
+  __device__ __forceinline__ void load(const bs_kv_pool& P, const int32_t* table, uint32_t h, int page, int end, int32_t* status) {
+    id = ~0u;
+    ks = vs = 0.0f;
+    if (page >= end) return;
+    id = (uint32_t)table[page];
+    if (id >= P.n_pages) {
+      report(status, BS_DEV_ERR_BOUNDS);
+      id = ~0u;
+      return;
+    }
+    ks = P.k_scale[(size_t)id * P.n_kv_heads + h];
+    vs = P.v_scale[(size_t)id * P.n_kv_heads + h];
+  }
+  __device__ __forceinline__ uint32_t number(int i) const { return (uint32_t)__builtin_amdgcn_readlane((int)id, i); }
+  __device__ __forceinline__ float scale_k(int i) const { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(ks), i)); }
+  __device__ __forceinline__ float scale_v(int i) const { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(vs), i)); }
+};
+
+// A split's pages are dealt to the four waves in turn. A wave reads the next page's K as soon as this one's is
+// multiplied, and its V after this one's: between 8 and 16 KiB a wave are always under way (heads of 128).
 template <int D, int KIND>
-__global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few, int32_t* status) {
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few, int32_t* status) {
   constexpr int STEPS = Dims<D>::STEPS, TILES = Dims<D>::TILES;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  constexpr int PART = D < 128 ? D : 128, PARTS = D / PART;      // channels joined at a time
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const uint32_t h = blockIdx.y % P.n_kv_heads, b = blockIdx.z;
   const uint32_t group = A.n_q_heads / P.n_kv_heads;
   const uint32_t row_tiles = gridDim.y / P.n_kv_heads;
-  __shared__ float part_o[WAVES][16][17];
+  __shared__ __attribute__((aligned(16))) float part_o[WAVES][16][PART + 4];
   __shared__ float part_m[WAVES][16], part_l[WAVES][16];
 
   SeqStep s;
@@ -226,7 +252,9 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
   if (!takes(take, rows, few)) return;
   const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
   const Score sc = {fabsf(A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E), A.softcap * LOG2E};
+  const bool biased = A.slopes != nullptr;
   const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
+  const int32_t* table = B.table + (size_t)b * B.table_stride;
 
   for (int tile = blockIdx.y / P.n_kv_heads; tile * 16 < rows; tile += row_tiles) {
     const int r = tile * 16 + (lane & 15);
@@ -235,9 +263,25 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
     const uint32_t hq = h * group + (uint32_t)(real ? r % (int)group : 0);
     const int pos = s.start + i;
     const int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
-    const bool biased = A.slopes != nullptr;
-    const float slope = biased ? A.slopes[hq] * LOG2E : 0.0f;
 
+    // pages that any row of the tile sees, cut into splits
+    int lo = see.x < see.y ? see.x : 0x7FFFFFFF, hi = see.x < see.y ? see.y : 0;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      lo = min(lo, __shfl_xor(lo, d));
+      hi = max(hi, __shfl_xor(hi, d));
+    }
+    const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
+    // pieces of one size for all sequences, so that long ones do not make long pieces
+    const int first = page_lo + W.piece * (int)blockIdx.x;
+    const int mine = __builtin_amdgcn_readfirstlane(first);
+    const int end = __builtin_amdgcn_readfirstlane(blockIdx.x + 1 == W.splits ? page_hi : min(first + W.piece, page_hi));
+    const int full_pages = s.len / (int)PAGE, full_end = min(end, full_pages);      // pages from full_pages on are the tail
+
+    PageList list;
+    list.load(P, table, h, mine + wave + WAVES * lane, full_end, status);
+
+    const float slope = biased ? A.slopes[hq] * LOG2E : 0.0f;
     // the row of q as f16, scaled by a power of two to lie below 2 (exact for what is within 2^-14 of the largest)
     const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
     half8v q16[STEPS];
@@ -270,55 +314,53 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
         for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[c][e]), -e2)) : (_Float16)0.0f;
     }
 
-    // pages that any row of the tile sees, cut into splits
-    int lo = real ? see.x : 0x7FFFFFFF, hi = see.y;
-    if (real && see.x >= see.y) lo = 0x7FFFFFFF, hi = 0;
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
-      lo = min(lo, __shfl_xor(lo, d));
-      hi = max(hi, __shfl_xor(hi, d));
-    }
-    const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
-    const int per = (page_hi - page_lo + (int)W.splits - 1) / (int)W.splits;
-    const int mine = page_lo + per * (int)blockIdx.x, end = min(mine + per, page_hi);
-    const int full_pages = s.len / (int)PAGE;      // pages from here on are the tail
-
     State<D> st;
 #pragma unroll
     for (int d = 0; d < TILES; ++d) st.o[d] = f32x4{0, 0, 0, 0};
     st.m = NEG_INF;
     st.l = 0;
 
-    for (int page = mine + wave; page < min(end, full_pages); page += WAVES) {
-      const uint32_t id = (uint32_t)uniform_load(B.table, (size_t)b * B.table_stride + page);
-      if (id >= P.n_pages) {
-        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
-        continue;
-      }
+    if (mine + wave < full_end) {
+      const uint8_t *const kp = (const uint8_t*)P.k + head, *const vp = (const uint8_t*)P.v + head;
       PageK<D, KIND> k;
       PageV<D, KIND> v;
-      k.load((const uint8_t*)P.k + id * unit + head, lane);
-      v.load((const uint8_t*)P.v + id * unit + head, lane);
-      const float ks = uniform_load(P.k_scale, (size_t)id * P.n_kv_heads + h), vs = uniform_load(P.v_scale, (size_t)id * P.n_kv_heads + h);
-      const float shift = __builtin_amdgcn_logf(vs);
-      f32x4 acc[4];
+      uint32_t id = list.number(0);
+      k.load(kp + (id == ~0u ? 0 : id * unit), lane);
+      v.load(vp + (id == ~0u ? 0 : id * unit), lane);
+      int at = 0;                       // place in the list
+      for (int page = mine + wave; page < full_end; page += WAVES) {
+        const bool ok = id != ~0u;
+        const float ks = list.scale_k(at), shift = __builtin_amdgcn_logf(list.scale_v(at));
+        f32x4 acc[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        acc[t] = f32x4{0, 0, 0, 0};
+        for (int t = 0; t < 4; ++t) {
+          acc[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int c = 0; c < STEPS; ++c) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.operand(t, c), q16[c], acc[t], 0, 0, 0);
-      }
-      const int j0 = page * (int)PAGE;
-      const bool inside = __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
-      scores<D>(acc, sc, row_scale, ks, shift, j0 + 16 * g, see, inside, biased, slope, pos);
-      weights<D>(acc, st, exp2_fast(-shift));
+          for (int c = 0; c < STEPS; ++c) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.operand(t, c), q16[c], acc[t], 0, 0, 0);
+        }
+        // the next page (past the end: this one again)
+        if (page + WAVES < full_end) {
+          if (++at == 64) {
+            at = 0;
+            list.load(P, table, h, page + WAVES + WAVES * lane, full_end, status);
+          }
+          id = list.number(at);
+        }
+        const size_t next = id == ~0u ? 0 : id * unit;
+        k.load(kp + next, lane);
+        const int j0 = page * (int)PAGE;
+        const bool inside = ok && __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
+        scores<D>(acc, sc, row_scale, ks, shift, j0 + 16 * g, ok ? see : make_int2(0, 0), inside, biased, slope, pos);
+        weights<D>(acc, st, exp2_fast(-shift));
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        half8v p;
+        for (int u = 0; u < 2; ++u) {
+          half8v p;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = (_Float16)acc[2 * u + e / 4][e % 4];
+          for (int e = 0; e < 8; ++e) p[e] = (_Float16)acc[2 * u + e / 4][e % 4];
 #pragma unroll
-        for (int d = 0; d < TILES; ++d) st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.operand(d, u), p, st.o[d], 0, 0, 0);
+          for (int d = 0; d < TILES; ++d) st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.operand(d, u), p, st.o[d], 0, 0, 0);
+        }
+        v.load(vp + next, lane);
       }
     }
 
@@ -360,14 +402,10 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
           const int key = 16 * g + 8 * u;
 #pragma unroll
           for (int d = 0; d < TILES; ++d) {
-            uint16_t x[8];
-            const uint4 w = *(const uint4*)(vt + (16 * d + (lane & 15)) * PAGE + key);
-            __builtin_memcpy(x, &w, 16);
+            bf16x8 vb = __builtin_bit_cast(bf16x8, *(const uint4*)(vt + (16 * d + (lane & 15)) * PAGE + key));
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              if (key + e >= used) x[e] = 0;
-            bf16x8 vb;
-            __builtin_memcpy(&vb, x, 16);
+              if (key + e >= used) vb[e] = (__bf16)0.0f;
             st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_hi, st.o[d], 0, 0, 0);
             st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_lo, st.o[d], 0, 0, 0);
           }
@@ -375,52 +413,50 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(bs_kv_pool P, bs_kv_ba
       }
     }
 
-    // join the waves: rows' m and l first, then O in pieces of 16 channels
+    // join the waves: rows' m and l, then O. A thread has eight channels of row tid / 16.
     st.l += __shfl_xor(st.l, 16);
     st.l += __shfl_xor(st.l, 32);
     __syncthreads();
     if (lane < 16) part_m[wave][lane] = st.m, part_l[wave][lane] = st.l;
-    __syncthreads();
-    float m = NEG_INF;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, part_m[w][lane & 15]);
-    const float ref = m == NEG_INF ? 0.0f : m;
-    const float mine_scale = exp2_fast(st.m - ref);
-    // this thread's part of a piece: row tid / 16, channel tid % 16
-    const int wr = (int)threadIdx.x >> 4, wc = (int)threadIdx.x & 15;
-    const int wrow = tile * 16 + wr;
-    float row_l = 0, row_m = NEG_INF;
-    {
-      float ws = 0;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) row_m = fmaxf(row_m, part_m[w][wr]);
-      const float rr = row_m == NEG_INF ? 0.0f : row_m;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) ws += part_l[w][wr] * exp2_fast(part_m[w][wr] - rr);
-      row_l = ws;
-    }
-    const float inv = row_l == 0.0f ? 0.0f : 1.0f / row_l;
+    const int wr = (int)threadIdx.x >> 4, wc = (int)threadIdx.x & 15, wrow = tile * 16 + wr;
     const size_t out_row = (size_t)(s.t0 + (wrow < rows ? wrow / (int)group : 0)) * A.n_q_heads + h * group + (uint32_t)(wrow < rows ? wrow % (int)group : 0);
     const size_t split_row = (size_t)blockIdx.x * B.n_rows * A.n_q_heads + out_row;
-    if (wrow < rows && wc == 0) mark_row(A, B, W, blockIdx.x, out_row, row_m, row_l);
-    if (W.splits > 1 && mine >= end) continue;      // nothing here: the joining kernel sees m = -inf and reads no O
 #pragma unroll
-    for (int d = 0; d < TILES; ++d) {
+    for (int part = 0; part < PARTS; ++part) {
+      if (part) __syncthreads();
+#pragma unroll
+      for (int d = 0; d < PART / 16; ++d) *(f32x4*)&part_o[wave][lane & 15][16 * d + 4 * g] = st.o[part * (PART / 16) + d];
       __syncthreads();
+      float m = NEG_INF, l = 0, f[WAVES];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part_o[wave][lane & 15][4 * g + e] = st.o[d][e] * mine_scale;
-      __syncthreads();
-      float x = 0;
+      for (int w = 0; w < WAVES; ++w) m = fmaxf(m, part_m[w][wr]);
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) x += part_o[w][wr][wc];
-      if (wrow < rows) {
-        if (W.splits > 1) W.o[split_row * D + 16 * d + wc] = x;
-        else A.out[out_row * D + 16 * d + wc] = f32_to_bf16(x * inv);
+      for (int w = 0; w < WAVES; ++w) {
+        f[w] = exp2_fast(part_m[w][wr] - (m == NEG_INF ? 0.0f : m));
+        l += part_l[w][wr] * f[w];
+      }
+      if (wrow >= rows) continue;
+      if (part == 0 && wc == 0) mark_row(A, B, W, blockIdx.x, out_row, m, l);
+      if ((W.splits > 1 && mine >= end) || 8 * wc >= PART) continue;    // nothing here: the joining kernel reads no O
+      float x[8] = {};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += part_o[w][wr][8 * wc + e] * f[w];
+      if (W.splits > 1) {
+        float* to = W.o + split_row * D + part * PART + 8 * wc;
+        *(float4*)to = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+      } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint32_t y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = f32_to_bf16(x[2 * e] * inv) | ((uint32_t)f32_to_bf16(x[2 * e + 1] * inv) << 16);
+        *(uint4*)(A.out + out_row * D + part * PART + 8 * wc) = make_uint4(y[0], y[1], y[2], y[3]);
       }
     }
   }
 }
-
 
 // Many rows: a workgroup of four waves takes 128 rows of a sequence and kv head,
 // 32 a wave, and goes through their pages together. Each page is converted to
@@ -811,35 +847,81 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
   }
 }
 
-// Rows' parts from all splits into the output: one wave a row.
-template <int D>
-__global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32_t n) {
-  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= n) return;
-  if (W.ml[row].y < 0.0f) return;
-  float m = NEG_INF;
-  for (uint32_t k = 0; k < W.slots; ++k) m = fmaxf(m, W.ml[(size_t)k * n + row].x);
-  const float ref = m == NEG_INF ? 0.0f : m;
-  float l = 0, x[(D + 63) / 64] = {};
-  for (uint32_t k = 0; k < W.slots; ++k) {
-    const float2 ml = W.ml[(size_t)k * n + row];
-    if (ml.x == NEG_INF && ml.y == 0.0f) continue;
-    const float f = exp2_fast(ml.x - ref);
-    l += ml.y * f;
-    const float* o = W.o + ((size_t)k * n + row) * D;
+// Rows' parts from all splits into the output, WAVES_A_ROW waves (1 or 4) a row: they deal the slots among them, 64 at a
+// time; lane k looks at its wave's slot k, then all lanes add up the slots that hold something. few > 0: only the rows
+// of sequences with at most that many rows a kv head are split (blockIdx.y: the sequence).
+template <int D, int WAVES_A_ROW>
+__global__ __launch_bounds__(256) void join_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, int few) {
+  constexpr int EACH = (D + 63) / 64, AT_ONCE = 8;
+  __shared__ float part_x[4][EACH * 64], part_m[4], part_l[4];
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = B.n_rows * A.n_q_heads;
+  const uint32_t share = WAVES_A_ROW == 4 ? wave : 0;
+  uint32_t row = WAVES_A_ROW == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
+  if (few) {
+    SeqStep s;
+    if (!seq_step(B, blockIdx.y, s) || s.n * (int)(A.n_q_heads / P.n_kv_heads) > few || row >= (uint32_t)s.n * A.n_q_heads) return;
+    row += (uint32_t)s.t0 * A.n_q_heads;
+  }
+  if (row >= n || W.ml[row].y < 0.0f) return;            // none, or written by its kernel
+  float m = NEG_INF, l = 0, x[EACH] = {};
+  for (uint32_t k0 = 0; k0 < W.slots; k0 += 64 * WAVES_A_ROW) {
+    const uint32_t mine = k0 + lane * WAVES_A_ROW + share;
+    float2 ml = make_float2(NEG_INF, 0.0f);
+    if (mine < W.slots) ml = W.ml[(size_t)mine * n + row];
+    const float now = fmaxf(m, wave_max(ml.x)), ref = now == NEG_INF ? 0.0f : now;
+    const float back = exp2_fast(m - ref), f = exp2_fast(ml.x - ref);
+    m = now;
+    l = l * back + ml.y * f;                             // (of this lane's slots)
 #pragma unroll
-    for (int c = 0; c < (D + 63) / 64; ++c)
-      if ((int)lane + 64 * c < D) x[c] += o[lane + 64 * c] * f;
+    for (int c = 0; c < EACH; ++c) x[c] *= back;
+    uint64_t some = __ballot(!(ml.x == NEG_INF && ml.y == 0.0f));
+    while (some) {
+      float fk[AT_ONCE], o[AT_ONCE][EACH];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const bool any = some != 0;
+        const int k = any ? __builtin_ctzll(some) : 0;
+        some &= some - 1;
+        fk[u] = any ? __shfl(f, k) : 0.0f;
+        const float* from = W.o + ((size_t)(k0 + (uint32_t)k * WAVES_A_ROW + share) * n + row) * D;
+#pragma unroll
+        for (int c = 0; c < EACH; ++c) o[u][c] = any && (int)lane + 64 * c < D ? from[lane + 64 * c] : 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+        for (int c = 0; c < EACH; ++c) x[c] += o[u][c] * fk[u];
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+  if constexpr (WAVES_A_ROW == 4) {
+#pragma unroll
+    for (int c = 0; c < EACH; ++c) part_x[wave][lane + 64 * c] = x[c];
+    if (lane == 0) part_m[wave] = m, part_l[wave] = l;
+    __syncthreads();
+    if (wave) return;
+    m = fmaxf(fmaxf(part_m[0], part_m[1]), fmaxf(part_m[2], part_m[3]));
+    l = 0;
+#pragma unroll
+    for (int c = 0; c < EACH; ++c) x[c] = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2_fast(part_m[w] - (m == NEG_INF ? 0.0f : m));
+      l += part_l[w] * f;
+#pragma unroll
+      for (int c = 0; c < EACH; ++c) x[c] += part_x[w][lane + 64 * c] * f;
+    }
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-  for (int c = 0; c < (D + 63) / 64; ++c)
+  for (int c = 0; c < EACH; ++c)
     if ((int)lane + 64 * c < D) A.out[(size_t)row * D + lane + 64 * c] = f32_to_bf16(x[c] * inv);
   if (A.lse && lane == 0) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // Launch shapes of a call. FEW_ROWS: rows of a sequence and kv head up to which rows_kernel takes it.
-constexpr uint32_t FEW_ROWS = 32;
+constexpr uint32_t FEW_ROWS = 16;
 
 struct Plan {
   Take rows_take, prompt_take;
@@ -866,7 +948,7 @@ Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
   if (rows <= FEW_ROWS || B->n_seqs > 1) {
     const uint64_t most = std::min<uint64_t>(rows, FEW_ROWS);
     p.row_tiles = (uint32_t)std::min<uint64_t>((most + 15) / 16, 65535 / heads);
-    p.row_splits = split_for(p.row_tiles * heads * B->n_seqs, 1024, pages, 8);
+    p.row_splits = split_for(p.row_tiles * heads * B->n_seqs, 1024, pages, WAVES);
   }
   if (p.prompt_tiles && p.row_tiles) p.rows_take = FEW, p.prompt_take = MANY;
   p.slots = std::max(p.row_splits, p.prompt_splits);
@@ -889,7 +971,7 @@ template <int D, int KIND>
 int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
-  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), 1, p.slots};
+  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), 1, p.slots, 0};
   if (p.prompt_tiles) {
     w.splits = p.prompt_splits;
     const dim3 grid(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs);
@@ -898,12 +980,17 @@ int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void
   }
   if (p.row_tiles) {
     w.splits = p.row_splits;
+    w.piece = (int)std::max<uint64_t>((((uint64_t)B->max_len + PAGE - 1) / PAGE + p.row_splits - 1) / p.row_splits, 1);
     rows_kernel<D, KIND><<<dim3(p.row_splits, p.row_tiles * P->n_kv_heads, B->n_seqs), 64 * WAVES, 0, stream>>>(
         *P, *B, *Q, w, p.rows_take, (int)FEW_ROWS, status);
   }
   if (p.slots > 1) {
-    const uint32_t n = B->n_rows * Q->n_q_heads;
-    join_kernel<D><<<(n + 3) / 4, 256, 0, stream>>>(*Q, w, n);
+    // where only short sequences are split, only their rows are looked at
+    const int few = p.rows_take == FEW && p.prompt_splits == 1 ? (int)FEW_ROWS : 0;
+    const uint32_t n = few ? FEW_ROWS * P->n_kv_heads : B->n_rows * Q->n_q_heads, seqs = few ? B->n_seqs : 1;
+    // Four waves a row from 8 slots on (64 rows of 64 slots: 6 us against 13 with one).
+    if (p.slots > 8) join_kernel<D, 4><<<dim3(n, seqs), 256, 0, stream>>>(*P, *B, *Q, w, few);
+    else join_kernel<D, 1><<<dim3((n + 3) / 4, seqs), 256, 0, stream>>>(*P, *B, *Q, w, few);
   }
   return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
 }
