@@ -391,7 +391,7 @@ bool pool_ok(const bs_kv_pool* p) {
 
 bool batch_ok(const bs_kv_batch* b) {
   return b && b->start && b->cu && b->table && b->tails && b->table_cols <= (1u << 24) && b->table_stride >= b->table_cols &&
-         b->n_rows <= (1u << 30) && b->n_seqs <= (1u << 24);
+         b->n_rows <= (1u << 30) && b->n_seqs <= (1u << 24) && (uint64_t)b->n_seqs * b->table_cols <= (1u << 30);
 }
 
 bool rows_ok(const void* p, int64_t token, int64_t head) {

@@ -47,16 +47,19 @@ constexpr float NEG_INF = -__builtin_inff();
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Split results: per slot and row O (f32, not divided), m, l. The kernels of a
-// call may split differently: `splits` is the kernel's own number, `slots` the
-// largest, 1 if nothing is split. A row has all its slots marked: parts without
-// keys with m = -inf and l = 0; a kernel that does not split while another does
-// writes the output itself and leaves l = -1.
+constexpr int WAVES = 4;      // of a workgroup of rows_kernel
+
+// Split results: per slot and row O (f32, not divided), m, l; `slots` is 1 if
+// nothing of the call is split. A row has all its slots marked: parts without
+// keys with m = -inf and l = 0; a row that was not split is written by its
+// kernel itself, which leaves l = -1.
 struct Work {
   float* o;
   float2* ml;
-  uint32_t splits, slots;
-  int piece;           // rows_kernel: pages of a split
+  uint32_t slots;
+  uint32_t splits;     // prompt_kernel: into how many parts it splits every tile's pages
+  uint32_t pieces;     // rows_kernel: into how many at most, of how many pages
+  int piece;
 };
 
 // Which sequences a kernel takes: those with few rows, with many, or all.
@@ -99,18 +102,28 @@ __device__ __forceinline__ int channel_of(int step, int g) {
   return step < 2 * Dims<D>::PAIRS ? 64 * (step / 2) + 16 * g + 8 * (step % 2) : 64 * Dims<D>::PAIRS + 8 * g;
 }
 
+// A page's bytes are used once in a call (128 sequences of 16,000 tokens, GB/s: 5,700 through the caches as usual, 6,130
+// as a stream).
+// `page` is the same in all lanes, so that an address is a scalar and a 32-bit offset.
+__device__ __forceinline__ uint4 stream16(const uint8_t* page, uint32_t at) {
+  const uint8_t* p = page + at;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 v = __builtin_nontemporal_load((const u32x4*)p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 template <int D, int KIND>
 struct PageK {       // a lane's part of a K page: 4 keys
   uint4 w[4][Dims<D>::PAIRS];
   uint2 r[4];
   __device__ __forceinline__ void load(const uint8_t* page, int lane) {
-    const int g = lane >> 4;
+    const uint32_t g = (uint32_t)lane >> 4, row = (16 * ((lane & 15) >> 2) + (lane & 3)) * D;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint8_t* row = page + (16 * ((lane & 15) >> 2) + 4 * t + (lane & 3)) * D;
+    for (uint32_t t = 0; t < 4; ++t) {
 #pragma unroll
-      for (int c = 0; c < Dims<D>::PAIRS; ++c) w[t][c] = *(const uint4*)(row + 64 * c + 16 * g);
-      if constexpr (Dims<D>::REST) r[t] = g < Dims<D>::REST_GROUPS ? *(const uint2*)(row + 64 * Dims<D>::PAIRS + 8 * g) : make_uint2(0, 0);
+      for (uint32_t c = 0; c < Dims<D>::PAIRS; ++c) w[t][c] = stream16(page, row + 16 * g + (4 * t * D + 64 * c));
+      if constexpr (Dims<D>::REST)
+        r[t] = g < (uint32_t)Dims<D>::REST_GROUPS ? *(const uint2*)(page + (row + 8 * g + (4 * t * D + 64 * Dims<D>::PAIRS))) : make_uint2(0, 0);
     }
   }
   __device__ __forceinline__ half8v operand(int t, int step) const {
@@ -127,8 +140,9 @@ template <int D, int KIND>
 struct PageV {
   uint4 w[Dims<D>::TILES];
   __device__ __forceinline__ void load(const uint8_t* page, int lane) {
+    const uint32_t at = (uint32_t)(lane & 15) * PAGE + 16 * ((uint32_t)lane >> 4);
 #pragma unroll
-    for (int d = 0; d < Dims<D>::TILES; ++d) w[d] = *(const uint4*)(page + (16 * d + (lane & 15)) * PAGE + 16 * (lane >> 4));
+    for (uint32_t d = 0; d < Dims<D>::TILES; ++d) w[d] = stream16(page, at + 16 * d * PAGE);
   }
   __device__ __forceinline__ half8v operand(int d, int u) const {
     return u ? codes8_to_f16<KIND>(w[d].z, w[d].w) : codes8_to_f16<KIND>(w[d].x, w[d].y);
@@ -143,8 +157,8 @@ struct State {
 };
 
 // Scores of a page from its products: s[t][i] belongs to key j0 + 4 t + i (j0: the lane group's first).
-template <int D>
-__device__ __forceinline__ void scores(f32x4 (&s)[4], const Score& sc, float row_scale, float page_scale, float shift,
+template <int N>
+__device__ __forceinline__ void scores(f32x4 (&s)[N], const Score& sc, float row_scale, float page_scale, float shift,
                                        int j0, int2 see, bool inside, bool biased, float slope, int pos) {
   const float c = row_scale * (page_scale * sc.scale);
   int lo = see.x - j0, hi = see.y - j0;
@@ -153,7 +167,7 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const Score& sc, float row
   BS_OPAQUE(hi);
   BS_OPAQUE(d);
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float x = s[t][i] * c;
@@ -167,11 +181,11 @@ __device__ __forceinline__ void scores(f32x4 (&s)[4], const Score& sc, float row
 }
 
 // Weights from scores; rescales what is already there.
-template <int D>
-__device__ __forceinline__ void weights(f32x4 (&s)[4], State<D>& st, float inv_vs) {
+template <int D, int N>
+__device__ __forceinline__ void weights(f32x4 (&s)[N], State<D>& st, float inv_vs) {
   float top = NEG_INF;
 #pragma unroll
-  for (int t = 0; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
+  for (int t = 0; t < N; ++t) top = fmaxf(top, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
   top = fmaxf(top, __shfl_xor(top, 16));
   top = fmaxf(top, __shfl_xor(top, 32));
   const float m = fmaxf(st.m, top);
@@ -180,7 +194,7 @@ __device__ __forceinline__ void weights(f32x4 (&s)[4], State<D>& st, float inv_v
   st.m = m;
   float sum = 0;
 #pragma unroll
-  for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < N; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       s[t][i] = exp2_fast(s[t][i] - base);
@@ -192,21 +206,19 @@ __device__ __forceinline__ void weights(f32x4 (&s)[4], State<D>& st, float inv_v
   for (int d = 0; d < Dims<D>::TILES; ++d) st.o[d] *= alpha;
 }
 
-// One row's m and l after all its keys of a split; without splits, its lse.
-__device__ __forceinline__ void mark_row(const bs_kv_query& A, const bs_kv_batch& B, const Work& W, uint32_t split, size_t row, float m,
-                                         float l) {
+// One row's m and l after its keys of part `slot` of `parts`; if that is all of them, its lse.
+__device__ __forceinline__ void mark_row(const bs_kv_query& A, const bs_kv_batch& B, const Work& W, uint32_t slot, uint32_t parts, size_t row,
+                                         float m, float l) {
   const size_t n = (size_t)B.n_rows * A.n_q_heads;
-  if (W.splits > 1) {
-    W.ml[split * n + row] = make_float2(m, l);
-    if (split == 0)
-      for (uint32_t k = W.splits; k < W.slots; ++k) W.ml[k * n + row] = make_float2(NEG_INF, 0.0f);
+  if (parts > 1) {
+    W.ml[slot * n + row] = make_float2(m, l);
+    if (slot == 0)
+      for (uint32_t k = parts; k < W.slots; ++k) W.ml[k * n + row] = make_float2(NEG_INF, 0.0f);
   } else {
     if (A.lse) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
     if (W.slots > 1) W.ml[row] = make_float2(NEG_INF, -1.0f);
   }
 }
-
-constexpr int WAVES = 4;
 
 // 64 of a wave's pages at a time, one a lane: number (or ~0: no such page) and scales.
 struct PageList {
@@ -230,18 +242,25 @@ struct PageList {
   __device__ __forceinline__ float scale_v(int i) const { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(vs), i)); }
 };
 
-// A split's pages are dealt to the four waves in turn. A wave reads the next page's K as soon as this one's is
-// multiplied, and its V after this one's: between 8 and 16 KiB a wave are always under way (heads of 128).
+// A tile of 16 rows of a sequence and kv head, and `piece` of the pages that it sees: pieces of one size for all
+// sequences, so that long ones do not make long pieces. The workgroup deals its pages to the four waves in turn. A wave
+// reads the next page's K as soon as this one's is multiplied, and its V after this one's: between 8 and 16 KiB a wave
+// are always under way (heads of 128).
 template <int D, int KIND>
-__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few, int32_t* status) {
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
+                                                                           int32_t* status) {
   constexpr int STEPS = Dims<D>::STEPS, TILES = Dims<D>::TILES;
   constexpr int PART = D < 128 ? D : 128, PARTS = D / PART;      // channels joined at a time
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-  const uint32_t h = blockIdx.y % P.n_kv_heads, b = blockIdx.z;
-  const uint32_t group = A.n_q_heads / P.n_kv_heads;
-  const uint32_t row_tiles = gridDim.y / P.n_kv_heads;
+  // consecutive workgroups go to the eight dies in turn: pieces, of which short sequences have few, come last
+  const uint32_t h = blockIdx.x % P.n_kv_heads, b = blockIdx.y, slot = blockIdx.z;
+  const uint32_t group = A.n_q_heads / P.n_kv_heads, row_tiles = gridDim.x / P.n_kv_heads;
   __shared__ __attribute__((aligned(16))) float part_o[WAVES][16][PART + 4];
   __shared__ float part_m[WAVES][16], part_l[WAVES][16];
+  const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
+  const Score sc = {fabsf(A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E), A.softcap * LOG2E};
+  const bool biased = A.slopes != nullptr;
+  const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
 
   SeqStep s;
   if (!seq_step(B, b, s)) {
@@ -250,13 +269,9 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
   }
   const int rows = s.n * (int)group;
   if (!takes(take, rows, few)) return;
-  const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
-  const Score sc = {fabsf(A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E), A.softcap * LOG2E};
-  const bool biased = A.slopes != nullptr;
-  const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
   const int32_t* table = B.table + (size_t)b * B.table_stride;
 
-  for (int tile = blockIdx.y / P.n_kv_heads; tile * 16 < rows; tile += row_tiles) {
+  for (int tile = blockIdx.x / P.n_kv_heads; tile * 16 < rows; tile += row_tiles) {
     const int r = tile * 16 + (lane & 15);
     const bool real = r < rows;
     const int i = real ? r / (int)group : 0;
@@ -264,41 +279,79 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     const int pos = s.start + i;
     const int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
 
-    // pages that any row of the tile sees, cut into splits
+    // pages that any row of the tile sees, and this workgroup's piece of them
     int lo = see.x < see.y ? see.x : 0x7FFFFFFF, hi = see.x < see.y ? see.y : 0;
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) {
       lo = min(lo, __shfl_xor(lo, d));
       hi = max(hi, __shfl_xor(hi, d));
     }
-    const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
-    // pieces of one size for all sequences, so that long ones do not make long pieces
-    const int first = page_lo + W.piece * (int)blockIdx.x;
-    const int mine = __builtin_amdgcn_readfirstlane(first);
-    const int end = __builtin_amdgcn_readfirstlane(blockIdx.x + 1 == W.splits ? page_hi : min(first + W.piece, page_hi));
+    const int page_lo = __builtin_amdgcn_readfirstlane(lo >= hi ? 0 : lo / (int)PAGE);
+    const int page_hi = __builtin_amdgcn_readfirstlane(lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE);
+    const uint32_t parts = min((uint32_t)max((page_hi - page_lo + W.piece - 1) / W.piece, 1), W.pieces);
+    if (slot >= parts) continue;
+    const int mine = page_lo + W.piece * (int)slot, end = slot + 1 == parts ? page_hi : mine + W.piece;
     const int full_pages = s.len / (int)PAGE, full_end = min(end, full_pages);      // pages from full_pages on are the tail
 
+    // The tail, 16 keys of it a wave, and the first page are on their way before q is looked at. Key 4 g + e of the
+    // wave's 16 belongs to lane group g, in S^T and as the right operand of the second product (of whose eight elements
+    // a lane the last four are 0). Slots after the sequence's end hold anything: they count as 0.
+    const bool tailed = end > full_pages;
+    const int used = tailed ? s.len - full_pages * (int)PAGE - 16 * wave : 0;       // of this wave's 16
+    uint4 kt[STEPS];
+    uint2 vt[TILES];
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    if (used > 0) {
+      uint32_t id = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
+      if (id >= P.n_tails) {
+        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
+        id = 0;
+      }
+      const uint16_t *const kr = P.k_tail + id * unit + head + 16 * wave * D, *const vr = P.v_tail + id * unit + head + 16 * wave;
+      const uint32_t row = (uint32_t)(lane & 15) * D, ahead = (uint32_t)(lane & 15) * PAGE + 4 * (uint32_t)g;
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c) {
+        const int ch = channel_of<D>(c, g);
+        kt[c] = ((lane & 15) < used && ch < D) ? *(const uint4*)(kr + (row + (uint32_t)ch)) : none;
+      }
+#pragma unroll
+      for (int d = 0; d < TILES; ++d) vt[d] = 4 * g < used ? *(const uint2*)(vr + (ahead + 16 * (uint32_t)d * PAGE)) : make_uint2(0, 0);
+    }
     PageList list;
     list.load(P, table, h, mine + wave + WAVES * lane, full_end, status);
+    const uint8_t *const kp = (const uint8_t*)P.k + head, *const vp = (const uint8_t*)P.v + head;
+    PageK<D, KIND> k;
+    PageV<D, KIND> v;
+    uint32_t id = list.number(0);
+    if (mine + wave < full_end) {
+      k.load(kp + (id == ~0u ? 0 : id * unit), lane);
+      v.load(vp + (id == ~0u ? 0 : id * unit), lane);
+    }
 
     const float slope = biased ? A.slopes[hq] * LOG2E : 0.0f;
     // the row of q as f16, scaled by a power of two to lie below 2 (exact for what is within 2^-14 of the largest)
     const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
     half8v q16[STEPS];
     float row_scale;
+    State<D> st;
+#pragma unroll
+    for (int d = 0; d < TILES; ++d) st.o[d] = f32x4{0, 0, 0, 0};
+    st.m = NEG_INF;
+    st.l = 0;
     {
-      uint16_t x[STEPS][8];
+      uint4 raw[STEPS];
       float top = 0;
       bool fine = true;
 #pragma unroll
       for (int c = 0; c < STEPS; ++c) {
         const int ch = channel_of<D>(c, g);
-        const uint4 w = (real && ch < D) ? *(const uint4*)(q + ch) : make_uint4(0, 0, 0, 0);
-        __builtin_memcpy(x[c], &w, 16);
+        raw[c] = (real && ch < D) ? *(const uint4*)(q + ch) : none;
+        uint16_t x[8];
+        __builtin_memcpy(x, &raw[c], 16);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          fine = fine && bf16_finite(x[c][e]);
-          top = fmaxf(top, fabsf(bf16_to_f32(x[c][e])));
+          fine = fine && bf16_finite(x[e]);
+          top = fmaxf(top, fabsf(bf16_to_f32(x[e])));
         }
       }
       top = fmaxf(top, __shfl_xor(top, 16));
@@ -309,24 +362,40 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
       const int e2 = (top == 0.0f || !ok) ? 0 : max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
       row_scale = ok ? ldexpf(1.0f, e2) : __uint_as_float(0x7FC00000u);
 #pragma unroll
-      for (int c = 0; c < STEPS; ++c)
+      for (int c = 0; c < STEPS; ++c) {
+        uint16_t x[8];
+        __builtin_memcpy(x, &raw[c], 16);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[c][e]), -e2)) : (_Float16)0.0f;
+        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[e]), -e2)) : (_Float16)0.0f;
+      }
+      // the tail: bf16 as it is; p' in two bf16 parts keeps 16 bits of it
+      if (used > 0) {
+        f32x4 acc[1] = {f32x4{0, 0, 0, 0}};
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c)
+          acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kt[c]), __builtin_bit_cast(bf16x8, raw[c]), acc[0], 0, 0, 0);
+        scores(acc, sc, ok ? sign : row_scale, 1.0f, 0.0f, full_pages * (int)PAGE + 16 * wave + 4 * g, see, false, biased, slope, pos);
+        weights<D>(acc, st, 1.0f);
+        bf16x8 p_hi, p_lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p_hi[e] = (__bf16)acc[0][e];
+          p_lo[e] = (__bf16)(acc[0][e] - (float)p_hi[e]);
+          p_hi[e + 4] = p_lo[e + 4] = (__bf16)0.0f;
+        }
+#pragma unroll
+        for (int d = 0; d < TILES; ++d) {
+          bf16x8 vb = __builtin_bit_cast(bf16x8, make_uint4(vt[d].x, vt[d].y, 0, 0));
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (4 * g + e >= used) vb[e] = (__bf16)0.0f;
+          st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_hi, st.o[d], 0, 0, 0);
+          st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_lo, st.o[d], 0, 0, 0);
+        }
+      }
     }
 
-    State<D> st;
-#pragma unroll
-    for (int d = 0; d < TILES; ++d) st.o[d] = f32x4{0, 0, 0, 0};
-    st.m = NEG_INF;
-    st.l = 0;
-
     if (mine + wave < full_end) {
-      const uint8_t *const kp = (const uint8_t*)P.k + head, *const vp = (const uint8_t*)P.v + head;
-      PageK<D, KIND> k;
-      PageV<D, KIND> v;
-      uint32_t id = list.number(0);
-      k.load(kp + (id == ~0u ? 0 : id * unit), lane);
-      v.load(vp + (id == ~0u ? 0 : id * unit), lane);
       int at = 0;                       // place in the list
       for (int page = mine + wave; page < full_end; page += WAVES) {
         const bool ok = id != ~0u;
@@ -350,7 +419,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
         k.load(kp + next, lane);
         const int j0 = page * (int)PAGE;
         const bool inside = ok && __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
-        scores<D>(acc, sc, row_scale, ks, shift, j0 + 16 * g, ok ? see : make_int2(0, 0), inside, biased, slope, pos);
+        scores(acc, sc, row_scale, ks, shift, j0 + 16 * g, ok ? see : make_int2(0, 0), inside, biased, slope, pos);
         weights<D>(acc, st, exp2_fast(-shift));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -364,55 +433,6 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
       }
     }
 
-    // the tail: bf16 as it is; p' in two bf16 parts keeps 16 bits of it. Slots after the sequence's end hold anything.
-    if (mine < end && end > full_pages && wave == (end - 1 - mine) % WAVES) {
-      const uint32_t id = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
-      if (id >= P.n_tails) {
-        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
-      } else {
-        const uint16_t* kt = P.k_tail + id * unit + head;
-        const uint16_t* vt = P.v_tail + id * unit + head;
-        const int used = s.len - full_pages * (int)PAGE;
-        f32x4 acc[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int c = 0; c < STEPS; ++c) {
-          const int ch = channel_of<D>(c, g);
-          const uint4 none = make_uint4(0, 0, 0, 0);
-          const bf16x8 qb = __builtin_bit_cast(bf16x8, (real && ch < D) ? *(const uint4*)(q + ch) : none);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const int key = 16 * ((lane & 15) >> 2) + 4 * t + (lane & 3);
-            const bf16x8 kb = __builtin_bit_cast(bf16x8, (key < used && ch < D) ? *(const uint4*)(kt + key * D + ch) : none);
-            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb, qb, acc[t], 0, 0, 0);
-          }
-        }
-        scores<D>(acc, sc, row_scale == row_scale ? sign : row_scale, 1.0f, 0.0f, full_pages * (int)PAGE + 16 * g, see, false, biased, slope, pos);
-        weights<D>(acc, st, 1.0f);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          bf16x8 p_hi, p_lo;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = acc[2 * u + e / 4][e % 4];
-            p_hi[e] = (__bf16)x;
-            p_lo[e] = (__bf16)(x - (float)p_hi[e]);
-          }
-          const int key = 16 * g + 8 * u;
-#pragma unroll
-          for (int d = 0; d < TILES; ++d) {
-            bf16x8 vb = __builtin_bit_cast(bf16x8, *(const uint4*)(vt + (16 * d + (lane & 15)) * PAGE + key));
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (key + e >= used) vb[e] = (__bf16)0.0f;
-            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_hi, st.o[d], 0, 0, 0);
-            st.o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p_lo, st.o[d], 0, 0, 0);
-          }
-        }
-      }
-    }
-
     // join the waves: rows' m and l, then O. A thread has eight channels of row tid / 16.
     st.l += __shfl_xor(st.l, 16);
     st.l += __shfl_xor(st.l, 32);
@@ -420,7 +440,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     if (lane < 16) part_m[wave][lane] = st.m, part_l[wave][lane] = st.l;
     const int wr = (int)threadIdx.x >> 4, wc = (int)threadIdx.x & 15, wrow = tile * 16 + wr;
     const size_t out_row = (size_t)(s.t0 + (wrow < rows ? wrow / (int)group : 0)) * A.n_q_heads + h * group + (uint32_t)(wrow < rows ? wrow % (int)group : 0);
-    const size_t split_row = (size_t)blockIdx.x * B.n_rows * A.n_q_heads + out_row;
+    const size_t split_row = (size_t)slot * B.n_rows * A.n_q_heads + out_row;
 #pragma unroll
     for (int part = 0; part < PARTS; ++part) {
       if (part) __syncthreads();
@@ -436,14 +456,14 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
         l += part_l[w][wr] * f[w];
       }
       if (wrow >= rows) continue;
-      if (part == 0 && wc == 0) mark_row(A, B, W, blockIdx.x, out_row, m, l);
-      if ((W.splits > 1 && mine >= end) || 8 * wc >= PART) continue;    // nothing here: the joining kernel reads no O
+      if (part == 0 && wc == 0) mark_row(A, B, W, slot, parts, out_row, m, l);
+      if (8 * wc >= PART) continue;
       float x[8] = {};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] += part_o[w][wr][8 * wc + e] * f[w];
-      if (W.splits > 1) {
+      if (parts > 1) {
         float* to = W.o + split_row * D + part * PART + 8 * wc;
         *(float4*)to = make_float4(x[0], x[1], x[2], x[3]);
         *(float4*)(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
@@ -764,7 +784,7 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
                           [&](int n, half8v a) { o[n % TILES] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[n / TILES], o[n % TILES], 0, 0, 0); });
     }
 
-    // the tail, as in rows_kernel
+    // the tail: bf16 as it is; p' in two bf16 parts keeps 16 bits of it. Slots after the sequence's end hold anything.
     if (begin < end && end > full_pages && full_pages * (int)PAGE < wave_hi) {
       const uint32_t id = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
       if (id >= P.n_tails) {
@@ -823,7 +843,7 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
     l = pair_sum(l);
     if (real) {
       const size_t out_row = (size_t)(s.t0 + i) * A.n_q_heads + hq;
-      if (half == 0) mark_row(A, B, W, split, out_row, m + (P_SHIFT - SHIFT), l);
+      if (half == 0) mark_row(A, B, W, split, W.splits, out_row, m + (P_SHIFT - SHIFT), l);
       if (W.splits == 1 || begin < end) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         float* part = W.o + ((size_t)split * B.n_rows * A.n_q_heads + out_row) * D;
@@ -925,10 +945,13 @@ constexpr uint32_t FEW_ROWS = 16;
 
 struct Plan {
   Take rows_take, prompt_take;
-  uint32_t row_tiles, row_splits;        // rows_kernel; 0 tiles: not launched
-  uint32_t prompt_tiles, prompt_splits;  // prompt_kernel
+  uint32_t row_tiles, pieces, piece;     // rows_kernel; 0 tiles: not launched
+  uint32_t prompt_tiles, prompt_splits;  // prompt_kernel; 0 tiles: not launched
   uint32_t slots;
 };
+
+constexpr uint64_t RESIDENT = 512;       // workgroups of 256 threads that run at once, two on each of 256 compute units
+constexpr uint64_t PIECES_WANTED = 512;
 
 uint32_t split_for(uint64_t blocks, uint64_t want, uint64_t pages, uint64_t least) {
   const uint64_t n = blocks >= want ? 1 : (want + blocks - 1) / blocks;
@@ -936,22 +959,23 @@ uint32_t split_for(uint64_t blocks, uint64_t want, uint64_t pages, uint64_t leas
 }
 
 Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
-  const uint64_t group = n_q_heads / P->n_kv_heads, heads = P->n_kv_heads;
+  const uint64_t group = n_q_heads / P->n_kv_heads, heads = P->n_kv_heads, seqs = B->n_seqs;
   const uint64_t rows = std::max<uint64_t>(B->max_new * group, 1), pages = (B->max_len + PAGE - 1) / PAGE;
-  Plan p = {ALL, ALL, 0, 1, 0, 1, 1};
+  Plan p = {ALL, ALL, 0, 1, 1, 0, 1, 1};
   if (rows > FEW_ROWS) {
     p.prompt_tiles = (uint32_t)std::min<uint64_t>((rows + PROMPT_ROWS - 1) / PROMPT_ROWS, 65535);
     // tiles that the sequences can have in all, if max_new is what it says
-    const uint64_t tiles = std::min<uint64_t>(p.prompt_tiles * (uint64_t)B->n_seqs, B->n_rows * group / PROMPT_ROWS + B->n_seqs);
-    p.prompt_splits = split_for(tiles * heads, 512, pages, 8);
+    const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(p.prompt_tiles * seqs, B->n_rows * group / PROMPT_ROWS + seqs), 1);
+    p.prompt_splits = split_for(tiles * heads, RESIDENT, pages, 8);
   }
-  if (rows <= FEW_ROWS || B->n_seqs > 1) {
+  if (rows <= FEW_ROWS || seqs > 1) {
     const uint64_t most = std::min<uint64_t>(rows, FEW_ROWS);
-    p.row_tiles = (uint32_t)std::min<uint64_t>((most + 15) / 16, 65535 / heads);
-    p.row_splits = split_for(p.row_tiles * heads * B->n_seqs, 1024, pages, WAVES);
+    p.row_tiles = (uint32_t)((most + 15) / 16);
+    p.pieces = split_for(p.row_tiles * heads * seqs, PIECES_WANTED, pages, WAVES);
+    p.piece = (uint32_t)std::max<uint64_t>((pages + p.pieces - 1) / p.pieces, 1);
   }
   if (p.prompt_tiles && p.row_tiles) p.rows_take = FEW, p.prompt_take = MANY;
-  p.slots = std::max(p.row_splits, p.prompt_splits);
+  p.slots = std::max(p.pieces, p.prompt_splits);
   return p;
 }
 
@@ -971,19 +995,15 @@ template <int D, int KIND>
 int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
-  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), 1, p.slots, 0};
+  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.slots, p.prompt_splits, p.pieces, (int)p.piece};
   if (p.prompt_tiles) {
-    w.splits = p.prompt_splits;
     const dim3 grid(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs);
     if (Q->softcap == 0.0f && !Q->slopes) prompt_launch<D, KIND, true>(P, B, Q, w, p.prompt_take, status, stream, grid);
     else prompt_launch<D, KIND, false>(P, B, Q, w, p.prompt_take, status, stream, grid);
   }
-  if (p.row_tiles) {
-    w.splits = p.row_splits;
-    w.piece = (int)std::max<uint64_t>((((uint64_t)B->max_len + PAGE - 1) / PAGE + p.row_splits - 1) / p.row_splits, 1);
-    rows_kernel<D, KIND><<<dim3(p.row_splits, p.row_tiles * P->n_kv_heads, B->n_seqs), 64 * WAVES, 0, stream>>>(
-        *P, *B, *Q, w, p.rows_take, (int)FEW_ROWS, status);
-  }
+  if (p.row_tiles)
+    rows_kernel<D, KIND><<<dim3(p.row_tiles * P->n_kv_heads, B->n_seqs, p.pieces), 64 * WAVES, 0, stream>>>(*P, *B, *Q, w, p.rows_take, (int)FEW_ROWS,
+                                                                                                        status);
   if (p.slots > 1) {
     // where only short sequences are split, only their rows are looked at
     const int few = p.rows_take == FEW && p.prompt_splits == 1 ? (int)FEW_ROWS : 0;
