@@ -18,7 +18,7 @@ namespace {
 
 using namespace bs_kv;
 
-constexpr uint32_t THREADS = 256;
+constexpr uint32_t THREADS = 256, DIES = 8;
 
 // Largest |x| of a page held to this range: a scale stays a normal f32 number,
 // and so do its inverse and the products of attention's weights with it.
@@ -48,13 +48,13 @@ struct alignas(2 * N) Half {
 // The page numbered `unit` among all pages that the step touches, sequence by
 // sequence: its sequence and its place in it. Every wave counts for itself, 64
 // sequences at a time.
-__device__ bool find_unit(const bs_kv_batch& B, uint32_t unit, uint32_t& b, uint32_t& page, int32_t* status) {
+__device__ bool find_unit(const bs_kv_batch& B, uint32_t unit, uint32_t& b, uint32_t& page, SeqStep& step, int32_t* status) {
   const uint32_t lane = threadIdx.x & 63;
   uint32_t base = 0;
   for (uint32_t b0 = 0; b0 < B.n_seqs; b0 += 64) {
     uint32_t pages = 0, at = 0;
+    SeqStep s = {0, 0, 0, 0};
     if (b0 + lane < B.n_seqs) {
-      SeqStep s;
       if (!seq_step(B, b0 + lane, s) && unit == 0) report(status, BS_DEV_ERR_BOUNDS);
       at = (uint32_t)s.start / PAGE;
       if (s.n > 0) pages = (uint32_t)(s.len - 1) / PAGE - at + 1;
@@ -69,10 +69,12 @@ __device__ bool find_unit(const bs_kv_batch& B, uint32_t unit, uint32_t& b, uint
     if (past) {
       const int l = __builtin_ctzll(past);
       b = b0 + (uint32_t)l;
-      page = (uint32_t)__shfl((int)(at + unit - (base + incl - pages)), l);
+      page = (uint32_t)__builtin_amdgcn_readlane((int)(at + unit - (base + incl - pages)), l);
+      step.t0 = __builtin_amdgcn_readlane(s.t0, l), step.n = __builtin_amdgcn_readlane(s.n, l);
+      step.start = __builtin_amdgcn_readlane(s.start, l), step.len = __builtin_amdgcn_readlane(s.len, l);
       return true;
     }
-    base += (uint32_t)__shfl((int)incl, 63);
+    base += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
   }
   return false;
 }
@@ -137,17 +139,18 @@ __global__ __launch_bounds__(THREADS) void append_kernel(bs_kv_pool P, bs_kv_bat
   __shared__ uint32_t vt[PAGE * ROW];
   __shared__ int poisoned[PAGE];
   __shared__ float tops[2][THREADS / 64];
-  const uint32_t tid = threadIdx.x, h = blockIdx.y;
+  // Consecutive workgroups go to the eight dies in turn. The heads of one page go to one die, one after another, which
+  // then reads their tokens' angles once.
+  const uint32_t tid = threadIdx.x, turn_of = blockIdx.x / DIES, h = turn_of % P.n_kv_heads;
   uint32_t b, page;
-  if (!find_unit(B, blockIdx.x, b, page, status)) return;
   SeqStep s;
-  seq_step(B, b, s);
+  if (!find_unit(B, turn_of / P.n_kv_heads * DIES + blockIdx.x % DIES, b, page, s, status)) return;
   const int p0 = (int)(page * PAGE);
   const int old = max(s.start - p0, 0), have = min(s.len - p0, (int)PAGE);  // slots [0, old) are in the tail, [old, have) are new
   const bool full = have == (int)PAGE;
   const int t_first = s.t0 + p0 - s.start;                                  // the row of slot 0 (old slots have none)
-  const uint32_t tail_in = (uint32_t)B.tails[2 * b], tail_out = (uint32_t)B.tails[2 * b + 1];
-  const uint32_t id = (uint32_t)B.table[(size_t)b * B.table_stride + page];
+  const uint32_t tail_in = (uint32_t)uniform_load(B.tails, 2 * (size_t)b), tail_out = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
+  const uint32_t id = (uint32_t)uniform_load(B.table, (size_t)b * B.table_stride + page);
   // the page's earlier tokens are needed to quantise it, or where the tail moves without a page being completed
   const bool from_tail = old > 0 && (full || tail_in != tail_out);
   const int lo = from_tail ? 0 : old;
@@ -164,6 +167,31 @@ __global__ __launch_bounds__(THREADS) void append_kernel(bs_kv_pool P, bs_kv_bat
 
   if (tid < PAGE) poisoned[tid] = 0;
   __syncthreads();
+
+  // The q heads of the group, new tokens only. With few tokens the heads go to different threads, with many one thread
+  // turns its channels in every head by the angles it has loaded. From the last thread on down: of a single token, q is
+  // the last waves' and k and v the first one's, side by side.
+  if (R.q) {
+    const uint32_t group = R.n_q_heads / P.n_kv_heads, tokens = (uint32_t)(have - old);
+    const uint32_t spread = tokens * ITEMS >= THREADS ? 1 : group;
+    for (uint32_t idx = THREADS - 1 - tid; idx < tokens * spread * ITEMS; idx += THREADS) {
+      const Item<VEC> it = item_at<VEC>(R, idx % ITEMS);
+      const uint32_t rest = idx / ITEMS;
+      const int slot = old + (int)(rest / spread);
+      const int64_t t = t_first + slot;
+      float c[VEC], sn[VEC];
+      if (it.angle >= 0) load_angles<VEC>(R, p0 + slot, it.angle, c, sn);
+      for (uint32_t g = rest % spread; g < group; g += spread) {
+        const int64_t hq = (int64_t)h * group + g;
+        const uint16_t* q = R.q + t * R.q_token + hq * R.q_head;
+        uint16_t* o = R.q_out + (t * R.n_q_heads + hq) * D;
+        Half<VEC> a = load_half<VEC>(q + it.a), e = load_half<VEC>(q + it.b);
+        if (it.angle >= 0) turn<VEC>(c, sn, R.interleaved, a, e);
+        *(Half<VEC>*)(o + it.a) = a;
+        *(Half<VEC>*)(o + it.b) = e;
+      }
+    }
+  }
 
   // K into registers, V into LDS
   Half<VEC> ka[NI], kb[NI];
@@ -302,30 +330,6 @@ __global__ __launch_bounds__(THREADS) void append_kernel(bs_kv_pool P, bs_kv_bat
       vo[d * PAGE + slot] = v16[slot * 2 * ROW + d];
     }
   }
-
-  // the q heads of the group: the new tokens' rows. With few tokens the heads go to different threads, with many one
-  // thread turns its channels in every head by the angles it has loaded.
-  if (R.q) {
-    const uint32_t group = R.n_q_heads / P.n_kv_heads, tokens = (uint32_t)(have - old);
-    const uint32_t spread = tokens * ITEMS >= THREADS ? 1 : group;
-    for (uint32_t idx = tid; idx < tokens * spread * ITEMS; idx += THREADS) {
-      const Item<VEC> it = item_at<VEC>(R, idx % ITEMS);
-      const uint32_t rest = idx / ITEMS;
-      const int slot = old + (int)(rest / spread);
-      const int64_t t = t_first + slot;
-      float c[VEC], sn[VEC];
-      if (it.angle >= 0) load_angles<VEC>(R, p0 + slot, it.angle, c, sn);
-      for (uint32_t g = rest % spread; g < group; g += spread) {
-        const int64_t hq = (int64_t)h * group + g;
-        const uint16_t* q = R.q + t * R.q_token + hq * R.q_head;
-        uint16_t* o = R.q_out + (t * R.n_q_heads + hq) * D;
-        Half<VEC> a = load_half<VEC>(q + it.a), e = load_half<VEC>(q + it.b);
-        if (it.angle >= 0) turn<VEC>(c, sn, R.interleaved, a, e);
-        *(Half<VEC>*)(o + it.a) = a;
-        *(Half<VEC>*)(o + it.b) = e;
-      }
-    }
-  }
 }
 
 template <int D, int KIND>
@@ -338,7 +342,7 @@ __global__ __launch_bounds__(THREADS) void read_kernel(bs_kv_pool P, const int32
   const uint32_t tid = threadIdx.x, page = blockIdx.x, h = blockIdx.y;
   const uint32_t p0 = page * PAGE, have = min(n - p0, PAGE);
   const bool full = have == PAGE;
-  const uint32_t id = (uint32_t)(full ? pages[page] : tail[0]);
+  const uint32_t id = (uint32_t)(full ? uniform_load(pages, page) : uniform_load(tail, 0));
   if (id >= (full ? P.n_pages : P.n_tails)) {
     if (tid == 0) report(status, BS_DEV_ERR_BOUNDS);
     return;
@@ -348,21 +352,32 @@ __global__ __launch_bounds__(THREADS) void read_kernel(bs_kv_pool P, const int32
   uint16_t* vo = v_out + ((size_t)h * n + p0) * D;
   uint16_t* v16 = (uint16_t*)vt;
   if (full) {
-    const float ks = P.k_scale[(size_t)id * P.n_kv_heads + h], vs = P.v_scale[(size_t)id * P.n_kv_heads + h];
-    for (uint32_t i = tid; i < PAGE * D / 8; i += THREADS) {
-      const uint2 w = *(const uint2*)((const uint8_t*)P.k + base + 8 * i);
-      const half8v x = codes8_to_f16<KIND>(w.x, w.y);
-      Half<8> y;
+    const float ks = uniform_load(P.k_scale, (size_t)id * P.n_kv_heads + h), vs = uniform_load(P.v_scale, (size_t)id * P.n_kv_heads + h);
+    constexpr uint32_t LOADS = (PAGE * D / 16 + THREADS - 1) / THREADS;
+    const uint4 *const kp = (const uint4*)((const uint8_t*)P.k + base), *const vp = (const uint4*)((const uint8_t*)P.v + base);
+    uint4 kw[LOADS], vw[LOADS];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y.x[e] = f32_to_bf16((float)x[e] * ks);
-      *(Half<8>*)(ko + 8 * i) = y;
+    for (uint32_t l = 0; l < LOADS; ++l) {
+      const uint32_t i = tid + l * THREADS;
+      if (PAGE * D % (16 * THREADS) == 0 || i < PAGE * D / 16) kw[l] = kp[i], vw[l] = vp[i];
     }
-    for (uint32_t i = tid; i < PAGE * D / 8; i += THREADS) {
-      const uint32_t d = i / (PAGE / 8), slot = i % (PAGE / 8) * 8;
-      const uint2 w = *(const uint2*)((const uint8_t*)P.v + base + d * PAGE + slot);
-      const half8v x = codes8_to_f16<KIND>(w.x, w.y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v16[(slot + e) * 2 * ROW + d] = f32_to_bf16((float)x[e] * vs);
+    for (uint32_t l = 0; l < LOADS; ++l) {
+      const uint32_t i = tid + l * THREADS;
+      if (PAGE * D % (16 * THREADS) != 0 && i >= PAGE * D / 16) continue;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const half8v x = p ? codes8_to_f16<KIND>(kw[l].z, kw[l].w) : codes8_to_f16<KIND>(kw[l].x, kw[l].y);
+        const half8v z = p ? codes8_to_f16<KIND>(vw[l].z, vw[l].w) : codes8_to_f16<KIND>(vw[l].x, vw[l].y);
+        const uint32_t d = i / (PAGE / 16), slot = i % (PAGE / 16) * 16 + 8 * p;
+        Half<8> y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          y.x[e] = f32_to_bf16((float)x[e] * ks);
+          v16[(slot + e) * 2 * ROW + d] = f32_to_bf16((float)z[e] * vs);
+        }
+        *(Half<8>*)(ko + 16 * i + 8 * p) = y;
+      }
     }
   } else {
     for (uint32_t i = tid; i < have * D / 8; i += THREADS) *(Half<8>*)(ko + 8 * i) = load_half<8>(P.k_tail + base + 8 * i);
@@ -402,7 +417,9 @@ template <int D, int VEC, int KIND>
 int append_launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_rows* R, int32_t* status, hipStream_t stream) {
   // n new tokens touch at most (n + 62) / 64 + 1 pages, and no more than n: enough workgroups for any sequence lengths
   const uint64_t units = std::min<uint64_t>(B->n_rows, (B->n_rows + 62ull * B->n_seqs) / 64 + B->n_seqs);
-  append_kernel<D, VEC, KIND><<<dim3((uint32_t)units, P->n_kv_heads), THREADS, 0, stream>>>(*P, *B, *R, status);
+  const uint64_t blocks = (units + DIES - 1) / DIES * DIES * P->n_kv_heads;
+  if (blocks > 0x7FFFFFFF) return BS_ERR_ARG;
+  append_kernel<D, VEC, KIND><<<(uint32_t)blocks, THREADS, 0, stream>>>(*P, *B, *R, status);
   return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
 }
 

@@ -26,6 +26,7 @@ another stream need the usual wait and record_stream by the caller.
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
@@ -35,7 +36,6 @@ from . import _native
 PAGE = 64
 HEAD_DIMS = (64, 80, 96, 128, 256)
 _KINDS = {torch.int8: 0, torch.float8_e4m3fn: 1}
-_byref = ctypes.byref
 
 
 def _tensor(name: str, t, dtype, device=None, shape=None):
@@ -51,8 +51,8 @@ def _tensor(name: str, t, dtype, device=None, shape=None):
 class KVPool:
     """One layer's storage: the six tensors (contiguous, on one GPU), checked once."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "device", "dtype", "n_pages", "n_tails", "n_kv_heads",
-                 "head_dim", "c")
+    __slots__ = ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "device", "index", "dtype", "n_pages", "n_tails",
+                 "n_kv_heads", "head_dim", "c", "ref")
 
     def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
         if not isinstance(k, torch.Tensor) or k.dtype not in _KINDS or k.dim() != 4 or k.shape[2] != PAGE:
@@ -74,10 +74,11 @@ class KVPool:
             if not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"KVPool: {name} must be contiguous and 16-byte aligned")
         self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
-        self.device, self.dtype = k.device, k.dtype
+        self.device, self.index, self.dtype = k.device, k.get_device(), k.dtype       # index: -1 on the host
         self.n_pages, self.n_tails, self.n_kv_heads, self.head_dim = n, m, h, d
         self.c = _native.BsKvPool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(),
                                   v_tail.data_ptr(), n, m, h, d, _KINDS[k.dtype])
+        self.ref = ctypes.byref(self.c)
 
 
 class KVBatch:
@@ -92,7 +93,7 @@ class KVBatch:
     sequence. They choose launch shapes; a wrong value costs time, not results.
     """
 
-    __slots__ = ("start", "cu", "table", "tails", "n_seqs", "max_new", "max_len", "c")
+    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "c", "ref")
 
     def __init__(self, start, cu, table, tails, max_new: int, max_len: int):
         _tensor("start", start, torch.int32)
@@ -113,18 +114,14 @@ class KVBatch:
         self.n_seqs, self.max_new, self.max_len = b, int(max_new), int(max_len)
         self.c = _native.BsKvBatch(start.data_ptr(), cu.data_ptr(), table.data_ptr(), tails.data_ptr(), b, stride,
                                    table.shape[1], 0, int(max_new), int(max_len))
-
-    def for_rows(self, n: int):
-        """The C struct with n packed rows."""
-        self.c.n_rows = n
-        return self.c
+        self.ref, self.index = ctypes.byref(self.c), start.get_device()
 
 
 class Rope:
     """Rotation angles by position: cos and sin f32 [positions, turned channels / 2] on the GPU.
     The first 2 * cos.shape[1] channels turn, in pairs (i, i + half), or (2i, 2i + 1) if interleaved."""
 
-    __slots__ = ("cos", "sin", "interleaved", "rot")
+    __slots__ = ("cos", "sin", "interleaved", "rot", "positions", "index", "cos_ptr", "sin_ptr")
 
     def __init__(self, cos, sin, interleaved: bool = False):
         _tensor("cos", cos, torch.float32)
@@ -133,7 +130,8 @@ class Rope:
         _tensor("sin", sin, torch.float32, cos.device, cos.shape)
         self.cos, self.sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
                               for t in (cos, sin))
-        self.interleaved, self.rot = bool(interleaved), 2 * cos.shape[1]
+        self.interleaved, self.rot, self.positions = bool(interleaved), 2 * cos.shape[1], cos.shape[0]
+        self.index, self.cos_ptr, self.sin_ptr = cos.get_device(), self.cos.data_ptr(), self.sin.data_ptr()
 
     @classmethod
     def from_theta(cls, rot: int, positions: int, theta: float = 10000.0, interleaved: bool = False, device="cuda") -> "Rope":
@@ -144,39 +142,64 @@ class Rope:
 
 
 def _rows(name: str, t, n: Optional[int], heads: Optional[int], pool: KVPool):
-    """t as bf16 rows [tokens, heads, dim] that the kernels can read: in place if its rows start at
-    multiples of 16 bytes and its last dimension is contiguous, else a contiguous copy."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or t.dim() != 3:
+    """t as bf16 rows [tokens, heads, dim] that the kernels can read, with its tokens, heads, address
+    and strides: in place if its rows start at multiples of 16 bytes and its last dimension is
+    contiguous, else a contiguous copy."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.bfloat16:
         raise ValueError(f"{name} must be a bfloat16 tensor [tokens, heads, head dim]")
-    if t.device != pool.device:
-        raise ValueError(f"{name} is on {t.device}, the cache is on {pool.device}")
-    if t.shape[2] != pool.head_dim or (n is not None and t.shape[0] != n) or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected [{n if n is not None else 'tokens'}, "
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != pool.head_dim or (n is not None and shape[0] != n) or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected [{n if n is not None else 'tokens'}, "
                          f"{heads if heads is not None else 'heads'}, {pool.head_dim}]")
-    s = t.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+    if t.get_device() != pool.index:
+        raise ValueError(f"{name} is on {t.device}, the cache is on {pool.device}")
+    s0, s1, s2 = t.stride()
+    p = t.data_ptr()
+    if s2 != 1 or (s0 | s1) & 7 or p & 15:
         t = t.contiguous()
-        if t.data_ptr() % 16:
+        if t.data_ptr() & 15:
             t = t.clone()
-    return t
+        s0, s1, _ = t.stride()
+        p = t.data_ptr()
+    return t, shape[0], shape[1], p, s0, s1
 
 
-def _q_heads(q, pool: KVPool) -> int:
-    h = q.shape[1]
+def _check_heads(h: int, pool: KVPool) -> None:
     if h < 1 or h % pool.n_kv_heads:
         raise ValueError(f"q has {h} heads, not a multiple of the cache's {pool.n_kv_heads} kv heads")
-    return h
 
 
 def _gpu(pool: KVPool) -> None:
-    if pool.device.type != "cuda":
+    if pool.index < 0:
         raise RuntimeError("the paged KV cache's operators run on an AMD GPU (MI355X); the pool is on " + str(pool.device))
 
 
 def _check_batch(pool: KVPool, batch: KVBatch) -> None:
     _gpu(pool)
-    if batch.start.device != pool.device:
+    if batch.index != pool.index:
         raise ValueError(f"the batch is on {batch.start.device}, the cache is on {pool.device}")
+
+
+# The current stream's handle of a device, without the Stream object that torch.cuda.current_stream makes (2 us of a
+# call that takes 10).
+_stream = torch._C._cuda_getCurrentRawStream
+
+# bs_kv_rows and bs_kv_query of include/bigsmall_kv.h, packed: a ctypes structure of as many fields takes 1 us more to fill
+_ROWS = struct.Struct("=6Q6q4I")
+_QUERY = struct.Struct("=6Q2q2I2f")
+assert _ROWS.size == ctypes.sizeof(_native.BsKvRows) and _QUERY.size == ctypes.sizeof(_native.BsKvQuery)
+
+
+def _call(name: str, pool: KVPool, *args) -> None:
+    """A C entry point on the pool's device and its current stream."""
+    index = pool.index
+    if index == torch.cuda.current_device():
+        rc = getattr(_native.lib(), name)(pool.ref, *args, _stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = getattr(_native.lib(), name)(pool.ref, *args, _stream(index))
+    if rc:
+        _native.check(rc, name)
 
 
 def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None, out=None, status=None):
@@ -189,38 +212,36 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
     device.StatusWord that gets BS_DEV_ERR_BOUNDS where the batch names pages, tails or positions that
     do not exist; such parts are not written."""
     _check_batch(pool, batch)
-    k = _rows("k", k, None, pool.n_kv_heads, pool)
-    t = k.shape[0]
-    v = _rows("v", v, t, pool.n_kv_heads, pool)
-    rot, cos, sin, inter, n_pos, heads = 0, 0, 0, 0, 0, 0
+    k, t, _, kp, k0, k1 = _rows("k", k, None, pool.n_kv_heads, pool)
+    v, _, _, vp, v0, v1 = _rows("v", v, t, pool.n_kv_heads, pool)
+    rot = cos = sin = inter = n_pos = heads = qp = op = q0 = q1 = 0
     if rope is not None:
-        rot, inter, n_pos = rope.rot, rope.interleaved, rope.cos.shape[0]
+        rot, inter, n_pos, cos, sin = rope.rot, rope.interleaved, rope.positions, rope.cos_ptr, rope.sin_ptr
         if rot > pool.head_dim:
             raise ValueError(f"rope turns {rot} channels, the head dim is {pool.head_dim}")
         if n_pos < batch.max_len:
             raise ValueError(f"rope has {n_pos} positions, the batch reaches {batch.max_len}")
-        if rope.cos.device != pool.device:
+        if rope.index != pool.index:
             raise ValueError(f"rope is on {rope.cos.device}, the cache is on {pool.device}")
-        cos, sin = rope.cos.data_ptr(), rope.sin.data_ptr()
-    qp, op, q_token, q_head = 0, 0, 0, 0
     result = q
     if q is not None:
-        q = _rows("q", q, t, None, pool)
-        heads = _q_heads(q, pool)
+        q, _, heads, qp, q0, q1 = _rows("q", q, t, None, pool)
+        _check_heads(heads, pool)
         if rot or out is not None:
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif _rows("out", out, t, heads, pool) is not out or not out.is_contiguous():
-                raise ValueError("out must be contiguous and 16-byte aligned")
-            qp, op, q_token, q_head = q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1)
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                op = out.data_ptr()
+            else:
+                copy, _, _, op, _, _ = _rows("out", out, t, heads, pool)
+                if copy is not out or not out.is_contiguous():
+                    raise ValueError("out must be contiguous and 16-byte aligned")
             result = out
-    if t == 0:
-        return result
-    rows = _native.BsKvRows(qp, k.data_ptr(), v.data_ptr(), op, cos, sin, q_token, q_head, k.stride(0), k.stride(1),
-                            v.stride(0), v.stride(1), heads, rot, inter, n_pos)
-    rc = _native.lib().bs_kv_append(_byref(pool.c), _byref(batch.for_rows(t)), _byref(rows), status.ptr if status else None,
-                                    torch.cuda.current_stream(pool.device).cuda_stream)
-    _native.check(rc, "bs_kv_append")
+        else:
+            qp = 0
+    if t:
+        batch.c.n_rows = t
+        _call("bs_kv_append", pool, batch.ref, _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
+              status.ptr if status else None)
     return result
 
 
@@ -236,29 +257,33 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     row and j > p - window; prefix: int32 [B], first: int32 [T], window 0: none. A row that sees
     nothing gives 0 and -inf."""
     _check_batch(pool, batch)
-    q = _rows("q", q, None, None, pool)
-    heads, t = _q_heads(q, pool), q.shape[0]
+    q, t, heads, qp, q0, q1 = _rows("q", q, None, None, pool)
+    _check_heads(heads, pool)
     if not 0 <= window < 1 << 31 or not 0.0 <= softcap < float("inf"):
         raise ValueError("window and softcap must not be negative or infinite")
-    for name, x, n, kind in (("slopes", slopes, heads, torch.float32), ("prefix", prefix, batch.n_seqs, torch.int32),
-                             ("first", first, t, torch.int32)):
-        if x is not None and not _tensor(name, x, kind, pool.device, (n,)).is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    sp = pp = fp = 0
+    if slopes is not None:
+        sp = _vector("slopes", slopes, heads, torch.float32, pool)
+    if prefix is not None:
+        pp = _vector("prefix", prefix, batch.n_seqs, torch.int32, pool)
+    if first is not None:
+        fp = _vector("first", first, t, torch.int32, pool)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((t, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if t:
-        L, b, p = _native.lib(), _byref(batch.for_rows(t)), _byref(pool.c)
-        query = _native.BsKvQuery(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                                  slopes.data_ptr() if slopes is not None else 0,
-                                  prefix.data_ptr() if prefix is not None else 0,
-                                  first.data_ptr() if first is not None else 0, q.stride(0), q.stride(1), heads, window,
-                                  pool.head_dim ** -0.5 if scale is None else scale, softcap)
-        n = L.bs_kv_attend_work_bytes(p, b, heads)
+        batch.c.n_rows = t
+        n = _native.lib().bs_kv_attend_work_bytes(pool.ref, batch.ref, heads)
         work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        rc = L.bs_kv_attend(p, b, _byref(query), work.data_ptr() if n else 0, n, status.ptr if status else None,
-                            torch.cuda.current_stream(pool.device).cuda_stream)
-        _native.check(rc, "bs_kv_attend")
+        query = _QUERY.pack(qp, out.data_ptr(), lse.data_ptr() if return_lse else 0, sp, pp, fp, q0, q1, heads, window,
+                            pool.head_dim ** -0.5 if scale is None else scale, softcap)
+        _call("bs_kv_attend", pool, batch.ref, query, work.data_ptr() if n else 0, n, status.ptr if status else None)
     return (out, lse) if return_lse else out
+
+
+def _vector(name: str, x, n: int, dtype, pool: KVPool) -> int:
+    if not _tensor(name, x, dtype, pool.device, (n,)).is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return x.data_ptr()
 
 
 def kv_read(pool: KVPool, pages, n: int, tail, status=None):
@@ -268,16 +293,14 @@ def kv_read(pool: KVPool, pages, n: int, tail, status=None):
     _gpu(pool)
     _tensor("pages", pages, torch.int32, pool.device)
     _tensor("tail", tail, torch.int32, pool.device)
-    if pages.dim() != 1 or not pages.is_contiguous() or tail.numel() < 1:
+    shape = pages.shape
+    if len(shape) != 1 or not pages.is_contiguous() or tail.numel() < 1:
         raise ValueError("kv_read: pages must be a contiguous row, tail must hold a number")
-    if not 0 <= n < 1 << 30 or n // PAGE > pages.shape[0]:
-        raise ValueError(f"kv_read: {n} tokens need {n // PAGE} full pages, {pages.shape[0]} given")
+    if not 0 <= n < 1 << 30 or n // PAGE > shape[0]:
+        raise ValueError(f"kv_read: {n} tokens need {n // PAGE} full pages, {shape[0]} given")
     k = torch.empty((pool.n_kv_heads, n, pool.head_dim), dtype=torch.bfloat16, device=pool.device)
     v = torch.empty_like(k)
-    rc = _native.lib().bs_kv_read(_byref(pool.c), pages.data_ptr(), pages.shape[0], tail.data_ptr(), n, k.data_ptr(),
-                                  v.data_ptr(), status.ptr if status else None,
-                                  torch.cuda.current_stream(pool.device).cuda_stream)
-    _native.check(rc, "bs_kv_read")
+    _call("bs_kv_read", pool, pages.data_ptr(), shape[0], tail.data_ptr(), n, k.data_ptr(), v.data_ptr(), status.ptr if status else None)
     return k, v
 
 

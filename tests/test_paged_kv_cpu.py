@@ -136,7 +136,9 @@ def test_calls_refuse_what_does_not_fit(on_gpu):
 def test_c_entries_refuse_bad_arguments():
     """Every refusal comes before any launch, so these run without a GPU."""
     L = _native.lib()
-    ok_pool, ok_batch = KVPool(*_parts()).c, _batch().for_rows(2)
+    keep = KVPool(*_parts()), _batch()                # (they own the memory)
+    ok_pool, ok_batch = (x.c for x in keep)
+    ok_batch.n_rows = 2
     P, ARG = ctypes.byref, _native.BS_ERR_ARG
     x = _aligned(2, 8, 64, dtype=torch.bfloat16)
 
