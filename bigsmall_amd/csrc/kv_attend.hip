@@ -70,7 +70,7 @@ __device__ __forceinline__ bool takes(Take take, int rows, int few) { return tak
 __device__ __forceinline__ int2 seen_by(const bs_kv_query& A, const SeqStep& s, uint32_t b, int i) {
   const int pos = s.start + i;
   int lo = 0, hi = pos + 1;
-  if (A.prefix) hi = max(hi, min(A.prefix[b], s.len));
+  if (A.prefix) hi = max(hi, min(uniform_load(A.prefix, b), s.len));
   if (A.first) lo = max(lo, A.first[s.t0 + i]);
   if (A.window && (uint32_t)pos >= A.window) lo = max(lo, pos - (int)A.window + 1);
   return make_int2(min(lo, hi), hi);
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
   const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
 
   SeqStep s;
-  if (!seq_step(B, b, s)) {
+  if (!seq_step<true>(B, b, s)) {
     if (threadIdx.x == 0) report(status, BS_DEV_ERR_BOUNDS);
     return;
   }
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
   const uint32_t h = blockIdx.x % P.n_kv_heads, split = blockIdx.x / P.n_kv_heads, b = blockIdx.z;
   const uint32_t group = A.n_q_heads / P.n_kv_heads;
   SeqStep s;
-  if (!seq_step(B, b, s)) {
+  if (!seq_step<true>(B, b, s)) {
     if (tid == 0) report(status, BS_DEV_ERR_BOUNDS);
     return;
   }
@@ -879,7 +879,7 @@ __global__ __launch_bounds__(256) void join_kernel(bs_kv_pool P, bs_kv_batch B, 
   uint32_t row = WAVES_A_ROW == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
   if (few) {
     SeqStep s;
-    if (!seq_step(B, blockIdx.y, s) || s.n * (int)(A.n_q_heads / P.n_kv_heads) > few || row >= (uint32_t)s.n * A.n_q_heads) return;
+    if (!seq_step<true>(B, blockIdx.y, s) || s.n * (int)(A.n_q_heads / P.n_kv_heads) > few || row >= (uint32_t)s.n * A.n_q_heads) return;
     row += (uint32_t)s.t0 * A.n_q_heads;
   }
   if (row >= n || W.ml[row].y < 0.0f) return;            // none, or written by its kernel
@@ -951,11 +951,20 @@ struct Plan {
 };
 
 constexpr uint64_t RESIDENT = 512;       // workgroups of 256 threads that run at once, two on each of 256 compute units
-constexpr uint64_t PIECES_WANTED = 512;
 
 uint32_t split_for(uint64_t blocks, uint64_t want, uint64_t pages, uint64_t least) {
   const uint64_t n = blocks >= want ? 1 : (want + blocks - 1) / blocks;
   return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(n, pages / least));
+}
+
+// Pieces of a cache of `pages` pages, `blocks` tiles of rows in all: as many as fill the card, of 4 pages (one a wave)
+// at least, and of 16 once there are 32, since every piece costs the joining kernel. Up to 16 pages a workgroup is done
+// before a second kernel has begun. (One row, heads of 128, 8 kv heads, us a call with one piece / pieces of 4 / 8 / 16
+// pages: 1,000 tokens 13.5 / 16.2 / 16.3 / 13.5, 4,000 tokens 36.8 / 17.0 / 18.9 / 23.5, 16,000 tokens - / 22.1 / 20.2 / 22.5,
+// 32,000 tokens - / 26.8 / 28.6 / 24.4.)
+uint32_t pieces_for(uint64_t blocks, uint64_t pages) {
+  if (pages <= 16) return 1;
+  return split_for(blocks, RESIDENT, std::min<uint64_t>(pages / 4, std::max<uint64_t>(32, pages / 16)), 1);
 }
 
 Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
@@ -971,7 +980,7 @@ Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
   if (rows <= FEW_ROWS || seqs > 1) {
     const uint64_t most = std::min<uint64_t>(rows, FEW_ROWS);
     p.row_tiles = (uint32_t)((most + 15) / 16);
-    p.pieces = split_for(p.row_tiles * heads * seqs, PIECES_WANTED, pages, WAVES);
+    p.pieces = pieces_for(p.row_tiles * heads * seqs, pages);
     p.piece = (uint32_t)std::max<uint64_t>((pages + p.pieces - 1) / p.pieces, 1);
   }
   if (p.prompt_tiles && p.row_tiles) p.rows_take = FEW, p.prompt_take = MANY;

@@ -77,10 +77,12 @@ __device__ __forceinline__ T uniform_load(const T* p, size_t i) {
 struct SeqStep {
   int t0, n, start, len;  // first new row, new rows, cached tokens before, tokens after
 };
+// SAME: b is the same in all lanes.
+template <bool SAME = false>
 __device__ __forceinline__ bool seq_step(const bs_kv_batch& B, uint32_t b, SeqStep& s) {
-  s.t0 = B.cu[b];
-  const int t1 = B.cu[b + 1];
-  s.start = B.start[b];
+  s.t0 = SAME ? uniform_load(B.cu, b) : B.cu[b];
+  const int t1 = SAME ? uniform_load(B.cu, (size_t)b + 1) : B.cu[b + 1];
+  s.start = SAME ? uniform_load(B.start, b) : B.start[b];
   s.n = t1 - s.t0;
   const int room = (int)(B.table_cols * PAGE);
   const bool ok = s.t0 >= 0 && t1 >= s.t0 && t1 <= (int)B.n_rows && s.start >= 0 && s.start <= room && s.n <= room - s.start;
