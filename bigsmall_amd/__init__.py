@@ -12,6 +12,7 @@ kernels on the GPU:
     decompress_delta(delta, base), load_delta(delta, base) -> a fine-tune from its XOR delta
     CompressedKVCache                       -> KV entries and blocks decoded on the GPU
     PagedKVCache, kv_append, kv_attend, kv_read -> a paged 8-bit KV cache filled, attended to and read back on the GPU
+    paged_llama.PagedLlama                  -> a Llama-architecture model generating from it, layers streamed
     codec_registry.register_codec / get_codec / auto_select_codec
     compress_for_hub(model_dir, out_dir), from_pretrained(path) -> multi-shard .bs models + index
     migrate.migrate(path)                   -> re-encode a container into the GPU formats where smaller
@@ -40,6 +41,9 @@ def __getattr__(name):
     if name == "BigSmallStreamingModel":
         from .streaming_inference import BigSmallStreamingModel
         return BigSmallStreamingModel
+    if name == "PagedLlama":
+        from .paged_llama import PagedLlama
+        return PagedLlama
     if name == "StreamingGPT2":
         from .streaming_model import StreamingGPT2
         return StreamingGPT2

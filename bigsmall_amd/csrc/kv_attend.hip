@@ -678,31 +678,9 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
     const float slope = !PLAIN && biased ? A.slopes[hq] * LOG2E : 0.0f;
 
     const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
-    half8v q16[STEPS];
-    float row_scale;
-    {
-      uint16_t x[STEPS][8];
-      float top = 0;
-      bool fine = true;
+    uint4 raw[STEPS];
 #pragma unroll
-      for (int c = 0; c < STEPS; ++c) {
-        const uint4 w = real ? *(const uint4*)(q + 16 * c + 8 * half) : make_uint4(0, 0, 0, 0);
-        __builtin_memcpy(x[c], &w, 16);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          fine = fine && bf16_finite(x[c][e]);
-          top = fmaxf(top, fabsf(bf16_to_f32(x[c][e])));
-        }
-      }
-      top = pair_max(top);
-      const bool ok = pair_max(fine ? 0.0f : 1.0f) == 0.0f;
-      const int e2 = (top == 0.0f || !ok) ? 0 : max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
-      row_scale = ok ? ldexpf(1.0f, e2) : __uint_as_float(0x7FC00000u);
-#pragma unroll
-      for (int c = 0; c < STEPS; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[c][e]), -e2)) : (_Float16)0.0f;
-    }
+    for (int c = 0; c < STEPS; ++c) raw[c] = real ? *(const uint4*)(q + 16 * c + 8 * half) : make_uint4(0, 0, 0, 0);
 
     // keys that any row of the wave, and of the workgroup, sees
     int lo = see.x < see.y ? see.x : 0x7FFFFFFF, hi = see.x < see.y ? see.y : 0;
@@ -722,13 +700,6 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
     const int begin = __builtin_amdgcn_readfirstlane(page_lo + per * (int)split);
     const int end = __builtin_amdgcn_readfirstlane(min(begin + per, page_hi));
     const int full_end = min(end, full_pages);
-
-    f32x16 o[TILES];
-#pragma unroll
-    for (int d = 0; d < TILES; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[d][e] = 0;
-    float m = NEG_INF, l = 0;
 
     // Page numbers and scales come through vector loads, in line with the pages' own: number n is asked for with page
     // n - 1, scales with their page, so that nothing waits for them. Past the end: the last page again.
@@ -752,6 +723,39 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
       coming = number(begin);
       fetch(begin);
     }
+    // with the first page on its way: the row of q as f16, scaled by a power of two to lie below 2
+    half8v q16[STEPS];
+    float row_scale;
+    {
+      uint16_t x[STEPS][8];
+      float top = 0;
+      bool fine = true;
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c) {
+        __builtin_memcpy(x[c], &raw[c], 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          fine = fine && bf16_finite(x[c][e]);
+          top = fmaxf(top, fabsf(bf16_to_f32(x[c][e])));
+        }
+      }
+      top = pair_max(top);
+      const bool ok = pair_max(fine ? 0.0f : 1.0f) == 0.0f;
+      const int e2 = (top == 0.0f || !ok) ? 0 : max((int)((__float_as_uint(top) >> 23) & 255) - 127, -100);
+      row_scale = ok ? ldexpf(1.0f, e2) : __uint_as_float(0x7FC00000u);
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q16[c][e] = ok ? (_Float16)(sign * ldexpf(bf16_to_f32(x[c][e]), -e2)) : (_Float16)0.0f;
+    }
+
+    f32x16 o[TILES];
+#pragma unroll
+    for (int d = 0; d < TILES; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[d][e] = 0;
+    float m = NEG_INF, l = 0;
+
     for (int page = begin; page < full_end; ++page) {
       uint8_t* buf = lds + ((page - begin) & 1) * Tile<D>::BYTES;
       st.store(buf, tid);
@@ -975,9 +979,12 @@ Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
     p.prompt_tiles = (uint32_t)std::min<uint64_t>((rows + PROMPT_ROWS - 1) / PROMPT_ROWS, 65535);
     // tiles that the sequences can have in all, if max_new is what it says
     const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(p.prompt_tiles * seqs, B->n_rows * group / PROMPT_ROWS + seqs), 1);
-    p.prompt_splits = split_for(tiles * heads, RESIDENT, pages, 8);
+    p.prompt_splits = split_for(tiles * heads, P->head_dim > 128 ? RESIDENT / 2 : RESIDENT, pages, 8);
   }
-  if (rows <= FEW_ROWS || seqs > 1) {
+  // the fewest new rows a sequence can have: what the caller says, or what the others cannot have between them
+  const uint64_t rest = (seqs - 1) * (uint64_t)B->max_new;
+  const uint64_t least = std::max<uint64_t>(B->min_new, B->n_rows > rest ? B->n_rows - rest : 0);
+  if (rows <= FEW_ROWS || (seqs > 1 && least * group <= FEW_ROWS)) {
     const uint64_t most = std::min<uint64_t>(rows, FEW_ROWS);
     p.row_tiles = (uint32_t)((most + 15) / 16);
     p.pieces = pieces_for(p.row_tiles * heads * seqs, pages);

@@ -1,0 +1,96 @@
+"""PagedLlama: a Llama-architecture model that generates from a paged KV cache,
+its layers streamed from a BigSmall container.
+
+The reference streams layers through the HuggingFace module and keeps its
+bf16 cache (bigsmall/streaming_inference.py:77-347); here a step takes the new
+tokens of any number of sequences at once (whole prompts, parts of prompts and
+single tokens side by side), and K and V go rotated into a PagedKVCache in 8
+bits, from which attention reads them.
+
+The rest of a layer is the architecture's own arithmetic in torch: RMS norm,
+projections without bias, SwiGLU. Tensor names follow the HuggingFace layout:
+`model.embed_tokens`, `model.layers.<i>.*`, `model.norm`, `lm_head`.
+"""
+from __future__ import annotations
+
+import torch
+from torch.nn.functional import linear, silu
+
+from .paged_kv import PagedKVCache, Rope
+
+
+class PagedLlama:
+    """loader: a StreamingLoader on a GPU; its `prefetch` sets how many layers decode ahead.
+    config: the model's transformers.LlamaConfig (plain rotation; scaled variants: pass `rope`).
+    pages, sequences: what the cache holds at most; kind: torch.int8 or torch.float8_e4m3fn."""
+
+    def __init__(self, loader, config, pages: int, sequences: int, kind=torch.int8, rope: Rope | None = None):
+        self.loader, self.config = loader, config
+        self.heads, self.kv_heads = config.num_attention_heads, config.num_key_value_heads
+        self.dim = getattr(config, "head_dim", None) or config.hidden_size // self.heads
+        top = loader.load_non_layer_tensors()
+        self.embed, self.norm = top["model.embed_tokens.weight"], top["model.norm.weight"]
+        self.head = top.get("lm_head.weight", self.embed)
+        self.device = self.embed.device
+        self.cache = PagedKVCache(loader.layer_count(), self.kv_heads, self.dim, pages, sequences, kind, self.device)
+        if rope is None:
+            theta = getattr(config, "rope_theta", None) or config.rope_parameters["rope_theta"]
+            rope = Rope.from_theta(self.dim, config.max_position_embeddings, theta, device=self.device)
+        self.rope = rope
+
+    def _norm(self, x, weight):
+        y = x.float()
+        return weight * (y * torch.rsqrt(y.square().mean(-1, keepdim=True) + self.config.rms_norm_eps)).to(x.dtype)
+
+    @torch.no_grad()
+    def forward(self, new: dict) -> torch.Tensor:
+        """new: {sequence: its new token ids (1-D)}; sequences come from `self.cache.add()`. Returns the
+        logits [sequences, vocab] after each sequence's last new token, in the dict's order."""
+        ids = [torch.as_tensor(t).to(self.device) for t in new.values()]
+        step = self.cache.step({seq: len(t) for seq, t in zip(new, ids)})
+        x = self.embed[torch.cat(ids)]
+        t = x.shape[0]
+        for i, layer in self.loader.iter_layers(progress=False):
+            p = f"model.layers.{i}."
+            y = self._norm(x, layer[p + "input_layernorm.weight"])
+            q, k, v = (linear(y, layer[p + f"self_attn.{n}_proj.weight"]).view(t, -1, self.dim) for n in "qkv")
+            q = self.cache.append(i, step, q, k, v, self.rope)
+            y = self.cache.attend(i, step, q)
+            x = x + linear(y.view(t, -1), layer[p + "self_attn.o_proj.weight"])
+            y = self._norm(x, layer[p + "post_attention_layernorm.weight"])
+            y = silu(linear(y, layer[p + "mlp.gate_proj.weight"])) * linear(y, layer[p + "mlp.up_proj.weight"])
+            x = x + linear(y, layer[p + "mlp.down_proj.weight"])
+        last = step.cu[1:].long() - 1
+        return linear(self._norm(x[last], self.norm), self.head)
+
+    def generate(self, prompts: list, max_new_tokens: int) -> list:
+        """Greedy continuations of prompts (1-D token ids), all in one batch."""
+        seqs = [self.cache.add() for _ in prompts]
+        try:
+            logits, out = self.forward(dict(zip(seqs, prompts))), []
+            for n in range(max_new_tokens):
+                out.append(logits.argmax(-1))
+                if n + 1 < max_new_tokens:
+                    logits = self.forward({s: out[-1][j:j + 1] for j, s in enumerate(seqs)})
+            return list(torch.stack(out, 1)) if out else [torch.empty(0, dtype=torch.int64) for _ in prompts]
+        finally:
+            for s in seqs:
+                self.cache.drop(s)
+
+    def park(self, seq: int, store) -> None:
+        """Move a sequence's K and V, as bf16, into a CompressedKVCache under (seq, layer) and drop it here."""
+        for i in range(len(self.cache.pools)):
+            store.set((seq, i), *self.cache.read(i, seq))
+        self.cache.drop(seq)
+
+    def resume(self, seq: int, store) -> int:
+        """Bring a parked sequence back: its K and V are already rotated. Returns its new number."""
+        new, step = self.cache.add(), None
+        for i in range(len(self.cache.pools)):
+            k, v = (x.transpose(0, 1).to(self.device) for x in store.get((seq, i)))
+            step = step or self.cache.step({new: k.shape[0]})
+            self.cache.append(i, step, None, k, v)
+        return new
+
+
+__all__ = ["PagedLlama"]
