@@ -60,6 +60,7 @@ struct Work {
   uint32_t splits;     // prompt_kernel: into how many parts it splits every tile's pages
   uint32_t pieces;     // rows_kernel: into how many at most, of how many pages
   int piece;
+  bool ranked;         // rows_kernel: more workgroups than run at once
 };
 
 // Which sequences a kernel takes: those with few rows, with many, or all.
@@ -252,9 +253,11 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
   constexpr int STEPS = Dims<D>::STEPS, TILES = Dims<D>::TILES;
   constexpr int PART = D < 128 ? D : 128, PARTS = D / PART;      // channels joined at a time
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-  // consecutive workgroups go to the eight dies in turn: pieces, of which short sequences have few, come last
-  const uint32_t h = blockIdx.x % P.n_kv_heads, b = blockIdx.y, slot = blockIdx.z;
+  // Consecutive workgroups go to the eight dies in turn, which so get heads and not sequences. Where not all run at once,
+  // the longest start first: the later parts of long sequences, then sequences by length, among 64 at a time.
+  const uint32_t h = blockIdx.x % P.n_kv_heads, slot = gridDim.z - 1 - blockIdx.z;
   const uint32_t group = A.n_q_heads / P.n_kv_heads, row_tiles = gridDim.x / P.n_kv_heads;
+  uint32_t b = blockIdx.y;
   __shared__ __attribute__((aligned(16))) float part_o[WAVES][16][PART + 4];
   __shared__ float part_m[WAVES][16], part_l[WAVES][16];
   const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
@@ -263,7 +266,24 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
   const size_t unit = (size_t)P.n_kv_heads * PAGE * D, head = (size_t)h * PAGE * D;
 
   SeqStep s;
-  if (!seq_step<true>(B, b, s)) {
+  bool sound;
+  if (W.ranked) {
+    const uint32_t b0 = b & ~63u, n = min(B.n_seqs - b0, 64u);
+    s = {0, 0, 0, 0};
+    sound = (uint32_t)lane >= n || seq_step(B, b0 + (uint32_t)lane, s);
+    // no two keys are alike, whatever the lengths: each rank below n is one lane's
+    const uint32_t key = (uint32_t)s.len * 64 + 63 - (uint32_t)lane;
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < n; ++j) rank += (uint32_t)__builtin_amdgcn_readlane((int)key, (int)j) > key;
+    const int l = __builtin_ctzll(__ballot(rank == b - b0 && (uint32_t)lane < n));
+    sound = __builtin_amdgcn_readlane((int)sound, l) != 0;
+    s = {__builtin_amdgcn_readlane(s.t0, l), __builtin_amdgcn_readlane(s.n, l), __builtin_amdgcn_readlane(s.start, l),
+         __builtin_amdgcn_readlane(s.len, l)};
+    b = b0 + (uint32_t)l;
+  } else {
+    sound = seq_step<true>(B, b, s);
+  }
+  if (!sound) {
     if (threadIdx.x == 0) report(status, BS_DEV_ERR_BOUNDS);
     return;
   }
@@ -290,7 +310,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     const int page_hi = __builtin_amdgcn_readfirstlane(lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE);
     const uint32_t parts = min((uint32_t)max((page_hi - page_lo + W.piece - 1) / W.piece, 1), W.pieces);
     if (slot >= parts) continue;
-    const int mine = page_lo + W.piece * (int)slot, end = slot + 1 == parts ? page_hi : mine + W.piece;
+    const int piece = (page_hi - page_lo + (int)parts - 1) / (int)parts;
+    const int mine = min(page_lo + piece * (int)slot, page_hi), end = min(mine + piece, page_hi);
     const int full_pages = s.len / (int)PAGE, full_end = min(end, full_pages);      // pages from full_pages on are the tail
 
     // The tail, 16 keys of it a wave, and the first page are on their way before q is looked at. Key 4 g + e of the
@@ -1011,7 +1032,8 @@ template <int D, int KIND>
 int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
-  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.slots, p.prompt_splits, p.pieces, (int)p.piece};
+  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.slots, p.prompt_splits, p.pieces, (int)p.piece,
+            (uint64_t)p.row_tiles * P->n_kv_heads * B->n_seqs * p.pieces > RESIDENT && B->n_seqs > 1};
   if (p.prompt_tiles) {
     const dim3 grid(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs);
     if (Q->softcap == 0.0f && !Q->slopes) prompt_launch<D, KIND, true>(P, B, Q, w, p.prompt_take, status, stream, grid);

@@ -83,10 +83,10 @@ __device__ __forceinline__ bool seq_step(const bs_kv_batch& B, uint32_t b, SeqSt
   s.t0 = SAME ? uniform_load(B.cu, b) : B.cu[b];
   const int t1 = SAME ? uniform_load(B.cu, (size_t)b + 1) : B.cu[b + 1];
   s.start = SAME ? uniform_load(B.start, b) : B.start[b];
-  s.n = t1 - s.t0;
   const int room = (int)(B.table_cols * PAGE);
-  const bool ok = s.t0 >= 0 && t1 >= s.t0 && t1 <= (int)B.n_rows && s.start >= 0 && s.start <= room && s.n <= room - s.start;
-  if (!ok) s.n = 0;
+  const bool ok = s.t0 >= 0 && t1 >= s.t0 && t1 <= (int)B.n_rows && s.start >= 0 && s.start <= room && t1 - s.t0 <= room - s.start;
+  if (!ok) s.start = 0;
+  s.n = ok ? t1 - s.t0 : 0;
   s.len = s.start + s.n;
   return ok;
 }

@@ -274,6 +274,26 @@ def test_attend_long_caches_and_prompts(kind, starts, news, hk, group, d):
     _check_attend(rig, q, out, lse, 0.07, first=first, softcap=30.0)
 
 
+@pytest.mark.parametrize("most", [1, 90])
+def test_attend_many_sequences_of_all_lengths(most):
+    """More workgroups than run at once, sequences without new rows and of one token among them."""
+    import bigsmall_amd as bs
+    g = _gen(21)
+    b, hk = 140, 4
+    starts = torch.randint(0, 300, (b,), generator=g).tolist()
+    news = torch.randint(0, 2, (b,), generator=g).tolist() if most == 1 else (torch.randint(0, most + 1, (b,), generator=g) // 10).tolist()
+    starts[3], news[3], news[7], news[-1] = 0, 1, most, 0
+    rig = Rig(starts, news, hk, 64, torch.int8, seed=5)
+    q = rig.rows(hk * 2)
+    out, lse = bs.kv_attend(rig.pool, rig.batch, q.cuda(), return_lse=True)
+    _check_attend(rig, q, out, lse, 64 ** -0.5)
+    # what the batch says of its sizes chooses the launches, not the results
+    for most_new, longest, least in ((1, 1, 0), (most, 20000, 0), (400, 400, 0), (max(news), max(news), max(news))):
+        other = bs.KVBatch(rig.batch.start, rig.batch.cu, rig.batch.table, rig.batch.tails, most_new, longest, least)
+        out, lse = bs.kv_attend(rig.pool, other, q.cuda(), return_lse=True)
+        _check_attend(rig, q, out, lse, 64 ** -0.5)
+
+
 @pytest.mark.parametrize("news", [[1, 1], [70, 130]])
 def test_attend_scales_of_very_different_pages(news):
     """Pages whose values differ by many powers of two, zero pages among them, and rows of q as different."""
