@@ -78,7 +78,7 @@ class BsKvPool(ctypes.Structure):
 
 class BsKvBatch(ctypes.Structure):
     _fields_ = [(n, _P) for n in ("start", "cu", "table", "tails")] + \
-               [(n, _U32) for n in ("n_seqs", "table_stride", "table_cols", "n_rows", "max_new", "max_len", "min_new")]
+               [(n, _U32) for n in ("n_seqs", "table_stride", "table_cols", "n_rows", "max_new", "max_len")]
 
 
 class BsKvRows(ctypes.Structure):

@@ -1,9 +1,9 @@
 // Attention over the paged 8-bit KV cache.
 //
 // The rows of a sequence and kv head are its new tokens times the q heads of
-// the group, row r = token r / G, head r % G. Sequences with few rows go to
-// rows_kernel, with many to prompt_kernel; join_kernel puts together what was
-// split over the cache's length.
+// the group, row r = token r / G, head r % G. A step whose sequences have few
+// rows goes to rows_kernel, any other to prompt_kernel (both take any number);
+// join_kernel puts together what was split over the cache's length.
 //
 // rows_kernel: tiles of 16 rows. A wave takes one page at a time:
 //   S^T = K Q^T   (64 keys x 16 rows; K's codes as f16, exactly)
@@ -49,23 +49,16 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 constexpr int WAVES = 4;      // of a workgroup of rows_kernel
 
-// Split results: per slot and row O (f32, not divided), m, l; `slots` is 1 if
-// nothing of the call is split. A row has all its slots marked: parts without
-// keys with m = -inf and l = 0; a row that was not split is written by its
-// kernel itself, which leaves l = -1.
+// Split results: per part and row O (f32, not divided), m, l. All parts of a
+// row are marked: those without keys with m = -inf and l = 0; a row that was not
+// split is written by its kernel itself, which leaves l = -1 in the first.
 struct Work {
   float* o;
   float2* ml;
-  uint32_t slots;
-  uint32_t splits;     // prompt_kernel: into how many parts it splits every tile's pages
-  uint32_t pieces;     // rows_kernel: into how many at most, of how many pages
-  int piece;
+  uint32_t parts;      // that the pages which a tile of rows sees are cut into at most: 1 if nothing is split
+  int piece;           // rows_kernel: pages of a part
   bool ranked;         // rows_kernel: more workgroups than run at once
 };
-
-// Which sequences a kernel takes: those with few rows, with many, or all.
-enum Take { FEW, MANY, ALL };
-__device__ __forceinline__ bool takes(Take take, int rows, int few) { return take == ALL || (rows <= few) == (take == FEW); }
 
 // Interval of keys that row (token i of the sequence) sees.
 __device__ __forceinline__ int2 seen_by(const bs_kv_query& A, const SeqStep& s, uint32_t b, int i) {
@@ -214,10 +207,10 @@ __device__ __forceinline__ void mark_row(const bs_kv_query& A, const bs_kv_batch
   if (parts > 1) {
     W.ml[slot * n + row] = make_float2(m, l);
     if (slot == 0)
-      for (uint32_t k = parts; k < W.slots; ++k) W.ml[k * n + row] = make_float2(NEG_INF, 0.0f);
+      for (uint32_t k = parts; k < W.parts; ++k) W.ml[k * n + row] = make_float2(NEG_INF, 0.0f);
   } else {
     if (A.lse) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
-    if (W.slots > 1) W.ml[row] = make_float2(NEG_INF, -1.0f);
+    if (W.parts > 1) W.ml[row] = make_float2(NEG_INF, -1.0f);
   }
 }
 
@@ -248,15 +241,15 @@ struct PageList {
 // reads the next page's K as soon as this one's is multiplied, and its V after this one's: between 8 and 16 KiB a wave
 // are always under way (heads of 128).
 template <int D, int KIND>
-__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
+__global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W,
                                                                            int32_t* status) {
   constexpr int STEPS = Dims<D>::STEPS, TILES = Dims<D>::TILES;
   constexpr int PART = D < 128 ? D : 128, PARTS = D / PART;      // channels joined at a time
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   // Consecutive workgroups go to the eight dies in turn, which so get heads and not sequences. Where not all run at once,
   // the longest start first: the later parts of long sequences, then sequences by length, among 64 at a time.
-  const uint32_t h = blockIdx.x % P.n_kv_heads, slot = gridDim.z - 1 - blockIdx.z;
-  const uint32_t group = A.n_q_heads / P.n_kv_heads, row_tiles = gridDim.x / P.n_kv_heads;
+  const uint32_t h = blockIdx.x, slot = gridDim.z - 1 - blockIdx.z;
+  const uint32_t group = A.n_q_heads / P.n_kv_heads;
   uint32_t b = blockIdx.y;
   __shared__ __attribute__((aligned(16))) float part_o[WAVES][16][PART + 4];
   __shared__ float part_m[WAVES][16], part_l[WAVES][16];
@@ -288,10 +281,9 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     return;
   }
   const int rows = s.n * (int)group;
-  if (!takes(take, rows, few)) return;
   const int32_t* table = B.table + (size_t)b * B.table_stride;
 
-  for (int tile = blockIdx.x / P.n_kv_heads; tile * 16 < rows; tile += row_tiles) {
+  for (int tile = 0; tile * 16 < rows; ++tile) {
     const int r = tile * 16 + (lane & 15);
     const bool real = r < rows;
     const int i = real ? r / (int)group : 0;
@@ -308,7 +300,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     }
     const int page_lo = __builtin_amdgcn_readfirstlane(lo >= hi ? 0 : lo / (int)PAGE);
     const int page_hi = __builtin_amdgcn_readfirstlane(lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE);
-    const uint32_t parts = min((uint32_t)max((page_hi - page_lo + W.piece - 1) / W.piece, 1), W.pieces);
+    const uint32_t parts = min((uint32_t)max((page_hi - page_lo + W.piece - 1) / W.piece, 1), W.parts);
     if (slot >= parts) continue;
     const int piece = (page_hi - page_lo + (int)parts - 1) / (int)parts;
     const int mine = min(page_lo + piece * (int)slot, page_hi), end = min(mine + piece, page_hi);
@@ -667,7 +659,7 @@ __device__ __forceinline__ void prompt_weights(f32x16 (&s)[2], f32x16 (&o)[Tile<
 
 // PLAIN: no cap, no bias.
 template <int D, int KIND, bool PLAIN>
-__global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, Take take, int few,
+__global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W,
                                                                       int32_t* status) {
   constexpr int STEPS = Tile<D>::STEPS, TILES = Tile<D>::TILES;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -681,7 +673,6 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
     return;
   }
   const int rows = s.n * (int)group;
-  if (!takes(take, rows, few)) return;
   const float sign = A.scale < 0.0f ? -1.0f : 1.0f;
   const Score sc = {fabsf(A.softcap != 0.0f ? A.scale / A.softcap : A.scale * LOG2E), A.softcap * LOG2E};
   const bool biased = A.slopes != nullptr;
@@ -717,7 +708,7 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
 #pragma unroll
     for (int w = 0; w < PROMPT_WAVES; ++w) lo = min(lo, bounds[0][w]), hi = max(hi, bounds[1][w]);
     const int page_lo = lo >= hi ? 0 : lo / (int)PAGE, page_hi = lo >= hi ? 0 : (hi + (int)PAGE - 1) / (int)PAGE;
-    const int per = (page_hi - page_lo + (int)W.splits - 1) / (int)W.splits;
+    const int per = (page_hi - page_lo + (int)W.parts - 1) / (int)W.parts;
     const int begin = __builtin_amdgcn_readfirstlane(page_lo + per * (int)split);
     const int end = __builtin_amdgcn_readfirstlane(min(begin + per, page_hi));
     const int full_end = min(end, full_pages);
@@ -868,8 +859,8 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
     l = pair_sum(l);
     if (real) {
       const size_t out_row = (size_t)(s.t0 + i) * A.n_q_heads + hq;
-      if (half == 0) mark_row(A, B, W, split, W.splits, out_row, m + (P_SHIFT - SHIFT), l);
-      if (W.splits == 1 || begin < end) {
+      if (half == 0) mark_row(A, B, W, split, W.parts, out_row, m + (P_SHIFT - SHIFT), l);
+      if (W.parts == 1 || begin < end) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         float* part = W.o + ((size_t)split * B.n_rows * A.n_q_heads + out_row) * D;
 #pragma unroll
@@ -878,7 +869,7 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
           for (int a = 0; a < 4; ++a) {
             const int ch = 32 * d + 8 * a + 4 * half;
             if (ch >= D) continue;
-            if (W.splits > 1) {
+            if (W.parts > 1) {
               *(float4*)(part + ch) = make_float4(o[d][4 * a], o[d][4 * a + 1], o[d][4 * a + 2], o[d][4 * a + 3]);
             } else {
               uint2 w;
@@ -893,26 +884,20 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
 }
 
 // Rows' parts from all splits into the output, WAVES_A_ROW waves (1 or 4) a row: they deal the slots among them, 64 at a
-// time; lane k looks at its wave's slot k, then all lanes add up the slots that hold something. few > 0: only the rows
-// of sequences with at most that many rows a kv head are split (blockIdx.y: the sequence).
+// time; lane k looks at its wave's slot k, then all lanes add up the slots that hold something.
 template <int D, int WAVES_A_ROW>
-__global__ __launch_bounds__(256) void join_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W, int few) {
+__global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32_t n) {
   constexpr int EACH = (D + 63) / 64, AT_ONCE = 8;
   __shared__ float part_x[4][EACH * 64], part_m[4], part_l[4];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = B.n_rows * A.n_q_heads;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t share = WAVES_A_ROW == 4 ? wave : 0;
-  uint32_t row = WAVES_A_ROW == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
-  if (few) {
-    SeqStep s;
-    if (!seq_step<true>(B, blockIdx.y, s) || s.n * (int)(A.n_q_heads / P.n_kv_heads) > few || row >= (uint32_t)s.n * A.n_q_heads) return;
-    row += (uint32_t)s.t0 * A.n_q_heads;
-  }
+  const uint32_t row = WAVES_A_ROW == 4 ? blockIdx.x : blockIdx.x * 4 + wave;
   if (row >= n || W.ml[row].y < 0.0f) return;            // none, or written by its kernel
   float m = NEG_INF, l = 0, x[EACH] = {};
-  for (uint32_t k0 = 0; k0 < W.slots; k0 += 64 * WAVES_A_ROW) {
+  for (uint32_t k0 = 0; k0 < W.parts; k0 += 64 * WAVES_A_ROW) {
     const uint32_t mine = k0 + lane * WAVES_A_ROW + share;
     float2 ml = make_float2(NEG_INF, 0.0f);
-    if (mine < W.slots) ml = W.ml[(size_t)mine * n + row];
+    if (mine < W.parts) ml = W.ml[(size_t)mine * n + row];
     const float now = fmaxf(m, wave_max(ml.x)), ref = now == NEG_INF ? 0.0f : now;
     const float back = exp2_fast(m - ref), f = exp2_fast(ml.x - ref);
     m = now;
@@ -965,14 +950,16 @@ __global__ __launch_bounds__(256) void join_kernel(bs_kv_pool P, bs_kv_batch B, 
   if (A.lse && lane == 0) A.lse[row] = l == 0.0f ? NEG_INF : (m - P_SHIFT + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// Launch shapes of a call. FEW_ROWS: rows of a sequence and kv head up to which rows_kernel takes it.
+// Launch shapes of a call. FEW_ROWS: rows of a sequence and kv head up to which rows_kernel takes a step. (64 sequences
+// of up to 8,192 tokens, 4 rows, us: 131 there, 193 in prompt_kernel; of up to 12,000, 4 to 16 rows: 206 and 265. With
+// more than one tile of rows it would read every page again. Where sequences differ, prompt_kernel takes all of them: the
+// same caches with 4 to 32 rows 275 us, against 410 with the two kernels one after the other.)
 constexpr uint32_t FEW_ROWS = 16;
 
 struct Plan {
-  Take rows_take, prompt_take;
-  uint32_t row_tiles, pieces, piece;     // rows_kernel; 0 tiles: not launched
-  uint32_t prompt_tiles, prompt_splits;  // prompt_kernel; 0 tiles: not launched
-  uint32_t slots;
+  bool few;              // rows_kernel, else prompt_kernel
+  uint32_t tiles;        // of 16 or PROMPT_ROWS rows, of the sequence that has most
+  uint32_t parts, piece; // pages are cut into at most so many parts; rows_kernel: of so many pages
 };
 
 constexpr uint64_t RESIDENT = 512;       // workgroups of 256 threads that run at once, two on each of 256 compute units
@@ -994,61 +981,50 @@ uint32_t pieces_for(uint64_t blocks, uint64_t pages) {
 
 Plan make_plan(const bs_kv_pool* P, const bs_kv_batch* B, uint32_t n_q_heads) {
   const uint64_t group = n_q_heads / P->n_kv_heads, heads = P->n_kv_heads, seqs = B->n_seqs;
-  const uint64_t rows = std::max<uint64_t>(B->max_new * group, 1), pages = (B->max_len + PAGE - 1) / PAGE;
-  Plan p = {ALL, ALL, 0, 1, 1, 0, 1, 1};
-  if (rows > FEW_ROWS) {
-    p.prompt_tiles = (uint32_t)std::min<uint64_t>((rows + PROMPT_ROWS - 1) / PROMPT_ROWS, 65535);
-    // tiles that the sequences can have in all, if max_new is what it says
-    const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(p.prompt_tiles * seqs, B->n_rows * group / PROMPT_ROWS + seqs), 1);
-    p.prompt_splits = split_for(tiles * heads, P->head_dim > 128 ? RESIDENT / 2 : RESIDENT, pages, 8);
+  const uint64_t rows = std::max<uint64_t>(B->max_new * group, 1), pages = std::max<uint64_t>((B->max_len + PAGE - 1) / PAGE, 1);
+  Plan p = {rows <= FEW_ROWS, 1, 1, 0};
+  if (p.few) {
+    p.parts = pieces_for(heads * seqs, pages);
+    p.piece = (uint32_t)((pages + p.parts - 1) / p.parts);
+  } else {
+    p.tiles = (uint32_t)std::min<uint64_t>((rows + PROMPT_ROWS - 1) / PROMPT_ROWS, 65535);
+    // tiles that the sequences can have in all, if max_new is what it says; one workgroup a compute unit with heads of 256
+    const uint64_t tiles = std::max<uint64_t>(std::min<uint64_t>(p.tiles * seqs, B->n_rows * group / PROMPT_ROWS + seqs), 1);
+    p.parts = split_for(tiles * heads, P->head_dim > 128 ? RESIDENT / 2 : RESIDENT, pages, 8);
   }
-  // the fewest new rows a sequence can have: what the caller says, or what the others cannot have between them
-  const uint64_t rest = (seqs - 1) * (uint64_t)B->max_new;
-  const uint64_t least = std::max<uint64_t>(B->min_new, B->n_rows > rest ? B->n_rows - rest : 0);
-  if (rows <= FEW_ROWS || (seqs > 1 && least * group <= FEW_ROWS)) {
-    const uint64_t most = std::min<uint64_t>(rows, FEW_ROWS);
-    p.row_tiles = (uint32_t)((most + 15) / 16);
-    p.pieces = pieces_for(p.row_tiles * heads * seqs, pages);
-    p.piece = (uint32_t)std::max<uint64_t>((pages + p.pieces - 1) / p.pieces, 1);
-  }
-  if (p.prompt_tiles && p.row_tiles) p.rows_take = FEW, p.prompt_take = MANY;
-  p.slots = std::max(p.pieces, p.prompt_splits);
   return p;
 }
 
 uint64_t split_rows(const bs_kv_batch* B, uint32_t n_q_heads, const Plan& p) {
-  return p.slots > 1 ? (uint64_t)p.slots * B->n_rows * n_q_heads : 0;
+  return p.parts > 1 ? (uint64_t)p.parts * B->n_rows * n_q_heads : 0;
 }
 
 template <int D, int KIND, bool PLAIN>
-void prompt_launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, const Work& w, Take take, int32_t* status,
-                   hipStream_t stream, dim3 grid) {
+void prompt_launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, const Work& w, int32_t* status, hipStream_t stream,
+                   dim3 grid) {
   static std::atomic<uint64_t> done{0};
   bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND, PLAIN>, 2 * Tile<D>::BYTES, done);
-  prompt_kernel<D, KIND, PLAIN><<<grid, PROMPT_THREADS, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, take, (int)FEW_ROWS, status);
+  prompt_kernel<D, KIND, PLAIN><<<grid, PROMPT_THREADS, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, status);
 }
 
 template <int D, int KIND>
 int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
-  Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.slots, p.prompt_splits, p.pieces, (int)p.piece,
-            (uint64_t)p.row_tiles * P->n_kv_heads * B->n_seqs * p.pieces > RESIDENT && B->n_seqs > 1};
-  if (p.prompt_tiles) {
-    const dim3 grid(P->n_kv_heads * p.prompt_splits, p.prompt_tiles, B->n_seqs);
-    if (Q->softcap == 0.0f && !Q->slopes) prompt_launch<D, KIND, true>(P, B, Q, w, p.prompt_take, status, stream, grid);
-    else prompt_launch<D, KIND, false>(P, B, Q, w, p.prompt_take, status, stream, grid);
+  const bool ranked = (uint64_t)P->n_kv_heads * B->n_seqs * p.parts > RESIDENT && B->n_seqs > 1;
+  const Work w = {(float*)work, (float2*)((char*)work + rows * D * 4), p.parts, (int)p.piece, ranked};
+  if (p.few) {
+    rows_kernel<D, KIND><<<dim3(P->n_kv_heads, B->n_seqs, p.parts), 64 * WAVES, 0, stream>>>(*P, *B, *Q, w, status);
+  } else {
+    const dim3 grid(P->n_kv_heads * p.parts, p.tiles, B->n_seqs);
+    if (Q->softcap == 0.0f && !Q->slopes) prompt_launch<D, KIND, true>(P, B, Q, w, status, stream, grid);
+    else prompt_launch<D, KIND, false>(P, B, Q, w, status, stream, grid);
   }
-  if (p.row_tiles)
-    rows_kernel<D, KIND><<<dim3(p.row_tiles * P->n_kv_heads, B->n_seqs, p.pieces), 64 * WAVES, 0, stream>>>(*P, *B, *Q, w, p.rows_take, (int)FEW_ROWS,
-                                                                                                        status);
-  if (p.slots > 1) {
-    // where only short sequences are split, only their rows are looked at
-    const int few = p.rows_take == FEW && p.prompt_splits == 1 ? (int)FEW_ROWS : 0;
-    const uint32_t n = few ? FEW_ROWS * P->n_kv_heads : B->n_rows * Q->n_q_heads, seqs = few ? B->n_seqs : 1;
-    // Four waves a row from 8 slots on (64 rows of 64 slots: 6 us against 13 with one).
-    if (p.slots > 8) join_kernel<D, 4><<<dim3(n, seqs), 256, 0, stream>>>(*P, *B, *Q, w, few);
-    else join_kernel<D, 1><<<dim3((n + 3) / 4, seqs), 256, 0, stream>>>(*P, *B, *Q, w, few);
+  if (p.parts > 1) {
+    const uint32_t n = B->n_rows * Q->n_q_heads;
+    // Four waves a row from 8 parts on (64 rows of 64 parts: 5 us, with one wave 25).
+    if (p.parts > 8) join_kernel<D, 4><<<n, 256, 0, stream>>>(*Q, w, n);
+    else join_kernel<D, 1><<<(n + 3) / 4, 256, 0, stream>>>(*Q, w, n);
   }
   return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
 }

@@ -90,13 +90,13 @@ class KVBatch:
     tails [B, 2]   the tail before the step and after it; where the step completes a page they
                    must differ (a step run again then reads what it read before)
     max_new, max_len: the largest number of new tokens and of tokens after the step of a
-    sequence; min_new: the smallest number of new tokens, 0 if not known. They choose launch
-    shapes; a wrong value costs time, not results.
+    sequence. They choose launch shapes; a wrong value costs time, not results. Rows of q, k
+    and v that no sequence covers are not read, and their outputs are not defined.
     """
 
     __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "c", "ref")
 
-    def __init__(self, start, cu, table, tails, max_new: int, max_len: int, min_new: int = 0):
+    def __init__(self, start, cu, table, tails, max_new: int, max_len: int):
         _tensor("start", start, torch.int32)
         if start.dim() != 1:
             raise ValueError("KVBatch: start must be [sequences]")
@@ -109,12 +109,12 @@ class KVBatch:
         stride = table.stride(0) if b > 1 else max(table.stride(0), table.shape[1])
         if not (start.is_contiguous() and cu.is_contiguous() and tails.is_contiguous()) or stride < table.shape[1]:
             raise ValueError("KVBatch: start, cu and tails must be contiguous, table's rows apart")
-        if b > 65535 or not 0 <= min_new <= max_new < 1 << 30 or not 0 <= max_len < 1 << 30:
-            raise ValueError("KVBatch: at most 65535 sequences; min_new <= max_new, max_len below 2^30")
+        if b > 65535 or not 0 <= max_new < 1 << 30 or not 0 <= max_len < 1 << 30:
+            raise ValueError("KVBatch: at most 65535 sequences, max_new and max_len below 2^30")
         self.start, self.cu, self.table, self.tails = start, cu, table, tails
         self.n_seqs, self.max_new, self.max_len = b, int(max_new), int(max_len)
         self.c = _native.BsKvBatch(start.data_ptr(), cu.data_ptr(), table.data_ptr(), tails.data_ptr(), b, stride,
-                                   table.shape[1], 0, int(max_new), int(max_len), int(min_new))
+                                   table.shape[1], 0, int(max_new), int(max_len))
         self.ref, self.index = ctypes.byref(self.c), start.get_device()
 
 
@@ -363,7 +363,7 @@ class PagedKVCache:
         flat = torch.tensor(arrays, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
         b, m = shape
         start, cu, tails, table = flat.split([b, b + 1, 2 * b, b * m])
-        return KVBatch(start, cu, table.view(b, m), tails.view(b, 2), max_new, max_len, min(new.values()))
+        return KVBatch(start, cu, table.view(b, m), tails.view(b, 2), max_new, max_len)
 
     # ---- one layer
     def append(self, layer: int, step: KVBatch, q, k, v, rope: Optional[Rope] = None):

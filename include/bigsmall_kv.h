@@ -43,9 +43,9 @@ typedef struct {
 } bs_kv_pool;
 
 /* One step over a batch of sequences, device memory. max_new and max_len are
- * the largest of their kind over the sequences, min_new the smallest number of
- * new rows (0: not known); they choose launch shapes and do not bound the work
- * (a wrong value costs time, not results). */
+ * the largest of their kind over the sequences; they choose launch shapes and
+ * do not bound the work (a wrong value costs time, not results). Rows that no
+ * sequence covers are not read, and their outputs are not defined. */
 typedef struct {
     const int32_t *start; /* [n_seqs] tokens in the cache before the step */
     const int32_t *cu;    /* [n_seqs + 1] first new row of each sequence, ascending from 0 */
@@ -54,7 +54,7 @@ typedef struct {
                              completes a page they differ, else they may be one */
     uint32_t n_seqs, table_stride, table_cols;
     uint32_t n_rows;      /* new rows in all */
-    uint32_t max_new, max_len, min_new;
+    uint32_t max_new, max_len;
 } bs_kv_batch;
 
 /* bf16 rows [n_rows][heads][head_dim]; strides in elements, multiples of 8,

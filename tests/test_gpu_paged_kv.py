@@ -288,8 +288,8 @@ def test_attend_many_sequences_of_all_lengths(most):
     out, lse = bs.kv_attend(rig.pool, rig.batch, q.cuda(), return_lse=True)
     _check_attend(rig, q, out, lse, 64 ** -0.5)
     # what the batch says of its sizes chooses the launches, not the results
-    for most_new, longest, least in ((1, 1, 0), (most, 20000, 0), (400, 400, 0), (max(news), max(news), max(news))):
-        other = bs.KVBatch(rig.batch.start, rig.batch.cu, rig.batch.table, rig.batch.tails, most_new, longest, least)
+    for most_new, longest in ((1, 1), (most, 20000), (400, 400), (max(news), max(news))):
+        other = bs.KVBatch(rig.batch.start, rig.batch.cu, rig.batch.table, rig.batch.tails, most_new, longest)
         out, lse = bs.kv_attend(rig.pool, other, q.cuda(), return_lse=True)
         _check_attend(rig, q, out, lse, 64 ** -0.5)
 
