@@ -1,15 +1,19 @@
 // Filling and reading back the paged 8-bit KV cache.
 //
 // bs_kv_append: one workgroup per (page that the step touches, kv head). It
-// rotates the K rows and the q rows of the head's group, and holds the page's K
+// rotates the q rows of the head's group and the K rows, and holds the page's K
 // in registers and its V, as bf16, in LDS, where V turns from rows of channels
 // into rows of tokens. If the step completes the page, the largest |x| of K and
 // of V give its scales and both go out as codes; the page's earlier tokens come
 // from the sequence's old tail. Otherwise the new tokens go into the tail. A
 // page is written by one workgroup in one go, so nothing is summed across
-// workgroups and a step run again writes the same bytes.
+// workgroups and a step run again writes the same bytes. The bound is memory: q
+// in and out, k and v in, 8-bit codes out. 32,768 tokens of 32 and 8 heads of 128:
+// 161 us, 4.7 TB/s, where a large copy reaches 5.1. One token: 4.5 us of kernel,
+// two dependent reads (the step's lengths, then rows and angles) and the launch.
 //
-// bs_kv_read: one workgroup per (page, kv head), codes times scale.
+// bs_kv_read: one workgroup per (page, kv head), codes times scale; V turns back
+// in LDS. 32,768 tokens, 8 heads of 128: 45 us from memory, 4.5 TB/s.
 #include "kv_common.h"
 
 #include <algorithm>

@@ -236,10 +236,15 @@ struct PageList {
   __device__ __forceinline__ float scale_v(int i) const { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(vs), i)); }
 };
 
-// A tile of 16 rows of a sequence and kv head, and `piece` of the pages that it sees: pieces of one size for all
-// sequences, so that long ones do not make long pieces. The workgroup deals its pages to the four waves in turn. A wave
-// reads the next page's K as soon as this one's is multiplied, and its V after this one's: between 8 and 16 KiB a wave
-// are always under way (heads of 128).
+// A tile of 16 rows of a sequence and kv head, and a part of the pages that it sees: about `piece` pages each, one size
+// for all sequences, so that long ones do not make long parts. The workgroup deals its pages to the four waves in turn.
+// A wave reads the next page's K as soon as this one's is multiplied, and its V after this one's: between 8 and 16 KiB a
+// wave are always under way (heads of 128), 64 to 128 KiB a compute unit. The bound is memory: 2 D bytes a key against
+// 4 D flops a row, and at 16 rows the matrix unit and the conversions still take a quarter of the time that the bytes
+// do. 128 sequences of 15,000 to 16,383 tokens, 8 kv heads of 128: 641 us, 6.4 TB/s; 64 sequences of up to 8,192: 131 us,
+// 4.2 TB/s (one workgroup a sequence and head just fills the card, and the longest goes on alone); a single row over
+// 1,024 tokens 12.5 us, which is the chain of dependent reads: the step, page numbers, pages. 168 registers a wave, for
+// three waves a SIMD instead of two, spill and cost a third.
 template <int D, int KIND>
 __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W,
                                                                            int32_t* status) {
@@ -491,15 +496,20 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
   }
 }
 
-// Many rows: a workgroup of four waves takes 128 rows of a sequence and kv head,
-// 32 a wave, and goes through their pages together. Each page is converted to
-// f16 once, on its way into LDS (two buffers, one barrier a page, the next
-// page's loads in flight meanwhile), and read from there by all four waves as
-// the left operand of 32x32x16 products. Keys are numbered so that the 16 keys
-// of a lane in a 32-key S^T tile are two runs of 8, which are its part of the
-// right operand of two products with V^T: key bits 2 and 3 change places
-// between a tile's row and the key in it. LDS rows have an odd number of 16-byte
-// pieces, so that the 8 lanes of one LDS cycle hit different banks.
+// Many rows: a workgroup of four waves takes 128 rows of a sequence and kv head, 32 a wave, and goes through their pages
+// together. Each page is converted to f16 once, on its way into LDS (two buffers, one barrier a page, the next page's
+// loads in flight meanwhile), and read from there by all four waves as the left operand of 32x32x16 products. Keys are
+// numbered so that the 16 keys of a lane in a 32-key S^T tile are two runs of 8, which are its part of the right operand
+// of two products with V^T: key bits 2 and 3 change places between a tile's row and the key in it. LDS rows have an odd
+// number of 16-byte pieces, so that the 8 lanes of one LDS cycle hit different banks.
+//
+// Two workgroups a compute unit (one with heads of 256, whose o alone is 128 registers a lane). A page costs a wave 32
+// products (heads of 128), about 500 ns of the matrix unit, and some 260 other vector instructions, 32 exponentials and 32
+// conversions among them; the bound is how far the two waves of a SIMD run one beside the other. 8,192-token causal prompt,
+// 32 and 8 heads of 128, e4m3: 585 us, 0.93 PFLOP/s, where a large f16 product of the library reaches 1.23; the products
+// alone take 320. 500 tokens over a window of 16,384, heads of 256, capped: 225 us, 0.6 PFLOP/s. Eight waves and 256 rows
+// a workgroup: 573 us there, but 90 us instead of 45 for short documents. One wave a SIMD with the next page's scores
+// woven into this page's weights: 800 us.
 constexpr int PROMPT_WAVES = 4, PROMPT_ROWS = 32 * PROMPT_WAVES, PROMPT_THREADS = 64 * PROMPT_WAVES;
 
 // The maximum of x over the two lanes that share a row (32 apart).
@@ -883,8 +893,8 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
   }
 }
 
-// Rows' parts from all splits into the output, WAVES_A_ROW waves (1 or 4) a row: they deal the slots among them, 64 at a
-// time; lane k looks at its wave's slot k, then all lanes add up the slots that hold something.
+// Rows' parts into the output, WAVES_A_ROW waves (1 or 4) a row: they deal the parts among them, 64 at a time; lane k
+// looks at its wave's k-th, then all lanes add up those that hold something, eight loads at a time. Latency: 3 to 5 us.
 template <int D, int WAVES_A_ROW>
 __global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32_t n) {
   constexpr int EACH = (D + 63) / 64, AT_ONCE = 8;
