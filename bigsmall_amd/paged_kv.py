@@ -137,8 +137,8 @@ class Rope:
     @classmethod
     def from_theta(cls, rot: int, positions: int, theta: float = 10000.0, interleaved: bool = False, device="cuda") -> "Rope":
         """Angles position * theta^(-2i / rot), computed in 64 bits."""
-        freq = float(theta) ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
-        angle = torch.arange(positions, dtype=torch.float64)[:, None] * freq
+        freq = float(theta) ** (-torch.arange(0, rot, 2, dtype=torch.float64, device="cpu") / rot)
+        angle = torch.arange(positions, dtype=torch.float64, device="cpu")[:, None] * freq
         return cls(angle.cos().float().to(device), angle.sin().float().to(device), interleaved)
 
 
@@ -360,7 +360,7 @@ class PagedKVCache:
         pages it needs (RuntimeError, and nothing taken, if there are too few). Appending must follow for
         every layer before the sequences' next step."""
         arrays, shape, max_new, max_len = self._books.step(new)
-        flat = torch.tensor(arrays, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        flat = torch.tensor(arrays, dtype=torch.int32, device="cpu").pin_memory().to(self.device, non_blocking=True)
         b, m = shape
         start, cu, tails, table = flat.split([b, b + 1, 2 * b, b * m])
         return KVBatch(start, cu, table.view(b, m), tails.view(b, 2), max_new, max_len)
@@ -375,7 +375,7 @@ class PagedKVCache:
     def read(self, layer: int, seq: int):
         """K and V of a sequence's appended tokens, bf16 [kv heads, tokens, dim]."""
         n, pages, tail = self._books.where(seq)
-        row = torch.tensor(pages + [tail], dtype=torch.int32).to(self.device)
+        row = torch.tensor(pages + [tail], dtype=torch.int32, device="cpu").to(self.device)
         return kv_read(self.pools[layer], row[:-1], n, row[-1:])
 
 

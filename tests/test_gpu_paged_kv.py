@@ -274,6 +274,36 @@ def test_attend_long_caches_and_prompts(kind, starts, news, hk, group, d):
     _check_attend(rig, q, out, lse, 0.07, first=first, softcap=30.0)
 
 
+@pytest.mark.parametrize("start,new,d", [(20011, 2, 64), (17000, 20, 64), (16500, 1, 128)])
+def test_attend_when_the_batch_says_too_little(start, new, d):
+    """One workgroup for a cache of over 256 pages, and the kernel for few rows with many and for many with few."""
+    import bigsmall_amd as bs
+    rig = Rig([start], [new], 1, d, torch.int8, seed=start)
+    q = rig.rows(2)
+    for most_new, longest in ((1, 1), (1, start), (500, 1), (500, start + new)):
+        batch = bs.KVBatch(rig.batch.start, rig.batch.cu, rig.batch.table, rig.batch.tails, most_new, longest)
+        out, lse = bs.kv_attend(rig.pool, batch, q.cuda(), return_lse=True)
+        _check_attend(rig, q, out, lse, d ** -0.5)
+
+
+def test_cache_under_a_gpu_default_device():
+    import bigsmall_amd as bs
+    g = _gen(9)
+    k = _bf16((70, 1, 64), g).cuda()
+    outs = []
+    for device in ("cpu", "cuda"):
+        torch.set_default_device(device)
+        try:
+            cache = bs.PagedKVCache(1, 1, 64, pages=4, sequences=1)
+            seq = cache.add()
+            step = cache.step({seq: 70})
+            q = cache.append(0, step, k, k, k, bs.Rope.from_theta(64, 100))
+            outs.append((cache.attend(0, step, q), *cache.read(0, seq)))
+        finally:
+            torch.set_default_device("cpu")
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 @pytest.mark.parametrize("most", [1, 90])
 def test_attend_many_sequences_of_all_lengths(most):
     """More workgroups than run at once, sequences without new rows and of one token among them."""
