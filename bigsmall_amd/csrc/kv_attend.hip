@@ -314,7 +314,8 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     // The tail, 16 keys of it a wave, and the first page are on their way before q is looked at. Key 4 g + e of the
     // wave's 16 belongs to lane group g, in S^T and as the right operand of the second product (of whose eight elements
     // a lane the last four are 0). Slots after the sequence's end hold anything: they count as 0.
-    const bool tailed = end > full_pages;
+    // (mine < end: a part that is left without pages, where there are more than the plan was made for, has no tail either.)
+    const bool tailed = mine < end && end > full_pages;
     const int used = tailed ? s.len - full_pages * (int)PAGE - 16 * wave : 0;       // of this wave's 16
     uint4 kt[STEPS];
     uint2 vt[TILES];
