@@ -316,17 +316,18 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
     // a lane the last four are 0). Slots after the sequence's end hold anything: they count as 0.
     // (mine < end: a part that is left without pages, where there are more than the plan was made for, has no tail either.)
     const bool tailed = mine < end && end > full_pages;
-    const int used = tailed ? s.len - full_pages * (int)PAGE - 16 * wave : 0;       // of this wave's 16
+    uint32_t tail = 0;
+    if (tailed) {
+      tail = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
+      if (tail >= P.n_tails && threadIdx.x == 0) report(status, BS_DEV_ERR_BOUNDS);
+    }
+    // of this wave's 16; a tail that does not exist is left out
+    const int used = tailed && tail < P.n_tails ? s.len - full_pages * (int)PAGE - 16 * wave : 0;
     uint4 kt[STEPS];
     uint2 vt[TILES];
     const uint4 none = make_uint4(0, 0, 0, 0);
     if (used > 0) {
-      uint32_t id = (uint32_t)uniform_load(B.tails, 2 * (size_t)b + 1);
-      if (id >= P.n_tails) {
-        if (lane == 0) report(status, BS_DEV_ERR_BOUNDS);
-        id = 0;
-      }
-      const uint16_t *const kr = P.k_tail + id * unit + head + 16 * wave * D, *const vr = P.v_tail + id * unit + head + 16 * wave;
+      const uint16_t *const kr = P.k_tail + tail * unit + head + 16 * wave * D, *const vr = P.v_tail + tail * unit + head + 16 * wave;
       const uint32_t row = (uint32_t)(lane & 15) * D, ahead = (uint32_t)(lane & 15) * PAGE + 4 * (uint32_t)g;
 #pragma unroll
       for (int c = 0; c < STEPS; ++c) {
