@@ -76,9 +76,22 @@ struct Score {
   float cap;      // softcap * log2 e, 0: none
 };
 
-__device__ __forceinline__ float capped(float x, float cap) {      // cap * tanh(x)
+// cap * tanh(x), two ways. Up to QUICK_CAP: cap - 2 cap / (e^2x + 1), off by 2^-22 of the cap, so by 2^-16 at most, a
+// sixteenth of what rounding the weights to f16 takes. Larger caps: within 2^-21 of its own value. 1 - 2 / (e^2|x| + 1)
+// takes small results from two ones, so that below 1/2 an odd polynomial stands in for it (x + x^3 P(x^2), P of degree 3
+// with the least largest relative error there, 2^-25.9). (us with quick / whole:
+// one row over 1,024 tokens 13.1 / 15.1, an 8,192-token prompt with heads of 128 690 / 829, 500 tokens over a window of
+// 16,384 with heads of 256 222 / 284.)
+constexpr float QUICK_CAP = 64.0f;
+__device__ __forceinline__ float quick_capped(float x, float cap) {
   const float e = exp2_fast(x * (2.0f * LOG2E));
   return cap - cap * 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+}
+__device__ __forceinline__ float whole_tanh(float x) {
+  const float a = fabsf(x), t = x * x;
+  const float p = fmaf(t, fmaf(t, fmaf(t, 0.017241491f, -0.053045493f), 0.13325879f), -0.33333144f);
+  const float far = 1.0f - 2.0f * __builtin_amdgcn_rcpf(exp2_fast(a * (2.0f * LOG2E)) + 1.0f);
+  return a < 0.5f ? fmaf(x * t, p, x) : copysignf(far, x);
 }
 
 template <int D>
@@ -154,7 +167,14 @@ struct State {
 template <int N>
 __device__ __forceinline__ void scores(f32x4 (&s)[N], const Score& sc, float row_scale, float page_scale, float shift,
                                        int j0, int2 see, bool inside, bool biased, float slope, int pos) {
-  const float c = row_scale * (page_scale * sc.scale);
+  float c = row_scale * (page_scale * sc.scale);
+  if (sc.cap > QUICK_CAP * LOG2E) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] = sc.cap * whole_tanh(s[t][i] * c);
+    c = 1.0f;
+  }
   int lo = see.x - j0, hi = see.y - j0;
   float d = (float)(pos - j0);
   BS_OPAQUE(lo);
@@ -165,7 +185,7 @@ __device__ __forceinline__ void scores(f32x4 (&s)[N], const Score& sc, float row
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float x = s[t][i] * c;
-      if (sc.cap != 0.0f) x = capped(x, sc.cap);
+      if (sc.cap != 0.0f && sc.cap <= QUICK_CAP * LOG2E) x = quick_capped(x, sc.cap);
       const int j = 4 * t + i;
       if (biased) x -= slope * fabsf(d - (float)j);
       x += shift;
@@ -587,13 +607,23 @@ __device__ __forceinline__ void products(Read read, Multiply multiply) {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Scores of 64 keys (two S^T tiles) as they come from the products, into what is left to multiply by c and add to:
-// caps, biases and masks where there are any. j0: this lane's first key.
-template <bool PLAIN>
+// What prompt_kernel is compiled for: no cap and no bias; a cap of at most QUICK_CAP, a bias or both; a larger cap.
+enum Caps { PLAIN, QUICK, WHOLE };
+
+// Scores of 64 keys (two S^T tiles) as they come from the products, into what is left to multiply by c and to add to
+// (QUICK: the cap): caps, biases and masks where there are any. j0: this lane's first key.
+template <int CAPS>
 __device__ __forceinline__ void prompt_scores(f32x16 (&s)[2], float& c, const Score& sc, bool inside, int j0, int2 see, bool biased,
                                               float slope, int pos) {
-  if constexpr (!PLAIN) {
-    if (sc.cap != 0.0f) {          // cap * tanh(x) = cap - 2 cap / (e^2x + 1): the quotient here, cap in the last step
+  if constexpr (CAPS == WHOLE) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[t][i] = whole_tanh(s[t][i] * c);
+    c = sc.cap;
+  }
+  if constexpr (CAPS != PLAIN) {
+    if (CAPS == QUICK && sc.cap != 0.0f) {       // the quotient here, cap in the last step
       const float k = c * (2.0f * LOG2E);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -669,8 +699,7 @@ __device__ __forceinline__ void prompt_weights(f32x16 (&s)[2], f32x16 (&o)[Tile<
   l += all == 0.0f ? 0.0f : all * inv_vs;
 }
 
-// PLAIN: no cap, no bias.
-template <int D, int KIND, bool PLAIN>
+template <int D, int KIND, int CAPS>
 __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) void prompt_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W,
                                                                       int32_t* status) {
   constexpr int STEPS = Tile<D>::STEPS, TILES = Tile<D>::TILES;
@@ -699,7 +728,7 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
     const uint32_t hq = h * group + (uint32_t)(real ? r % (int)group : 0);
     const int pos = s.start + i;
     int2 see = real ? seen_by(A, s, b, i) : make_int2(0, 0);
-    const float slope = !PLAIN && biased ? A.slopes[hq] * LOG2E : 0.0f;
+    const float slope = CAPS != PLAIN && biased ? A.slopes[hq] * LOG2E : 0.0f;
 
     const uint16_t* q = A.q + (int64_t)(s.t0 + i) * A.q_token + (int64_t)hq * A.q_head;
     uint4 raw[STEPS];
@@ -800,8 +829,8 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
                           [&](int n, half8v a) { acc[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q16[n / 2], acc[n % 2], 0, 0, 0); });
       const bool inside = __ballot(real && (j0 < see.x || j0 + (int)PAGE > see.y)) == 0;
       float c = row_scale * (ks * sc.scale);
-      prompt_scores<PLAIN>(acc, c, sc, inside, j0 + 8 * half, see, biased, slope, pos);
-      prompt_weights<D>(acc, o, m, l, c, shift + sc.cap, exp2_fast(-shift));
+      prompt_scores<CAPS>(acc, c, sc, inside, j0 + 8 * half, see, biased, slope, pos);
+      prompt_weights<D>(acc, o, m, l, c, CAPS == WHOLE ? shift : shift + sc.cap, exp2_fast(-shift));
       half8v p[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
@@ -842,8 +871,8 @@ __global__ __launch_bounds__(PROMPT_THREADS, D <= 128 ? 8 / PROMPT_WAVES : 1) vo
 #pragma unroll
           for (int t = 0; t < 2; ++t) acc[t] = -acc[t];
         float c = row_scale == row_scale ? sc.scale : row_scale;
-        prompt_scores<PLAIN>(acc, c, sc, false, full_pages * (int)PAGE + 8 * half, see, biased, slope, pos);
-        prompt_weights<D>(acc, o, m, l, c, sc.cap, 1.0f);
+        prompt_scores<CAPS>(acc, c, sc, false, full_pages * (int)PAGE + 8 * half, see, biased, slope, pos);
+        prompt_weights<D>(acc, o, m, l, c, CAPS == WHOLE ? 0.0f : sc.cap, 1.0f);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           bf16x8 p_hi, p_lo;
@@ -1011,16 +1040,21 @@ uint64_t split_rows(const bs_kv_batch* B, uint32_t n_q_heads, const Plan& p) {
   return p.parts > 1 ? (uint64_t)p.parts * B->n_rows * n_q_heads : 0;
 }
 
-template <int D, int KIND, bool PLAIN>
+template <int D, int KIND, int CAPS>
 void prompt_launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, const Work& w, int32_t* status, hipStream_t stream,
                    dim3 grid) {
   static std::atomic<uint64_t> done{0};
-  bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND, PLAIN>, 2 * Tile<D>::BYTES, done);
-  prompt_kernel<D, KIND, PLAIN><<<grid, PROMPT_THREADS, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, status);
+  bs_internal::ensure_lds_limit((const void*)prompt_kernel<D, KIND, CAPS>, 2 * Tile<D>::BYTES, done);
+  prompt_kernel<D, KIND, CAPS><<<grid, PROMPT_THREADS, 2 * Tile<D>::BYTES, stream>>>(*P, *B, *Q, w, status);
 }
 
 template <int D, int KIND>
-int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void* work, int32_t* status, hipStream_t stream) {
+int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* given, void* work, int32_t* status, hipStream_t stream) {
+  // A cap outside [2^-60, 2^60] does to f32 scores what the nearer end does (below 2^48 they pass whole; all become 0), and
+  // the quotients by it would leave f32's range.
+  bs_kv_query query = *given;
+  if (query.softcap != 0.0f) query.softcap = std::min(std::max(query.softcap, 0x1p-60f), 0x1p60f);
+  const bs_kv_query* const Q = &query;
   const Plan p = make_plan(P, B, Q->n_q_heads);
   const uint64_t rows = split_rows(B, Q->n_q_heads, p);
   const bool ranked = (uint64_t)P->n_kv_heads * B->n_seqs * p.parts > RESIDENT && B->n_seqs > 1;
@@ -1029,8 +1063,9 @@ int launch(const bs_kv_pool* P, const bs_kv_batch* B, const bs_kv_query* Q, void
     rows_kernel<D, KIND><<<dim3(P->n_kv_heads, B->n_seqs, p.parts), 64 * WAVES, 0, stream>>>(*P, *B, *Q, w, status);
   } else {
     const dim3 grid(P->n_kv_heads * p.parts, p.tiles, B->n_seqs);
-    if (Q->softcap == 0.0f && !Q->slopes) prompt_launch<D, KIND, true>(P, B, Q, w, status, stream, grid);
-    else prompt_launch<D, KIND, false>(P, B, Q, w, status, stream, grid);
+    if (Q->softcap > QUICK_CAP) prompt_launch<D, KIND, WHOLE>(P, B, Q, w, status, stream, grid);
+    else if (Q->softcap != 0.0f || Q->slopes) prompt_launch<D, KIND, QUICK>(P, B, Q, w, status, stream, grid);
+    else prompt_launch<D, KIND, PLAIN>(P, B, Q, w, status, stream, grid);
   }
   if (p.parts > 1) {
     const uint32_t n = B->n_rows * Q->n_q_heads;

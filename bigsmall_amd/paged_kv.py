@@ -275,6 +275,8 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
         batch.c.n_rows = t
         n = _native.lib().bs_kv_attend_work_bytes(pool.ref, batch.ref, heads)
         work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        if softcap:               # (what f32 can hold; the library takes what lies outside for these)
+            softcap = min(max(softcap, 2.0 ** -60), 2.0 ** 60)
         query = _QUERY.pack(qp, out.data_ptr(), lse.data_ptr() if return_lse else 0, sp, pp, fp, q0, q1, heads, window,
                             pool.head_dim ** -0.5 if scale is None else scale, softcap)
         _call("bs_kv_attend", pool, batch.ref, query, work.data_ptr() if n else 0, n, status.ptr if status else None)

@@ -96,7 +96,7 @@ typedef struct {
     uint32_t n_q_heads;
     uint32_t window;    /* 0: none */
     float scale;        /* of q . k */
-    float softcap;      /* 0: none */
+    float softcap;      /* 0: none; others are held to [2^-60, 2^60] */
 } bs_kv_query;
 
 /* Attention of each new row over its sequence's cache, the step's own tokens

@@ -55,3 +55,44 @@ def test_attend_skips_a_tail_that_does_not_exist(start, new, tail):
         assert not bool(got.any()) and bool((got_l == -math.inf).all())
     good = bs.kv_attend(rig.pool, rig.batch, q.cuda())           # the others are as ever
     assert torch.equal(out[:new], good[:new]) and torch.equal(out[2 * new:], good[2 * new:])
+
+
+def _capped(pool, pages, tail, start, q, scale, cap):
+    """ref.attend for causal rows with a cap, its bound without the cap in it: a score before the cap is off by at most
+    2^-20 of the sum A of its terms' absolute values, which the cap (slope 1 at most) does not widen, and cap * tanh by
+    2^-20 of its own value, which is A at most, again."""
+    n, hq, d = q.shape
+    hk = pool[0].shape[1]
+    group, length = hq // hk, start + n
+    see = torch.arange(length)[None] <= start + torch.arange(n)[:, None]
+    out, tol = torch.zeros(2, n, hq, d, dtype=torch.float64)
+    lse, off = torch.zeros(2, n, hq, dtype=torch.float64)
+    for head in range(hq):
+        k, v = ref.cached(pool, pages, tail, length, head // group)
+        x = cap * torch.tanh((q[:, head].double() @ k.T) * scale / cap)
+        a = (q[:, head].double().abs() @ k.abs().T) * abs(scale)
+        lse[:, head] = torch.logsumexp(x.masked_fill(~see, -math.inf), 1)
+        w = torch.exp(x - lse[:, head, None]).masked_fill(~see, 0.0)
+        off[:, head] = 2.0 ** -20 * (2 * a.masked_fill(~see, 0.0).amax(1) + 16)
+        out[:, head] = w @ v
+        tol[:, head] = 2.0 ** -8 * out[:, head].abs() + (2.0 ** -11 + 2 * off[:, head, None]) * (w @ v.abs()) + \
+            2.0 ** -36 * w.amax(1, keepdim=True) * (see.double() @ v.abs())
+    return out, lse, tol, off
+
+
+@pytest.mark.parametrize("cap", [0.25, 50.0, 100.0, 1000.0, 1e4, 1e5, 1e9, 1e30, 1e60, 1e-50])
+@pytest.mark.parametrize("starts,news,d,scale", [([700, 64, 13], [1, 1, 1], 64, 0.125), ([300, 0, 5], [90, 65, 1], 64, 0.125),
+                                                 ([300, 20], [70, 1], 256, 0.3), ([500, 3], [2, 1], 128, -1.0)])
+def test_caps_of_every_size(cap, starts, news, d, scale):
+    """Scores far below the cap come out as they went in, not off by the cap's own rounding; scores above it are held."""
+    import bigsmall_amd as bs
+    _say("cap", cap, starts, news, d, scale)
+    rig = Rig(starts, news, 1, d, torch.int8, seed=d)
+    q = rig.rows(2)
+    out, lse = bs.kv_attend(rig.pool, rig.batch, q.cuda(), scale=scale, softcap=cap, return_lse=True)
+    pool, out, lse = _cpu(rig.pool), out.cpu().double(), lse.cpu().double()
+    for b, n in enumerate(news):
+        at = slice(int(rig.cu[b]), int(rig.cu[b]) + n)
+        o, l, tol, ltol = _capped(pool, rig.pages[b], rig.tails[b], starts[b], q[at], scale, cap)
+        assert bool(((lse[at] - l).abs() <= ltol).all()), (b, float(((lse[at] - l).abs() / ltol).max()))
+        assert bool(((out[at] - o).abs() <= tol).all()), (b, float(((out[at] - o).abs() / tol.clamp(min=1e-30)).max()))
