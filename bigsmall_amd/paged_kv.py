@@ -92,11 +92,14 @@ class KVBatch:
     max_new, max_len: the largest number of new tokens and of tokens after the step of a
     sequence. They choose launch shapes; a wrong value costs time, not results. Rows of q, k
     and v that no sequence covers are not read, and their outputs are not defined.
+    total: the rows of all sequences, where the host knows them: calls with another number of
+    rows are then refused. None: rows that reach past the given ones drop their sequence, which
+    only a status word tells.
     """
 
-    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "c", "ref")
+    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "c", "ref")
 
-    def __init__(self, start, cu, table, tails, max_new: int, max_len: int):
+    def __init__(self, start, cu, table, tails, max_new: int, max_len: int, total: Optional[int] = None):
         _tensor("start", start, torch.int32)
         if start.dim() != 1:
             raise ValueError("KVBatch: start must be [sequences]")
@@ -112,7 +115,7 @@ class KVBatch:
         if b > 65535 or not 0 <= max_new < 1 << 30 or not 0 <= max_len < 1 << 30:
             raise ValueError("KVBatch: at most 65535 sequences, max_new and max_len below 2^30")
         self.start, self.cu, self.table, self.tails = start, cu, table, tails
-        self.n_seqs, self.max_new, self.max_len = b, int(max_new), int(max_len)
+        self.n_seqs, self.max_new, self.max_len, self.total = b, int(max_new), int(max_len), total
         self.c = _native.BsKvBatch(start.data_ptr(), cu.data_ptr(), table.data_ptr(), tails.data_ptr(), b, stride,
                                    table.shape[1], 0, int(max_new), int(max_len))
         self.ref, self.index = ctypes.byref(self.c), start.get_device()
@@ -175,6 +178,11 @@ def _gpu(pool: KVPool) -> None:
         raise RuntimeError("the paged KV cache's operators run on an AMD GPU (MI355X); the pool is on " + str(pool.device))
 
 
+def _check_total(batch: KVBatch, n: int) -> None:
+    if batch.total is not None and n != batch.total:
+        raise ValueError(f"{n} rows, the step has {batch.total}")
+
+
 def _check_batch(pool: KVPool, batch: KVBatch) -> None:
     _gpu(pool)
     if batch.index != pool.index:
@@ -214,6 +222,7 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
     do not exist; such parts are not written."""
     _check_batch(pool, batch)
     k, t, _, kp, k0, k1 = _rows("k", k, None, pool.n_kv_heads, pool)
+    _check_total(batch, t)
     v, _, _, vp, v0, v1 = _rows("v", v, t, pool.n_kv_heads, pool)
     rot = cos = sin = inter = n_pos = heads = qp = op = q0 = q1 = 0
     if rope is not None:
@@ -259,6 +268,7 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     nothing gives 0 and -inf."""
     _check_batch(pool, batch)
     q, t, heads, qp, q0, q1 = _rows("q", q, None, None, pool)
+    _check_total(batch, t)
     _check_heads(heads, pool)
     if not 0 <= window < 1 << 31 or not 0.0 <= softcap < float("inf"):
         raise ValueError("window and softcap must not be negative or infinite")
@@ -365,20 +375,20 @@ class PagedKVCache:
         flat = torch.tensor(arrays, dtype=torch.int32, device="cpu").pin_memory().to(self.device, non_blocking=True)
         b, m = shape
         start, cu, tails, table = flat.split([b, b + 1, 2 * b, b * m])
-        return KVBatch(start, cu, table.view(b, m), tails.view(b, 2), max_new, max_len)
+        return KVBatch(start, cu, table.view(b, m), tails.view(b, 2), max_new, max_len, arrays[2 * b])
 
     # ---- one layer
-    def append(self, layer: int, step: KVBatch, q, k, v, rope: Optional[Rope] = None):
-        return kv_append(self.pools[layer], step, q, k, v, rope)
+    def append(self, layer: int, step: KVBatch, q, k, v, rope: Optional[Rope] = None, **options):
+        return kv_append(self.pools[layer], step, q, k, v, rope, **options)
 
     def attend(self, layer: int, step: KVBatch, q, **options):
         return kv_attend(self.pools[layer], step, q, **options)
 
-    def read(self, layer: int, seq: int):
+    def read(self, layer: int, seq: int, status=None):
         """K and V of a sequence's appended tokens, bf16 [kv heads, tokens, dim]."""
         n, pages, tail = self._books.where(seq)
         row = torch.tensor(pages + [tail], dtype=torch.int32, device="cpu").to(self.device)
-        return kv_read(self.pools[layer], row[:-1], n, row[-1:])
+        return kv_read(self.pools[layer], row[:-1], n, row[-1:], status)
 
 
 class _Books:

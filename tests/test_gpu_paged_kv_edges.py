@@ -96,3 +96,24 @@ def test_caps_of_every_size(cap, starts, news, d, scale):
         o, l, tol, ltol = _capped(pool, rig.pages[b], rig.tails[b], starts[b], q[at], scale, cap)
         assert bool(((lse[at] - l).abs() <= ltol).all()), (b, float(((lse[at] - l).abs() / ltol).max()))
         assert bool(((out[at] - o).abs() <= tol).all()), (b, float(((out[at] - o).abs() / tol.clamp(min=1e-30)).max()))
+
+
+def test_cache_refuses_rows_that_are_not_the_steps():
+    """Fewer or more rows than a step has: refused before anything is written; numbers that do not exist reach a status."""
+    import bigsmall_amd as bs
+    from bigsmall_amd.device import StatusWord
+    cache = bs.PagedKVCache(1, 1, 64, pages=4, sequences=2)
+    a, b = cache.add(), cache.add()
+    step = cache.step({a: 3, b: 2})
+    x = torch.ones(7, 1, 64, dtype=torch.bfloat16, device="cuda")
+    for n in (0, 3, 4, 6, 7):
+        with pytest.raises(ValueError, match="5"):
+            cache.append(0, step, None, x[:n], x[:n])
+        with pytest.raises(ValueError, match="5"):
+            cache.attend(0, step, x[:n])
+    assert not bool(cache.pools[0].k_tail.any())
+    st = StatusWord("cuda")
+    out = torch.empty(5, 1, 64, dtype=torch.bfloat16, device="cuda")
+    assert cache.append(0, step, x[:5], x[:5], x[:5], out=out, status=st) is out and torch.equal(out, x[:5])
+    k, v = cache.read(0, a, status=st)
+    assert torch.equal(k[0], x[:3, 0]) and torch.equal(v[0], x[:3, 0]) and int(st.t) == 0
