@@ -97,7 +97,7 @@ class KVBatch:
     only a status word tells.
     """
 
-    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "c", "ref")
+    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "before", "c", "ref")
 
     def __init__(self, start, cu, table, tails, max_new: int, max_len: int, total: Optional[int] = None):
         _tensor("start", start, torch.int32)
@@ -116,6 +116,7 @@ class KVBatch:
             raise ValueError("KVBatch: at most 65535 sequences, max_new and max_len below 2^30")
         self.start, self.cu, self.table, self.tails = start, cu, table, tails
         self.n_seqs, self.max_new, self.max_len, self.total = b, int(max_new), int(max_len), total
+        self.before = None           # of a PagedKVCache's step: how to take it back
         self.c = _native.BsKvBatch(start.data_ptr(), cu.data_ptr(), table.data_ptr(), tails.data_ptr(), b, stride,
                                    table.shape[1], 0, int(max_new), int(max_len))
         self.ref, self.index = ctypes.byref(self.c), start.get_device()
@@ -370,8 +371,27 @@ class PagedKVCache:
     def step(self, new: dict) -> KVBatch:
         """A step that appends new[seq] tokens to each sequence, rows packed in the dict's order. Takes the
         pages it needs (RuntimeError, and nothing taken, if there are too few). Appending must follow for
-        every layer before the sequences' next step."""
+        every layer before the sequences' next step; where it does not, `undo` takes the step back."""
+        before = self._books.note(new)
         arrays, shape, max_new, max_len = self._books.step(new)
+        try:
+            step = self._upload(arrays, shape, max_new, max_len)
+        except BaseException:
+            self._books.undo(before)
+            raise
+        step.before = before
+        return step
+
+    def undo(self, step: KVBatch) -> None:
+        """Take back a step whose appends were refused or came to an end half-way: its sequences have their
+        lengths, pages and tails of before it, and what they held then is untouched. Once, and before their
+        next step (RuntimeError otherwise)."""
+        if step.before is None:
+            raise RuntimeError("not a step of this cache, or taken back already")
+        self._books.undo(step.before)
+        step.before = None
+
+    def _upload(self, arrays, shape, max_new, max_len) -> KVBatch:
         flat = torch.tensor(arrays, dtype=torch.int32, device="cpu").pin_memory().to(self.device, non_blocking=True)
         b, m = shape
         start, cu, tails, table = flat.split([b, b + 1, 2 * b, b * m])
@@ -425,6 +445,23 @@ class _Books:
     def where(self, seq):
         n, pages, tail, _ = self._get(seq)
         return n, list(pages), tail
+
+    def note(self, new: dict) -> list:
+        """What `undo` needs to take back the step that comes next: sequence, entry, length before and after it."""
+        return [(seq, self._get(seq), self._get(seq)[0], self._get(seq)[0] + int(n)) for seq, n in new.items()]
+
+    def undo(self, before: list) -> None:
+        for seq, e, _, after in before:
+            if self.seqs.get(seq) is not e or e[0] != after:
+                raise RuntimeError(f"sequence {seq} has gone on or been dropped since the step")
+        for _, e, length, after in reversed(before):
+            # a completed page's step went on in the other tail, and an unfinished one's wrote past `length` only
+            pages = e[1]
+            while len(pages) > length // PAGE:
+                self.free.append(pages.pop())
+            if after // PAGE > length // PAGE:
+                e[2], e[3] = e[3], e[2]
+            e[0] = length
 
     def step(self, new: dict):
         """(start, cu, tails, table) as one flat list, (sequences, table width), max_new, max_len."""

@@ -45,10 +45,18 @@ class PagedLlama:
     @torch.no_grad()
     def forward(self, new: dict) -> torch.Tensor:
         """new: {sequence: its new token ids (1-D)}; sequences come from `self.cache.add()`. Returns the
-        logits [sequences, vocab] after each sequence's last new token, in the dict's order."""
+        logits [sequences, vocab] after each sequence's last new token, in the dict's order. If it raises, the
+        sequences are as they were before."""
         ids = [torch.as_tensor(t).to(self.device) for t in new.values()]
         step = self.cache.step({seq: len(t) for seq, t in zip(new, ids)})
-        x = self.embed[torch.cat(ids)]
+        try:
+            return self._forward(step, torch.cat(ids))
+        except BaseException:         # the cache would claim tokens that some layer never got
+            self.cache.undo(step)
+            raise
+
+    def _forward(self, step, ids):
+        x = self.embed[ids]
         t = x.shape[0]
         for i, layer in self.loader.iter_layers(progress=False):
             p = f"model.layers.{i}."

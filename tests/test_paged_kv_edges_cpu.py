@@ -4,7 +4,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from bigsmall_amd.paged_kv import KVPool, kv_append, kv_attend
+from bigsmall_amd.paged_kv import KVPool, _Books, kv_append, kv_attend
 from test_paged_kv_cpu import _batch, _parts, on_gpu  # noqa: F401 (a fixture)
 
 
@@ -18,3 +18,67 @@ def test_calls_refuse_rows_that_are_not_the_steps(on_gpu):
             kv_append(pool, batch, None, x, x)
         with pytest.raises(ValueError, match="the step has 2"):
             kv_attend(pool, batch, x)
+
+
+def _state(books):
+    return books.free[:], books.free_tails[:], {s: [e[0], e[1][:], e[2], e[3]] for s, e in books.seqs.items()}
+
+
+def test_books_take_a_step_back():
+    books = _Books(10, 4)
+    a, b, c = books.add(), books.add(), books.add()
+    books.step({a: 70, b: 64, c: 1})
+    for new in ({a: 1}, {b: 63, a: 58}, {c: 63, b: 130, a: 200}, {a: 57, c: 64}):
+        was, before = _state(books), books.note(new)
+        books.step(new)
+        assert _state(books) != was
+        books.undo(before)
+        assert _state(books) == was
+        with pytest.raises(RuntimeError, match="gone on"):
+            books.undo(before)
+        assert _state(books) == was
+    # not after a later step, nor after a drop: nothing is touched
+    first, _ = books.note({a: 3, b: 3}), books.step({a: 3, b: 3})
+    second, _ = books.note({b: 1}), books.step({b: 1})
+    was = _state(books)
+    with pytest.raises(RuntimeError, match=f"sequence {b}"):
+        books.undo(first)
+    assert _state(books) == was
+    books.undo(second)
+    books.undo(first)
+    before, _ = books.note({a: 3}), books.step({a: 3})
+    books.drop(a)
+    was = _state(books)
+    with pytest.raises(RuntimeError, match="dropped"):
+        books.undo(before)
+    assert _state(books) == was
+    with pytest.raises(KeyError):
+        books.note({a: 1})
+
+
+def test_forward_that_raises_takes_its_step_back():
+    """With the cache's books and a layer that fails, on the host."""
+    from bigsmall_amd.paged_llama import PagedLlama
+    books = _Books(10, 2)
+
+    class Cache:
+        def step(self, new):
+            self.before = books.note(new)
+            books.step(new)
+            return self
+
+        def undo(self, step):
+            books.undo(step.before)
+
+    class Loader:
+        def iter_layers(self, progress):
+            raise MemoryError("layer 0")
+    m = PagedLlama.__new__(PagedLlama)
+    m.loader, m.cache, m.device, m.embed = Loader(), Cache(), torch.device("cpu"), torch.zeros(10, 4)
+    a, b = books.add(), books.add()
+    books.step({a: 60})
+    was = _state(books)
+    for new in ({a: [1] * 540, b: [2]}, {b: torch.tensor([3.5])}, {b: torch.zeros(1, 4, dtype=torch.int64)}):
+        with pytest.raises((MemoryError, IndexError, RuntimeError)):
+            m.forward(new)
+        assert _state(books) == was
