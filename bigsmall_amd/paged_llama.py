@@ -73,8 +73,10 @@ class PagedLlama:
 
     def generate(self, prompts: list, max_new_tokens: int) -> list:
         """Greedy continuations of prompts (1-D token ids), all in one batch."""
-        seqs = [self.cache.add() for _ in prompts]
+        seqs = []
         try:
+            for _ in prompts:
+                seqs.append(self.cache.add())
             logits, out = self.forward(dict(zip(seqs, prompts))), []
             for n in range(max_new_tokens):
                 out.append(logits.argmax(-1))

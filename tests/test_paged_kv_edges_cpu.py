@@ -82,3 +82,17 @@ def test_forward_that_raises_takes_its_step_back():
         with pytest.raises((MemoryError, IndexError, RuntimeError)):
             m.forward(new)
         assert _state(books) == was
+
+
+def test_generate_with_more_prompts_than_places_keeps_none():
+    from types import SimpleNamespace
+
+    from bigsmall_amd.paged_llama import PagedLlama
+    books = _Books(4, 2)
+    m = PagedLlama.__new__(PagedLlama)
+    m.cache = SimpleNamespace(add=books.add, drop=books.drop)
+    kept = books.add()
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="sequences"):
+            m.generate([torch.zeros(1, dtype=torch.int64)] * 2, 1)
+    assert list(books.seqs) == [kept] and len(books.free_tails) == 1
