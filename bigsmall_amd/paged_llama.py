@@ -96,10 +96,14 @@ class PagedLlama:
     def resume(self, seq: int, store) -> int:
         """Bring a parked sequence back: its K and V are already rotated. Returns its new number."""
         new, step = self.cache.add(), None
-        for i in range(len(self.cache.pools)):
-            k, v = (x.transpose(0, 1).to(self.device) for x in store.get((seq, i)))
-            step = step or self.cache.step({new: k.shape[0]})
-            self.cache.append(i, step, None, k, v)
+        try:
+            for i in range(len(self.cache.pools)):
+                k, v = (x.transpose(0, 1).to(self.device) for x in store.get((seq, i)))
+                step = step or self.cache.step({new: k.shape[0]})
+                self.cache.append(i, step, None, k, v)
+        except BaseException:
+            self.cache.drop(new)
+            raise
         return new
 
 

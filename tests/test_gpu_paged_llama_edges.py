@@ -66,3 +66,32 @@ def test_steps_are_taken_back_once():
     cache.step({a: 1})
     with pytest.raises(RuntimeError, match="gone on"):
         cache.undo(step)
+
+
+def test_resume_without_room_or_entry_takes_nothing():
+    import bigsmall_amd
+    from bigsmall_amd.paged_llama import PagedLlama
+    m = PagedLlama.__new__(PagedLlama)
+    m.device = torch.device("cuda")
+    m.cache = bigsmall_amd.PagedKVCache(2, 1, 64, pages=4, sequences=2)
+    x = torch.randn(200, 1, 64, device="cuda").bfloat16()
+    seq, store = m.cache.add(), bigsmall_amd.CompressedKVCache(device="cuda")
+    step = m.cache.step({seq: 200})
+    for i in range(2):
+        m.cache.append(i, step, None, x, x)
+    kept = m.cache.read(1, seq)
+    m.park(seq, store)
+    assert m.cache.free_pages() == 4
+    other = m.cache.add()
+    m.cache.step({other: 130})                        # two of four pages: three are needed
+    was = _books(m)
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="pages"):
+            m.resume(seq, store)
+        with pytest.raises(KeyError):
+            m.resume(seq + 100, store)                # never parked
+        assert _books(m) == was
+    m.cache.drop(other)
+    back = m.resume(seq, store)
+    for got, want in zip(m.cache.read(1, back), kept):
+        assert got.shape == want.shape
