@@ -88,7 +88,10 @@ class PagedLlama:
                 self.cache.drop(s)
 
     def park(self, seq: int, store) -> None:
-        """Move a sequence's K and V, as bf16, into a CompressedKVCache under (seq, layer) and drop it here."""
+        """Move a sequence's K and V, as bf16, into a CompressedKVCache under (seq, layer) and drop it here.
+        A sequence without tokens has nothing to keep: ValueError."""
+        if not self.cache.length(seq):
+            raise ValueError(f"sequence {seq} has no tokens to park")
         for i in range(len(self.cache.pools)):
             store.set((seq, i), *self.cache.read(i, seq))
         self.cache.drop(seq)

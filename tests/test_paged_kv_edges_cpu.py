@@ -96,3 +96,20 @@ def test_generate_with_more_prompts_than_places_keeps_none():
         with pytest.raises(RuntimeError, match="sequences"):
             m.generate([torch.zeros(1, dtype=torch.int64)] * 2, 1)
     assert list(books.seqs) == [kept] and len(books.free_tails) == 1
+
+
+def test_park_refuses_a_sequence_without_tokens():
+    """(The store has no entries of no elements: it could not be brought back.)"""
+    from types import SimpleNamespace
+
+    from bigsmall_amd.paged_llama import PagedLlama
+    books, sets = _Books(4, 2), []
+    m = PagedLlama.__new__(PagedLlama)
+    m.cache = SimpleNamespace(length=books.length, drop=books.drop, pools=[None], read=lambda i, seq: (None, None))
+    seq = books.add()
+    with pytest.raises(ValueError, match="no tokens"):
+        m.park(seq, SimpleNamespace(set=lambda *a: sets.append(a)))
+    assert not sets and seq in books.seqs
+    books.step({seq: 1})
+    m.park(seq, SimpleNamespace(set=lambda *a: sets.append(a)))
+    assert len(sets) == 1 and seq not in books.seqs
