@@ -97,7 +97,7 @@ class KVBatch:
     only a status word tells.
     """
 
-    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "before", "c", "ref")
+    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "before", "c", "_head", "_rest")
 
     def __init__(self, start, cu, table, tails, max_new: int, max_len: int, total: Optional[int] = None):
         _tensor("start", start, torch.int32)
@@ -119,7 +119,13 @@ class KVBatch:
         self.before = None           # of a PagedKVCache's step: how to take it back
         self.c = _native.BsKvBatch(start.data_ptr(), cu.data_ptr(), table.data_ptr(), tails.data_ptr(), b, stride,
                                    table.shape[1], 0, int(max_new), int(max_len))
-        self.ref, self.index = ctypes.byref(self.c), start.get_device()
+        self.index = start.get_device()
+        at = _native.BsKvBatch.n_rows.offset
+        self._head, self._rest = bytes(self.c)[:at], bytes(self.c)[at + 4:]
+
+    def with_rows(self, n: int) -> bytes:
+        """The C structure of a call with n rows: a value of its own, since layers and threads share the batch."""
+        return self._head + n.to_bytes(4, "little") + self._rest
 
 
 class Rope:
@@ -250,8 +256,7 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
         else:
             qp = 0
     if t:
-        batch.c.n_rows = t
-        _call("bs_kv_append", pool, batch.ref, _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
+        _call("bs_kv_append", pool, batch.with_rows(t), _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
               status.ptr if status else None)
     return result
 
@@ -283,14 +288,14 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((t, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if t:
-        batch.c.n_rows = t
-        n = _native.lib().bs_kv_attend_work_bytes(pool.ref, batch.ref, heads)
+        step = batch.with_rows(t)
+        n = _native.lib().bs_kv_attend_work_bytes(pool.ref, step, heads)
         work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         if softcap:               # (what f32 can hold; the library takes what lies outside for these)
             softcap = min(max(softcap, 2.0 ** -60), 2.0 ** 60)
         query = _QUERY.pack(qp, out.data_ptr(), lse.data_ptr() if return_lse else 0, sp, pp, fp, q0, q1, heads, window,
                             pool.head_dim ** -0.5 if scale is None else scale, softcap)
-        _call("bs_kv_attend", pool, batch.ref, query, work.data_ptr() if n else 0, n, status.ptr if status else None)
+        _call("bs_kv_attend", pool, step, query, work.data_ptr() if n else 0, n, status.ptr if status else None)
     return (out, lse) if return_lse else out
 
 

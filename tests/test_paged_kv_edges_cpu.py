@@ -113,3 +113,32 @@ def test_park_refuses_a_sequence_without_tokens():
     books.step({seq: 1})
     m.park(seq, SimpleNamespace(set=lambda *a: sets.append(a)))
     assert len(sets) == 1 and seq not in books.seqs
+
+
+def test_rows_of_a_call_are_its_own(on_gpu, monkeypatch):
+    """Two calls of different sizes on one batch, the second made while the first is on its way: each C structure names
+    its own rows."""
+    from bigsmall_amd import _native, paged_kv
+    pool, batch = KVPool(*_parts()), _batch()
+    seen = []
+
+
+    class Lib:
+        def bs_kv_attend_work_bytes(self, pool_ref, step, heads):
+            return 0
+
+    def call(name, p, step, *rest):
+        if len(seen) < 2:                              # another thread's turn
+            seen.append(None)
+            kv_attend(pool, batch, torch.zeros(5, 2, 64, dtype=torch.bfloat16))
+        c = _native.BsKvBatch.from_buffer_copy(step if isinstance(step, bytes) else step._obj)
+        seen.append((name, c.n_rows, c.n_seqs, c.max_len, c.start))
+    monkeypatch.setattr(paged_kv._native, "lib", lambda: Lib())
+    monkeypatch.setattr(paged_kv, "_call", call)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    kv_attend(pool, batch, x)
+    del seen[:]
+    kv_append(pool, batch, None, x, x)
+    calls = [s for s in seen if s]
+    assert calls == [("bs_kv_attend", 5, 2, 6, batch.start.data_ptr()), ("bs_kv_attend", 5, 2, 6, batch.start.data_ptr()),
+                     ("bs_kv_append", 3, 2, 6, batch.start.data_ptr())]
