@@ -51,10 +51,12 @@ struct alignas(2 * N) Half {
 
 // The page numbered `unit` among all pages that the step touches, sequence by
 // sequence: its sequence and its place in it. Every wave counts for itself, 64
-// sequences at a time.
+// sequences at a time; those of the first page, where a status is asked for, go on to
+// the last sequence to report lengths and offsets that make no sense.
 __device__ bool find_unit(const bs_kv_batch& B, uint32_t unit, uint32_t& b, uint32_t& page, SeqStep& step, int32_t* status) {
   const uint32_t lane = threadIdx.x & 63;
   uint32_t base = 0;
+  bool found = false;
   for (uint32_t b0 = 0; b0 < B.n_seqs; b0 += 64) {
     uint32_t pages = 0, at = 0;
     SeqStep s = {0, 0, 0, 0};
@@ -70,17 +72,18 @@ __device__ bool find_unit(const bs_kv_batch& B, uint32_t unit, uint32_t& b, uint
       if (lane >= (uint32_t)d) incl += up;
     }
     const uint64_t past = __ballot(base + incl > unit);
-    if (past) {
+    if (past && !found) {
       const int l = __builtin_ctzll(past);
       b = b0 + (uint32_t)l;
       page = (uint32_t)__builtin_amdgcn_readlane((int)(at + unit - (base + incl - pages)), l);
       step.t0 = __builtin_amdgcn_readlane(s.t0, l), step.n = __builtin_amdgcn_readlane(s.n, l);
       step.start = __builtin_amdgcn_readlane(s.start, l), step.len = __builtin_amdgcn_readlane(s.len, l);
-      return true;
+      if (unit != 0 || !status) return true;
+      found = true;
     }
     base += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
   }
-  return false;
+  return found;
 }
 
 // One token's 2 * VEC channels: VEC pairs that turn together, or as many channels that do not turn.

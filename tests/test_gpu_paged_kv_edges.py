@@ -117,3 +117,30 @@ def test_cache_refuses_rows_that_are_not_the_steps():
     assert cache.append(0, step, x[:5], x[:5], x[:5], out=out, status=st) is out and torch.equal(out, x[:5])
     k, v = cache.read(0, a, status=st)
     assert torch.equal(k[0], x[:3, 0]) and torch.equal(v[0], x[:3, 0]) and int(st.t) == 0
+
+
+@pytest.mark.parametrize("bad", [[66], [3], [64, 127, 129], list(range(64, 130))])
+def test_append_reports_any_sequence_of_a_long_step(bad):
+    """Starts that make no sense, wherever they stand in a step of 130 sequences: reported, and the others appended."""
+    import bigsmall_amd as bs
+    from bigsmall_amd import _native
+    from bigsmall_amd.device import StatusWord
+    n, d = 130, 64
+    rig = Rig([5] * n, [1] * n, 1, d, torch.int8, seed=6)
+    k, v = rig.rows(1), rig.rows(1)
+    start = rig.batch.start.clone()
+    start[bad] = 1 << 28
+    st = StatusWord("cuda")
+    before = _cpu(rig.pool)
+    bs.kv_append(rig.pool, rig.batch, None, k.cuda(), v.cuda(), status=st)
+    assert int(st.t) == 0
+    rig.pool.k_tail.copy_(before[4])
+    batch = bs.KVBatch(start, rig.batch.cu, rig.batch.table, rig.batch.tails, 1, 6)
+    bs.kv_append(rig.pool, batch, None, k.cuda(), v.cuda(), status=st)
+    assert int(st.t) == _native.BS_DEV_ERR_BOUNDS
+    after = rig.pool.k_tail.cpu()
+    for b in range(n):
+        want = before[4][rig.tails[b]].clone()
+        if b not in bad:
+            want[:, 5] = k[b]
+        assert torch.equal(after[rig.tails[b]].view(torch.uint8), want.view(torch.uint8)), b
