@@ -165,13 +165,14 @@ def _rows(name: str, t, n: Optional[int], heads: Optional[int], pool: KVPool):
     if t.get_device() != pool.index:
         raise ValueError(f"{name} is on {t.device}, the cache is on {pool.device}")
     s0, s1, s2 = t.stride()
+    if shape[0] == 1:          # the stride of a dimension of one is any number: torch calls such a tensor contiguous
+        s0 = 0
+    if shape[1] == 1:
+        s1 = 0
     p = t.data_ptr()
     if s2 != 1 or (s0 | s1) & 7 or p & 15:
-        t = t.contiguous()
-        if t.data_ptr() & 15:
-            t = t.clone()
-        s0, s1, _ = t.stride()
-        p = t.data_ptr()
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, p = shape[1] * shape[2], shape[2], t.data_ptr()
     return t, shape[0], shape[1], p, s0, s1
 
 

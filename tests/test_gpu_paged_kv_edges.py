@@ -144,3 +144,34 @@ def test_append_reports_any_sequence_of_a_long_step(bad):
         if b not in bad:
             want[:, 5] = k[b]
         assert torch.equal(after[rig.tails[b]].view(torch.uint8), want.view(torch.uint8)), b
+
+
+@pytest.mark.parametrize("unaligned", [False, True])
+def test_strides_of_dimensions_of_one(unaligned):
+    """One token, or one head, out of a wider buffer: the stride of a dimension of one says nothing and is not looked at."""
+    import bigsmall_amd as bs
+    hk, group, d = 2, 4, 128
+    rig = Rig([70], [1], hk, d, torch.int8, seed=1)
+    rope = bs.Rope.from_theta(d, 100)
+    rows = rig.rows(hk * group + 2 * hk).cuda()
+    wide = torch.zeros(2, rows.shape[1] * d + 3, dtype=torch.bfloat16, device="cuda")
+    at = int(unaligned)
+    one = wide[:, :-3].unflatten(1, (-1, d))[at:at + 1]
+    one.copy_(rows)
+    q, k, v = one.split([hk * group, hk, hk], 1)
+    assert q.stride(0) % 8 and q.is_contiguous() and bool(q.data_ptr() % 16) == unaligned
+    want = bs.kv_append(rig.pool, rig.batch, q.clone(), k.clone(), v.clone(), rope)
+    want_tails = rig.pool.k_tail.clone()
+    rig.pool.k_tail[rig.tails[0], :, 70 % PAGE] = 0
+    got = bs.kv_append(rig.pool, rig.batch, q, k, v, rope)
+    assert torch.equal(got, want) and torch.equal(rig.pool.k_tail.view(torch.uint8), want_tails.view(torch.uint8))
+    if not unaligned:
+        wide_out = torch.empty_like(wide)
+        out = wide_out[:, :-3].unflatten(1, (-1, d))[:1, :hk * group]
+        assert bs.kv_append(rig.pool, rig.batch, q, k, v, rope, out=out) is out and torch.equal(out, want)
+    assert torch.equal(bs.kv_attend(rig.pool, rig.batch, q), bs.kv_attend(rig.pool, rig.batch, q.clone()))
+    # one head whose stride is odd
+    rig = Rig([70], [3], 1, d, torch.int8, seed=2)
+    x = rig.rows(1).cuda()
+    odd = x.as_strided(x.shape, (d, 5, 1))
+    assert torch.equal(bs.kv_attend(rig.pool, rig.batch, odd), bs.kv_attend(rig.pool, rig.batch, x))

@@ -142,3 +142,21 @@ def test_rows_of_a_call_are_its_own(on_gpu, monkeypatch):
     calls = [s for s in seen if s]
     assert calls == [("bs_kv_attend", 5, 2, 6, batch.start.data_ptr()), ("bs_kv_attend", 5, 2, 6, batch.start.data_ptr()),
                      ("bs_kv_append", 3, 2, 6, batch.start.data_ptr())]
+
+
+def test_strides_of_dimensions_of_one_are_not_looked_at():
+    from bigsmall_amd.paged_kv import _rows
+    pool = KVPool(*_parts())
+    wide = torch.zeros(4, 2 * 64 + 3, dtype=torch.bfloat16)
+    many = wide[:, :-3].unflatten(1, (2, 64))
+    for i in range(4):
+        one = many[i:i + 1]
+        assert one.is_contiguous() and one.stride(0) % 8
+        t, n, heads, p, s0, s1 = _rows("q", one, None, None, pool)
+        assert (n, heads) == (1, 2) and p % 16 == 0 and s0 % 8 == 0 and s1 == 64 and t.data_ptr() == p
+        assert (t is one) == (one.data_ptr() % 16 == 0)
+    t, _, _, p, s0, s1 = _rows("q", many, None, None, pool)
+    assert t is not many and (s0, s1) == (128, 64) and p % 16 == 0
+    odd = torch.zeros(3, 1, 64, dtype=torch.bfloat16).as_strided((3, 1, 64), (64, 5, 1))
+    t, _, _, _, s0, s1 = _rows("q", odd, None, None, pool)
+    assert (s0, s1 % 8) == (64, 0)
