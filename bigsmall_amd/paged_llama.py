@@ -9,7 +9,8 @@ bits, from which attention reads them.
 
 The rest of a layer is the architecture's own arithmetic in torch: RMS norm,
 projections without bias, SwiGLU. Tensor names follow the HuggingFace layout:
-`model.embed_tokens`, `model.layers.<i>.*`, `model.norm`, `lm_head`.
+`model.embed_tokens`, `model.layers.<i>.*`, `model.norm`, `lm_head`. Models that
+need anything else are refused (`check_model`).
 """
 from __future__ import annotations
 
@@ -19,12 +20,52 @@ from torch.nn.functional import linear, silu
 from .paged_kv import PagedKVCache, Rope
 
 
+_TOP = {"model.embed_tokens.weight", "model.norm.weight", "lm_head.weight"}
+_LAYER = {"input_layernorm.weight", "post_attention_layernorm.weight"} | \
+    {f"self_attn.{n}_proj.weight" for n in "qkvo"} | {f"mlp.{n}_proj.weight" for n in ("gate", "up", "down")}
+_UNUSED = "rotary_emb.inv_freq"       # a buffer that old checkpoints hold
+
+
+def check_model(config, loader, rope=None) -> None:
+    """ValueError if PagedLlama does not compute this model: another architecture, activation or rotation than it has,
+    a sliding window, or tensors (biases, further norms) that it would pass over."""
+    kind = getattr(config, "model_type", "llama")
+    if kind not in ("llama", "mistral"):
+        raise ValueError(f"PagedLlama does not compute models of type {kind!r}")
+    window = getattr(config, "sliding_window", None)
+    if window is not None and window < config.max_position_embeddings:
+        raise ValueError(f"PagedLlama attends to all tokens; the model has a sliding window of {window}")
+    if getattr(config, "hidden_act", "silu") not in ("silu", "swish"):
+        raise ValueError(f"PagedLlama's activation is silu, the model's {config.hidden_act}")
+    for bias in ("attention_bias", "mlp_bias"):
+        if getattr(config, bias, False):
+            raise ValueError(f"PagedLlama has no biases; the model has {bias}")
+    if rope is None:
+        given = getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {}
+        variant = given.get("rope_type") or given.get("type") or "default"
+        part = given.get("partial_rotary_factor") or getattr(config, "partial_rotary_factor", None) or 1.0
+        if variant != "default" or part != 1.0:
+            raise ValueError(f"the model's rotation is {variant!r} over {part} of a head; pass its angles as `rope`")
+    layers = loader.layer_count()
+    if layers != getattr(config, "num_hidden_layers", layers):
+        raise ValueError(f"the config has {config.num_hidden_layers} layers, the container {layers}")
+    groups = [("", set(loader.non_layer_tensor_names()), _TOP, _TOP - {"lm_head.weight"})]
+    groups += [(f"model.layers.{i}.", set(loader.layer_tensor_names(i)), _LAYER, _LAYER) for i in range(layers)]
+    for prefix, names, known, needed in groups:
+        missing = {prefix + n for n in needed} - names
+        other = {n for n in names if not n.endswith(_UNUSED)} - {prefix + n for n in known}
+        if missing or other:
+            raise ValueError("PagedLlama: " + "; ".join(f"{what}: {', '.join(sorted(x)[:4])}" for what, x in
+                                                        (("missing tensors", missing), ("tensors it does not use", other)) if x))
+
+
 class PagedLlama:
     """loader: a StreamingLoader on a GPU; its `prefetch` sets how many layers decode ahead.
-    config: the model's transformers.LlamaConfig (plain rotation; scaled variants: pass `rope`).
+    config: the model's transformers.LlamaConfig (plain rotation; scaled or partial ones: pass `rope`).
     pages, sequences: what the cache holds at most; kind: torch.int8 or torch.float8_e4m3fn."""
 
     def __init__(self, loader, config, pages: int, sequences: int, kind=torch.int8, rope: Rope | None = None):
+        check_model(config, loader, rope)
         self.loader, self.config = loader, config
         self.heads, self.kv_heads = config.num_attention_heads, config.num_key_value_heads
         self.dim = getattr(config, "head_dim", None) or config.hidden_size // self.heads

@@ -160,3 +160,68 @@ def test_strides_of_dimensions_of_one_are_not_looked_at():
     odd = torch.zeros(3, 1, 64, dtype=torch.bfloat16).as_strided((3, 1, 64), (64, 5, 1))
     t, _, _, _, s0, s1 = _rows("q", odd, None, None, pool)
     assert (s0, s1 % 8) == (64, 0)
+
+
+class _Names:
+    """A loader's names; nothing may be decoded."""
+
+    def __init__(self, layers=2, extra=(), without=()):
+        names = ["model.embed_tokens.weight", "model.norm.weight", "lm_head.weight"]
+        for i in range(layers):
+            names += [f"model.layers.{i}.{n}.weight" for n in
+                      ("input_layernorm", "post_attention_layernorm", "self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj",
+                       "self_attn.o_proj", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")]
+        self.names, self.layers = [n for n in names + list(extra) if n not in without], layers
+
+    def layer_count(self):
+        return self.layers
+
+    def layer_tensor_names(self, i):
+        return [n for n in self.names if n.startswith(f"model.layers.{i}.")]
+
+    def non_layer_tensor_names(self):
+        return [n for n in self.names if not n.startswith("model.layers.")]
+
+    def load_non_layer_tensors(self):
+        raise AssertionError("decoding began")
+
+
+def test_models_that_are_not_computed_are_refused():
+    from transformers import LlamaConfig, MistralConfig
+
+    from bigsmall_amd.paged_kv import Rope
+    from bigsmall_amd.paged_llama import PagedLlama, check_model
+
+    def config(kind=LlamaConfig, **change):
+        args = dict(hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                    max_position_embeddings=512)
+        return kind(**{**args, **change})
+
+    llama3 = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+              "original_max_position_embeddings": 128, "rope_theta": 10000.0}
+    old = config()
+    old.rope_parameters, old.rope_theta = None, 10000.0             # as earlier versions of the library have it
+    old.rope_scaling = {"type": "dynamic", "factor": 2.0}
+    other = config()
+    other.model_type = "granite"
+    for c, what in ((config(rope_parameters=llama3), "llama3"), (config(rope_parameters={"rope_type": "linear", "factor": 2.0, "rope_theta": 1e4}), "linear"),
+                    (old, "dynamic"), (config(rope_parameters={"rope_type": "default", "rope_theta": 1e4, "partial_rotary_factor": 0.5}), "0.5"),
+                    (config(attention_bias=True), "attention_bias"), (config(mlp_bias=True), "mlp_bias"),
+                    (config(hidden_act="gelu"), "gelu"), (other, "granite"), (config(MistralConfig, sliding_window=128), "window of 128"),
+                    (config(num_hidden_layers=3), "3 layers")):
+        with pytest.raises(ValueError, match=what):
+            PagedLlama(_Names(), c, pages=1, sequences=1)
+    for names, what in ((_Names(extra=["model.layers.1.self_attn.q_proj.bias"]), "q_proj.bias"),
+                        (_Names(extra=["model.layers.0.self_attn.q_norm.weight"]), "q_norm"), (_Names(extra=["lm_head.bias"]), "lm_head.bias"),
+                        (_Names(without=["model.layers.1.mlp.up_proj.weight"]), "missing tensors: model.layers.1.mlp.up_proj")):
+        with pytest.raises(ValueError, match=what):
+            PagedLlama(names, config(), pages=1, sequences=1)
+    # what it does compute
+    rope = Rope.from_theta(64, 10, device="cpu")
+    check_model(config(), _Names())
+    check_model(config(rope_parameters=llama3), _Names(), rope)
+    check_model(config(MistralConfig, sliding_window=None), _Names())
+    check_model(config(MistralConfig, sliding_window=512), _Names())
+    check_model(config(), _Names(extra=["model.layers.0.self_attn.rotary_emb.inv_freq"], without=["lm_head.weight"]))
+    with pytest.raises(AssertionError, match="decoding began"):
+        PagedLlama(_Names(), config(), pages=1, sequences=1)
