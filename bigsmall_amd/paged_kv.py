@@ -186,6 +186,11 @@ def _gpu(pool: KVPool) -> None:
         raise RuntimeError("the paged KV cache's operators run on an AMD GPU (MI355X); the pool is on " + str(pool.device))
 
 
+def _check_grad(a, b=None, c=None) -> None:
+    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)):
+        raise RuntimeError("the paged KV cache has no backward pass: call it under torch.no_grad(), or detach q, k and v")
+
+
 def _check_total(batch: KVBatch, n: int) -> None:
     if batch.total is not None and n != batch.total:
         raise ValueError(f"{n} rows, the step has {batch.total}")
@@ -256,6 +261,7 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
             result = out
         else:
             qp = 0
+    _check_grad(k, v, q)
     if t:
         _call("bs_kv_append", pool, batch.with_rows(t), _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
               status.ptr if status else None)
@@ -279,6 +285,7 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     _check_heads(heads, pool)
     if not 0 <= window < 1 << 31 or not 0.0 <= softcap < float("inf"):
         raise ValueError("window and softcap must not be negative or infinite")
+    _check_grad(q, slopes)
     sp = pp = fp = 0
     if slopes is not None:
         sp = _vector("slopes", slopes, heads, torch.float32, pool)

@@ -225,3 +225,27 @@ def test_models_that_are_not_computed_are_refused():
     check_model(config(), _Names(extra=["model.layers.0.self_attn.rotary_emb.inv_freq"], without=["lm_head.weight"]))
     with pytest.raises(AssertionError, match="decoding began"):
         PagedLlama(_Names(), config(), pages=1, sequences=1)
+
+
+def test_calls_that_would_lose_a_gradient_are_refused(on_gpu, monkeypatch):
+    from bigsmall_amd import paged_kv
+    pool, batch = KVPool(*_parts()), _batch()
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    g = x.clone().requires_grad_()
+    for call in (lambda: kv_append(pool, batch, g, x, x), lambda: kv_append(pool, batch, x, g, x), lambda: kv_append(pool, batch, x, x, g),
+                 lambda: kv_append(pool, batch, x, x, g * 2), lambda: kv_attend(pool, batch, g),
+                 lambda: kv_attend(pool, batch, x, slopes=torch.zeros(2, requires_grad=True))):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
+    calls = []
+
+    class Lib:
+        def bs_kv_attend_work_bytes(self, *a):
+            return 0
+    monkeypatch.setattr(paged_kv._native, "lib", lambda: Lib())
+    monkeypatch.setattr(paged_kv, "_call", lambda name, *rest: calls.append(name))
+    kv_append(pool, batch, g.detach(), x, x)
+    with torch.no_grad():
+        kv_append(pool, batch, g, g, g)
+        kv_attend(pool, batch, g)
+    assert calls == ["bs_kv_append", "bs_kv_append", "bs_kv_attend"]
