@@ -24,3 +24,13 @@ def gpu_available() -> bool:
 def golden():
     import numpy as np
     return dict(np.load(ROOT / "tests" / "golden" / "ref_vectors.npz"))
+
+
+@pytest.fixture(autouse=True)
+def _no_default_device_left():
+    """A default device that a test sets ends with it (torch.set_default_device("cpu") sets one, too)."""
+    yield
+    torch = sys.modules.get("torch")
+    if torch is not None and getattr(torch, "_GLOBAL_DEVICE_CONTEXT", None) is not None and \
+            getattr(torch._GLOBAL_DEVICE_CONTEXT, "device_context", None) is not None:
+        torch.set_default_device(None)
