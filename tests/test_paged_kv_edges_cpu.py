@@ -1,6 +1,8 @@
 """The paged KV cache's host side at the edges of what its calls take."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -249,3 +251,45 @@ def test_calls_that_would_lose_a_gradient_are_refused(on_gpu, monkeypatch):
         kv_append(pool, batch, g, g, g)
         kv_attend(pool, batch, g)
     assert calls == ["bs_kv_append", "bs_kv_append", "bs_kv_attend"]
+
+
+def test_struct_layouts_match_the_kv_header(tmp_path):
+    """Offsets and sizes of every field of include/bigsmall_kv.h's structures: of their ctypes copies, and of the two that
+    are packed by hand."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    from bigsmall_amd import _native, paged_kv
+    if shutil.which("gcc") is None:
+        pytest.skip("needs gcc")
+    structs = {"bs_kv_pool": _native.BsKvPool, "bs_kv_batch": _native.BsKvBatch, "bs_kv_rows": _native.BsKvRows,
+               "bs_kv_query": _native.BsKvQuery}
+    lines = ["#include <stddef.h>", "#include <stdio.h>", '#include "bigsmall_kv.h"', "int main(void) {"]
+    for name, c in structs.items():
+        lines.append(f'  printf("{name} sizeof %zu 0\\n", sizeof({name}));')
+        lines += [f'  printf("{name} {f[0]} %zu %zu\\n", offsetof({name}, {f[0]}), sizeof((({name}*)0)->{f[0]}));' for f in c._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]))
+    inc = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run(["gcc", "-I", str(inc), str(src), "-o", str(exe)], check=True, capture_output=True)
+    got = {}
+    for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
+        name, field, at, size = line.split()
+        got[name, field] = (int(at), int(size))
+    for name, c in structs.items():
+        assert got[name, "sizeof"][0] == ctypes.sizeof(c), name
+        for f in c._fields_:
+            assert got[name, f[0]] == (getattr(c, f[0]).offset, getattr(c, f[0]).size), (name, f[0])
+        # nothing between the fields: together they are the structure, the last one's padding aside
+        end = max(at + size for (n, f), (at, size) in got.items() if n == name and f != "sizeof")
+        assert sum(size for (n, f), (at, size) in got.items() if n == name and f != "sizeof") == end and ctypes.sizeof(c) - end < 8
+    # packed by hand: each field's number, recognisable, where the C structure has it
+    for packer, c in ((paged_kv._ROWS, _native.BsKvRows), (paged_kv._QUERY, _native.BsKvQuery)):
+        assert packer.size == ctypes.sizeof(c)
+        values = [float(i + 1) if f[1] is ctypes.c_float else i + 1 for i, f in enumerate(c._fields_)]
+        back = c.from_buffer_copy(packer.pack(*values))
+        assert [getattr(back, f[0]) for f in c._fields_] == values
+    batch = _batch()
+    a, b = _native.BsKvBatch.from_buffer_copy(batch.with_rows(12345)), batch.c
+    assert a.n_rows == 12345 and all(getattr(a, f[0]) == getattr(b, f[0]) for f in b._fields_ if f[0] != "n_rows")
