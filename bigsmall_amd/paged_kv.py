@@ -165,14 +165,13 @@ def _rows(name: str, t, n: Optional[int], heads: Optional[int], pool: KVPool):
     if t.get_device() != pool.index:
         raise ValueError(f"{name} is on {t.device}, the cache is on {pool.device}")
     s0, s1, s2 = t.stride()
-    if shape[0] == 1:          # the stride of a dimension of one is any number: torch calls such a tensor contiguous
-        s0 = 0
-    if shape[1] == 1:
-        s1 = 0
     p = t.data_ptr()
     if s2 != 1 or (s0 | s1) & 7 or p & 15:
-        t = t.clone(memory_format=torch.contiguous_format)
-        s0, s1, p = shape[1] * shape[2], shape[2], t.data_ptr()
+        # the stride of a dimension of one is any number: torch calls such a tensor contiguous
+        s0, s1 = 0 if shape[0] == 1 else s0, 0 if shape[1] == 1 else s1
+        if s2 != 1 or (s0 | s1) & 7 or p & 15:
+            t = t.clone(memory_format=torch.contiguous_format)
+            s0, s1, p = shape[1] * shape[2], shape[2], t.data_ptr()
     return t, shape[0], shape[1], p, s0, s1
 
 
@@ -186,14 +185,12 @@ def _gpu(pool: KVPool) -> None:
         raise RuntimeError("the paged KV cache's operators run on an AMD GPU (MI355X); the pool is on " + str(pool.device))
 
 
-def _check_grad(a, b=None, c=None) -> None:
-    if torch.is_grad_enabled() and (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)):
-        raise RuntimeError("the paged KV cache has no backward pass: call it under torch.no_grad(), or detach q, k and v")
+def _refuse_grad() -> None:
+    raise RuntimeError("the paged KV cache has no backward pass: call it under torch.no_grad(), or detach q, k and v")
 
 
-def _check_total(batch: KVBatch, n: int) -> None:
-    if batch.total is not None and n != batch.total:
-        raise ValueError(f"{n} rows, the step has {batch.total}")
+def _refuse_total(batch: KVBatch, n: int) -> None:
+    raise ValueError(f"{n} rows, the step has {batch.total}")
 
 
 def _check_batch(pool: KVPool, batch: KVBatch) -> None:
@@ -205,6 +202,7 @@ def _check_batch(pool: KVPool, batch: KVBatch) -> None:
 # The current stream's handle of a device, without the Stream object that torch.cuda.current_stream makes (2 us of a
 # call that takes 10).
 _stream = torch._C._cuda_getCurrentRawStream
+_recording = torch.is_grad_enabled
 
 # bs_kv_rows and bs_kv_query of include/bigsmall_kv.h, packed: a ctypes structure of as many fields takes 1 us more to fill
 _ROWS = struct.Struct("=6Q6q4I")
@@ -235,7 +233,8 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
     do not exist; such parts are not written."""
     _check_batch(pool, batch)
     k, t, _, kp, k0, k1 = _rows("k", k, None, pool.n_kv_heads, pool)
-    _check_total(batch, t)
+    if t != batch.total and batch.total is not None:
+        _refuse_total(batch, t)
     v, _, _, vp, v0, v1 = _rows("v", v, t, pool.n_kv_heads, pool)
     rot = cos = sin = inter = n_pos = heads = qp = op = q0 = q1 = 0
     if rope is not None:
@@ -261,7 +260,8 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
             result = out
         else:
             qp = 0
-    _check_grad(k, v, q)
+    if _recording() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
+        _refuse_grad()
     if t:
         _call("bs_kv_append", pool, batch.with_rows(t), _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
               status.ptr if status else None)
@@ -281,11 +281,13 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     nothing gives 0 and -inf."""
     _check_batch(pool, batch)
     q, t, heads, qp, q0, q1 = _rows("q", q, None, None, pool)
-    _check_total(batch, t)
+    if t != batch.total and batch.total is not None:
+        _refuse_total(batch, t)
     _check_heads(heads, pool)
     if not 0 <= window < 1 << 31 or not 0.0 <= softcap < float("inf"):
         raise ValueError("window and softcap must not be negative or infinite")
-    _check_grad(q, slopes)
+    if _recording() and (q.requires_grad or (slopes is not None and slopes.requires_grad)):
+        _refuse_grad()
     sp = pp = fp = 0
     if slopes is not None:
         sp = _vector("slopes", slopes, heads, torch.float32, pool)
