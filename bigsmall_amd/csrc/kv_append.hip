@@ -147,7 +147,7 @@ __global__ __launch_bounds__(THREADS) void append_kernel(bs_kv_pool P, bs_kv_bat
   __shared__ int poisoned[PAGE];
   __shared__ float tops[2][THREADS / 64];
   // Consecutive workgroups go to the eight dies in turn. The heads of one page go to one die, one after another, which
-  // then reads their tokens' angles once (32,768 tokens: 164 us, with the heads of a page on eight dies 181).
+  // then reads their tokens' angles once (32,768 tokens: with the heads of a page on eight dies a tenth more time).
   const uint32_t tid = threadIdx.x, turn_of = blockIdx.x / DIES, h = turn_of % P.n_kv_heads;
   uint32_t b, page;
   SeqStep s;
@@ -455,7 +455,7 @@ extern "C" int bs_kv_append(const bs_kv_pool* P, const bs_kv_batch* B, const bs_
     return BS_ERR_ARG;
   hipStream_t s = (hipStream_t)stream;
   // Eight pairs an item (16-byte loads) where the turned channels divide by it, else four (2,048 tokens,
-  // heads of 128: 17 us, by fours 21; 32,768 tokens: 169 and 173).
+  // heads of 128: 17 us, by fours 21; 32,768 tokens: by fours 2 % more).
   const bool wide = R->rot % 16 == 0;
 #define BS_KV_GO(D, K) return wide ? append_launch<D, 8, K>(P, B, R, d_status, s) : append_launch<D, 4, K>(P, B, R, d_status, s)
 #define BS_KV_DIMS(K)              \

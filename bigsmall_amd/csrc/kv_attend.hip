@@ -20,8 +20,12 @@
 // exponent, p' = 2^(s + log2(vs) - m) with m the running maximum of s +
 // log2(vs), so that O adds up codes * p' over pages of different scales, and
 // the denominator adds up (sum of p' in the page) / vs. Scores and log2 in base
-// 2, all in f32; p' goes to the product as f16 (11 bits), multiplied by 2^12 so
-// that weights down to 2^-26 of the largest keep them all.
+// 2, sums and maxima all in f32. p' goes to the product as f16, multiplied by 2^12
+// so that weights down to 2^-26 of the largest keep all 11 bits: an eighth of what
+// rounding the output to bf16 takes, and a second part of 11 more would double the
+// second product. q goes as f16 after a power of two: exact down to 2^-14 of the
+// row's largest channel, below that within 2^-25 of it, the size of the rounding in
+// the f32 sum.
 //
 // A row sees one interval of keys [lo, hi), whatever masks are set. A page that
 // lies inside the interval of all rows needs no comparison.
@@ -261,9 +265,9 @@ struct PageList {
 // A wave reads the next page's K as soon as this one's is multiplied, and its V after this one's: between 8 and 16 KiB a
 // wave are always under way (heads of 128), 64 to 128 KiB a compute unit. The bound is memory: 2 D bytes a key against
 // 4 D flops a row, and at 16 rows the matrix unit and the conversions still take a quarter of the time that the bytes
-// do. 128 sequences of 15,000 to 16,383 tokens, 8 kv heads of 128: 641 us, 6.4 TB/s; 64 sequences of up to 8,192: 131 us,
+// do. 128 sequences of 15,000 to 16,383 tokens, 8 kv heads of 128: 639 us, 6.4 TB/s; 64 sequences of up to 8,192: 129 us,
 // 4.2 TB/s (one workgroup a sequence and head just fills the card, and the longest goes on alone); a single row over
-// 1,024 tokens 12.5 us, which is the chain of dependent reads: the step, page numbers, pages. 168 registers a wave, for
+// 1,024 tokens 13 us, which is the chain of dependent reads: the step, page numbers, pages. 168 registers a wave, for
 // three waves a SIMD instead of two, spill and cost a third.
 template <int D, int KIND>
 __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_kv_pool P, bs_kv_batch B, bs_kv_query A, Work W,
@@ -528,10 +532,11 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 ? 2 : 1) void rows_kernel(bs_k
 // Two workgroups a compute unit (one with heads of 256, whose o alone is 128 registers a lane). A page costs a wave 32
 // products (heads of 128), about 500 ns of the matrix unit, and some 260 other vector instructions, 32 exponentials and 32
 // conversions among them; the bound is how far the two waves of a SIMD run one beside the other. 8,192-token causal prompt,
-// 32 and 8 heads of 128, e4m3: 585 us, 0.93 PFLOP/s, where a large f16 product of the library reaches 1.23; the products
-// alone take 320. 500 tokens over a window of 16,384, heads of 256, capped: 225 us, 0.6 PFLOP/s. Eight waves and 256 rows
-// a workgroup: 573 us there, but 90 us instead of 45 for short documents. One wave a SIMD with the next page's scores
-// woven into this page's weights: 800 us.
+// 32 and 8 heads of 128, e4m3: 565 to 585 us from run to run, 0.95 PFLOP/s, where a large f16 product of the library
+// reaches 1.23; the products alone take 320. 500 tokens over a window of 16,384, heads of 256, capped: 224 us, 0.6 PFLOP/s
+// (all 512 registers are in use there, and 10 to 18 more spill once a cap or a bias is set). Eight waves and 256 rows a
+// workgroup, on one card: 573 us where four waves took 578, but 90 us instead of 46 for short documents. One wave a SIMD
+// with the next page's scores woven into this page's weights: 800 us.
 constexpr int PROMPT_WAVES = 4, PROMPT_ROWS = 32 * PROMPT_WAVES, PROMPT_THREADS = 64 * PROMPT_WAVES;
 
 // The maximum of x over the two lanes that share a row (32 apart).
@@ -994,7 +999,9 @@ __global__ __launch_bounds__(256) void join_kernel(bs_kv_query A, Work W, uint32
 // Launch shapes of a call. FEW_ROWS: rows of a sequence and kv head up to which rows_kernel takes a step. (64 sequences
 // of up to 8,192 tokens, 4 rows, us: 131 there, 193 in prompt_kernel; of up to 12,000, 4 to 16 rows: 206 and 265. With
 // more than one tile of rows it would read every page again. Where sequences differ, prompt_kernel takes all of them: the
-// same caches with 4 to 32 rows 275 us, against 410 with the two kernels one after the other.)
+// same caches with 4 to 32 rows 275 us, against 410 with the two kernels one after the other. That holds for caches of
+// that size: a prompt of 2,048 tokens beside 63 single tokens on caches of 1,000 to 100,000 takes 3,380 us, where the two
+// alone take 66 and 729, because the prompt's tiles fill the card and the long caches are not split.)
 constexpr uint32_t FEW_ROWS = 16;
 
 struct Plan {
@@ -1012,9 +1019,10 @@ uint32_t split_for(uint64_t blocks, uint64_t want, uint64_t pages, uint64_t leas
 
 // Pieces of a cache of `pages` pages, `blocks` tiles of rows in all: as many as fill the card, of 4 pages (one a wave)
 // at least, and of 16 once there are 32, since every piece costs the joining kernel. Up to 16 pages a workgroup is done
-// before a second kernel has begun. (One row, heads of 128, 8 kv heads, us a call with one piece / pieces of 4 / 8 / 16
+// before a second kernel has begun. Not where sequences differ: with blocks enough for the card a step is not split, and
+// 63 sequences near 1,000 tokens with one of 131,072 take 890 us, where the two alone take 50 and 59. (One row, heads of 128, 8 kv heads, us a call with one piece / pieces of 4 / 8 / 16
 // pages: 1,000 tokens 13.5 / 16.2 / 16.3 / 13.5, 4,000 tokens 36.8 / 17.0 / 18.9 / 23.5, 16,000 tokens - / 22.1 / 20.2 / 22.5,
-// 32,000 tokens - / 26.8 / 28.6 / 24.4.)
+// 32,000 tokens - / 26.8 / 28.6 / 24.4. As the rule has it: 256 tokens 9.5, 512 10.5, 1,024 14.0, 1,500 14.1, 2,048 13.3, 3,000 14.7.)
 uint32_t pieces_for(uint64_t blocks, uint64_t pages) {
   if (pages <= 16) return 1;
   return split_for(blocks, RESIDENT, std::min<uint64_t>(pages / 4, std::max<uint64_t>(32, pages / 16)), 1);

@@ -19,7 +19,8 @@ new rows lie, how many tokens it has cached, its pages and its tails.
 PagedKVCache keeps the pools of all layers and does the bookkeeping: sequences,
 pages, tails, steps.
 
-All calls run on the current torch stream of the pool's device and do not
+Inference only: inputs that require a gradient are refused while gradients are
+recorded. All calls run on the current torch stream of the pool's device and do not
 synchronise. Work areas come from torch's allocator for each call. Tensors of
 another stream need the usual wait and record_stream by the caller.
 """
@@ -49,7 +50,8 @@ def _tensor(name: str, t, dtype, device=None, shape=None):
 
 
 class KVPool:
-    """One layer's storage: the six tensors (contiguous, on one GPU), checked once."""
+    """One layer's storage: the six tensors (contiguous, on one GPU), checked once. What kv_append writes is what
+    kv_attend takes; where something else fills them: v_scale positive (2^-49 to 2^54), the tails' V finite."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "device", "index", "dtype", "n_pages", "n_tails",
                  "n_kv_heads", "head_dim", "c", "ref")
@@ -90,7 +92,8 @@ class KVBatch:
     tails [B, 2]   the tail before the step and after it; where the step completes a page they
                    must differ (a step run again then reads what it read before)
     max_new, max_len: the largest number of new tokens and of tokens after the step of a
-    sequence. They choose launch shapes; a wrong value costs time, not results. Rows of q, k
+    sequence. They choose launch shapes; a wrong value costs time, not results (kv_append asks for
+    a rope of max_len positions). Rows of q, k
     and v that no sequence covers are not read, and their outputs are not defined.
     total: the rows of all sequences, where the host knows them: calls with another number of
     rows are then refused. None: rows that reach past the given ones drop their sequence, which
@@ -346,6 +349,7 @@ class PagedKVCache:
         cache.drop(a)
 
     A page number names the same page in every layer's pool. kind: torch.int8 or torch.float8_e4m3fn.
+    Where a step's calls raise, `undo(step)` takes it back.
     Memory: each page 64 * head_dim * kv_heads * 2 bytes a layer, each sequence two tails of four
     times that in all (a tail is bf16 and has a second one to move to when its page is completed)."""
 

@@ -29,7 +29,9 @@ extern "C" {
 /* One layer's storage, device memory, 16-byte aligned. A full page is held in
  * 8 bits with one scale per kv head for K and one for V; the tokens of a
  * sequence's unfinished page are held in bf16 in a tail, from which the page
- * is quantised once, when it is full. Value = code * scale. */
+ * is quantised once, when it is full. Value = code * scale. bs_kv_attend takes
+ * v_scale as bs_kv_append leaves it, positive and between 2^-49 and 2^54 (a page
+ * of zeros among them): under a v_scale of 0 a page's keys lose their weight. */
 typedef struct {
     void *k;            /* [n_pages][n_kv_heads][64][head_dim] */
     void *v;            /* [n_pages][n_kv_heads][head_dim][64]: tokens innermost */
@@ -103,7 +105,8 @@ typedef struct {
  * included (append first). Score s = scale * q.k, then softcap * tanh(s /
  * softcap), then minus slope * |p - j|; key j is seen by the row at position p
  * if j <= p or j < prefix, and j >= first, and j > p - window. A row that sees
- * nothing gives 0 and lse -inf. d_work: bs_kv_attend_work_bytes bytes of
+ * nothing gives 0 and lse -inf. Scores, softmax and sums are f32; the weights
+ * are f16 in the product with V (over a tail two bf16 parts). d_work: bs_kv_attend_work_bytes bytes of
  * scratch, 16-byte aligned (0 bytes may be NULL). */
 uint64_t bs_kv_attend_work_bytes(const bs_kv_pool *pool, const bs_kv_batch *batch, uint32_t n_q_heads);
 int bs_kv_attend(const bs_kv_pool *pool, const bs_kv_batch *batch, const bs_kv_query *query, void *d_work,
