@@ -175,3 +175,18 @@ def test_strides_of_dimensions_of_one(unaligned):
     x = rig.rows(1).cuda()
     odd = x.as_strided(x.shape, (d, 5, 1))
     assert torch.equal(bs.kv_attend(rig.pool, rig.batch, odd), bs.kv_attend(rig.pool, rig.batch, x))
+
+
+@pytest.mark.parametrize("cap", [40.0, 100.0, 2000.0])
+@pytest.mark.parametrize("starts,news,d,scale", [([700, 64, 13], [1, 3, 1], 64, 0.125), ([300, 0, 5], [90, 65, 1], 80, -0.4), ([300, 20], [70, 1], 256, 0.3)])
+def test_large_caps_beside_biases_and_masks(cap, starts, news, d, scale):
+    import bigsmall_amd as bs
+    _say("cap and masks", cap, starts, news, d, scale)
+    rig = Rig(starts, news, 2, d, torch.float8_e4m3fn, seed=d + 1)
+    q = rig.rows(4)
+    pos = torch.cat([s + torch.arange(n) for s, n in zip(starts, news)])
+    options = dict(softcap=cap, slopes=torch.tensor([0.5, 0.0, 0.25, 0.01]), window=130, first=(pos // 37 * 37).to(torch.int32),
+                   prefix=torch.tensor([40, 100, 3][:len(starts)], dtype=torch.int32))
+    gpu = {n: x.cuda() if isinstance(x, torch.Tensor) else x for n, x in options.items()}
+    out, lse = bs.kv_attend(rig.pool, rig.batch, q.cuda(), scale=scale, return_lse=True, **gpu)
+    _check_attend(rig, q, out, lse, scale, **options)
