@@ -12,6 +12,9 @@ kernels on the GPU:
     decompress_delta(delta, base), load_delta(delta, base) -> a fine-tune from its XOR delta
     CompressedKVCache                       -> KV entries and blocks decoded on the GPU
     PagedKVCache, kv_append, kv_attend, kv_read -> a paged 8-bit KV cache filled, attended to and read back on the GPU
+    KVTables                                -> that cache's tables built on the GPU, drafted tokens taken back
+    Fp8Weight, fp8_quantise, fp8_linear     -> products of e4m3 weights with a scale for each block of 128
+    draft_verify                            -> drafted tokens against the model's probabilities
     paged_llama.PagedLlama                  -> a Llama-architecture model generating from it, layers streamed
     codec_registry.register_codec / get_codec / auto_select_codec
     compress_for_hub(model_dir, out_dir), from_pretrained(path) -> multi-shard .bs models + index
@@ -29,14 +32,20 @@ from .streaming import StreamingLoader, decompress_layers
 from .verify import verify
 
 
-_PAGED_KV = ("PagedKVCache", "KVPool", "KVBatch", "Rope", "kv_append", "kv_attend", "kv_read")
+# what imports torch, which the rest imports on first use only
+_WITH_TORCH = {"paged_kv": ("PagedKVCache", "KVPool", "KVBatch", "Rope", "kv_append", "kv_attend", "kv_read"),
+               "kv_tables": ("KVTables", "StepRows"),
+               "fp8": ("Fp8Weight", "Fp8Rows", "fp8_quantise", "fp8_linear"),
+               "draft": ("draft_verify",)}
 
 
 def __getattr__(name):
-    if name in _PAGED_KV:         # imports torch, which the rest imports on first use only
-        from . import paged_kv
-        globals().update({n: getattr(paged_kv, n) for n in _PAGED_KV})
-        return globals()[name]
+    for module, names in _WITH_TORCH.items():
+        if name in names:
+            from importlib import import_module
+            found = import_module("." + module, __name__)
+            globals().update({n: getattr(found, n) for n in names})
+            return globals()[name]
     # transformers/accelerate are only needed by the streaming model
     if name == "BigSmallStreamingModel":
         from .streaming_inference import BigSmallStreamingModel
@@ -53,5 +62,6 @@ def __getattr__(name):
 __all__ = ["compress", "decompress", "load", "info", "verify", "StreamingLoader", "BigSmallStreamingModel",
            "decompress_layers", "decompress_delta", "load_delta",
            "CompressedKVCache", "PagedKVCache", "KVPool", "KVBatch", "Rope", "kv_append", "kv_attend", "kv_read",
+           "KVTables", "StepRows", "Fp8Weight", "Fp8Rows", "fp8_quantise", "fp8_linear", "draft_verify",
            "BigSmallVersionError", "DecodeError", "compress_for_hub", "from_pretrained",
            "__version__"]

@@ -35,7 +35,7 @@ class BsChunkInfo(ctypes.Structure):
                 ("plane_mode", ctypes.c_uint32), ("coder", ctypes.c_uint32)]
 
 
-# (restype, argtypes) of every symbol include/bigsmall_hip.h and bigsmall_kv.h declare
+# (restype, argtypes) of every symbol that the headers in include/ declare
 _P, _U8P = ctypes.c_void_p, ctypes.c_void_p
 _U32, _U64, _I32, _INT = ctypes.c_uint32, ctypes.c_uint64, ctypes.c_int32, ctypes.c_int
 SIGNATURES = {
@@ -67,6 +67,14 @@ SIGNATURES = {
     "bs_kv_attend_work_bytes": (_U64, [_P, _P, _U32]),
     "bs_kv_attend": (_INT, [_P, _P, _P, _P, _U64, _P, _P]),
     "bs_kv_read": (_INT, [_P, _P, _U32, _P, _U32, _P, _P, _P, _P]),
+    "bs_kv_books_step": (_INT, [_P, _P, _P, _P, _P, _P]),
+    "bs_kv_books_keep": (_INT, [_P, _P, _P, _P, _P]),
+    "bs_kv_books_drop": (_INT, [_P, _P, _U32, _P, _P]),
+    "bs_fp8_quantise": (_INT, [_P, _U32, ctypes.c_int64, _P, _P]),
+    "bs_fp8_linear_work_bytes": (_U64, [_P, _P]),
+    "bs_fp8_linear": (_INT, [_P, _P, _P, _U32, ctypes.c_int64, _P, _U64, _P]),
+    "bs_draft_verify_work_bytes": (_U64, [_U32, _U32]),
+    "bs_draft_verify": (_INT, [_P, _P, _U64, _P, _P]),
 }
 
 
@@ -91,6 +99,34 @@ class BsKvQuery(ctypes.Structure):
     _fields_ = [(n, _P) for n in ("q", "out", "lse", "slopes", "prefix", "first")] + \
                [("q_token", ctypes.c_int64), ("q_head", ctypes.c_int64), ("n_q_heads", _U32), ("window", _U32),
                 ("scale", ctypes.c_float), ("softcap", ctypes.c_float)]
+
+
+
+class BsKvBooks(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("length", "which", "table", "free", "n_free", "tails")] + \
+               [(n, _U32) for n in ("n_places", "cols", "n_pages")]
+
+
+class BsKvTables(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("seqs", "start", "cu", "tails", "table", "owner", "position", "slot")] + \
+               [(n, _U32) for n in ("n_seqs", "n_rows", "max_new")]
+
+
+# include/bigsmall_fp8.h
+class BsFp8Rows(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("codes", "scales")] + [(n, _U32) for n in ("rows", "cols", "code_stride", "scale_stride")]
+
+
+class BsFp8Weight(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("codes", "scales")] + [(n, _U32) for n in ("outer", "inner", "stride", "scale_stride")]
+
+
+# include/bigsmall_draft.h
+class BsDraftBatch(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("p", "q", "draft", "accept", "cu", "pick", "tokens", "counts")] + \
+               [(n, ctypes.c_int64) for n in ("p_stride", "q_stride")] + \
+               [(n, _U32) for n in ("type", "n_rows", "vocab", "n_seqs", "max_drafts")]
+
 
 _lib = None
 

@@ -118,6 +118,47 @@ int bs_kv_attend(const bs_kv_pool *pool, const bs_kv_batch *batch, const bs_kv_q
 int bs_kv_read(const bs_kv_pool *pool, const int32_t *d_pages, uint32_t n_cols, const int32_t *d_tail, uint32_t n,
                uint16_t *d_k, uint16_t *d_v, int32_t *d_status, void *stream);
 
+/* The books of a cache on the GPU: which pages and tails belong to which sequence. A place holds a sequence of `length`
+ * tokens: its first length / 64 pages are in its row of `table`, the rest of its tokens in tail tails[place] +
+ * which[place]. Pages that nobody holds are free[0 .. n_free - 1], taken from the end. */
+typedef struct {
+    int32_t *length, *which; /* [n_places] */
+    int32_t *table;          /* [n_places][cols] */
+    int32_t *free;           /* [n_pages] */
+    int32_t *n_free;         /* one number */
+    const int32_t *tails;    /* [n_places] the first of a place's two tails */
+    uint32_t n_places;       /* at most 65536 */
+    uint32_t cols, n_pages;  /* cols * 64 tokens at most in a place */
+} bs_kv_books;
+
+/* A step over them. The arrays are a bs_kv_batch's, and of each row its sequence's number in the step, its position
+ * and place * cols * 64 + position; -1 for rows that no sequence covers. */
+typedef struct {
+    const int32_t *seqs;     /* [n_seqs] places, each once */
+    int32_t *start, *cu, *tails, *table; /* [n_seqs], [n_seqs + 1], [n_seqs][2], [n_seqs][cols] */
+    int32_t *owner, *position; /* [n_rows] */
+    int64_t *slot;           /* [n_rows] */
+    uint32_t n_seqs, n_rows; /* n_seqs at most n_places */
+    uint32_t max_new;        /* the largest number of new tokens: a launch shape only */
+} bs_kv_tables;
+
+/* The tables of a step that brings d_new[b] tokens (none is allowed) to place seqs[b]. The first d_sure[b] of them (NULL:
+ * all) are certain. The others may be taken back by bs_kv_books_keep, so a sequence gets as many of them as complete no
+ * page: a page is quantised once. Table entries past a sequence's pages are 0. The books stay as they are; a step made
+ * anew before bs_kv_books_keep replaces the one before. All or nothing: where places are no places or named twice,
+ * numbers negative or lengths wrong (BS_DEV_ERR_BOUNDS), or where pages, rows or a place's columns do not suffice
+ * (BS_DEV_ERR_COUNT), no sequence has a new token. */
+int bs_kv_books_step(const bs_kv_books *books, const bs_kv_tables *step, const int32_t *d_new, const int32_t *d_sure,
+                     int32_t *d_status, void *stream);
+
+/* Enter the last step into the books: of sequence b's new tokens the first d_kept[b] stay (NULL: all), held to what is
+ * certain and what there is. Once. */
+int bs_kv_books_keep(const bs_kv_books *books, const bs_kv_tables *step, const int32_t *d_sure, const int32_t *d_kept,
+                     void *stream);
+
+/* Empty places: their pages become free, the first sequence's first page the last to be taken. All or nothing, as above. */
+int bs_kv_books_drop(const bs_kv_books *books, const int32_t *d_seqs, uint32_t n_seqs, int32_t *d_status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
