@@ -25,7 +25,7 @@ from . import _native
 
 BLOCK = 128
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
-_MOST_ROWS, _MOST_COLS = 65535 * 16, 1 << 24
+_MOST_ROWS, _MOST_COLS, _MOST_STRIDE = 65535 * 16, 1 << 22, 1 << 23
 
 
 def _blocks(n: int) -> int:
@@ -76,7 +76,7 @@ class Fp8Weight:
         if scales.device != codes.device:
             raise ValueError(f"Fp8Weight: scales are on {scales.device}, codes on {codes.device}")
         stride = codes.stride(0) if n > 1 else _blocks(k) * BLOCK
-        if k % BLOCK or (k > 1 and codes.stride(1) != 1) or stride % BLOCK or not k <= stride < 1 << 32 or codes.data_ptr() % 16:
+        if k % BLOCK or (k > 1 and codes.stride(1) != 1) or stride % BLOCK or not k <= stride <= _MOST_STRIDE or codes.data_ptr() % 16:
             padded = torch.zeros(n, _blocks(k) * BLOCK, dtype=torch.uint8, device=codes.device)
             padded[:, :k] = codes.view(torch.uint8)
             codes, stride = padded.view(torch.float8_e4m3fn)[:, :k], padded.shape[1]

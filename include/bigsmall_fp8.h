@@ -25,8 +25,8 @@ extern "C" {
 
 /* Rows of e4m3 (OCP, finite) codes with a scale for each 128 columns:
  * x[t][k] = codes[t * code_stride + k] * scales[(k / 128) * scale_stride + t].
- * code_stride is a multiple of 128, codes from `cols` on to it are 0, both
- * bases 16-byte aligned. */
+ * code_stride is `cols` rounded up to a multiple of 128, codes from `cols` on to it
+ * are 0, both bases 16-byte aligned. At most 65,535 * 16 rows and 2^22 columns. */
 typedef struct {
     uint8_t *codes;
     float *scales;      /* [ceil(cols / 128)][scale_stride]: a block's rows next to one another */
@@ -40,8 +40,8 @@ typedef struct {
  * infinity or a NaN has codes 0 and scale NaN. */
 int bs_fp8_quantise(const void *x, uint32_t type, int64_t x_stride, const bs_fp8_rows *out, void *stream);
 
-/* A weight [outer][inner]: codes as above, `stride` bytes from row to row (a multiple of 128, zeros
- * from `inner` on), and scales[outer / 128][inner / 128], both rounded up. */
+/* A weight [outer][inner]: codes as above, `stride` bytes from row to row (a multiple of 128, 2^23 at most,
+ * zeros from `inner` to the next multiple of 128), and scales[outer / 128][inner / 128], both rounded up. */
 typedef struct {
     const uint8_t *codes;
     const float *scales;
