@@ -71,8 +71,9 @@ SIGNATURES = {
     "bs_kv_books_keep": (_INT, [_P, _P, _P, _P, _P]),
     "bs_kv_books_drop": (_INT, [_P, _P, _U32, _P, _P]),
     "bs_fp8_quantise": (_INT, [_P, _U32, ctypes.c_int64, _P, _P]),
-    "bs_fp8_linear_work_bytes": (_U64, [_P, _P]),
-    "bs_fp8_linear": (_INT, [_P, _P, _P, _U32, ctypes.c_int64, _P, _U64, _P]),
+    "bs_fp8_linear_values_work_bytes": (_U64, [_U32, _P]),
+    "bs_fp8_linear_values": (_INT, [_P, _U32, ctypes.c_int64, _U32, _P, _P, _U32, ctypes.c_int64, _P, _U64, _P]),
+    "bs_fp8_linear": (_INT, [_P, _P, _P, _U32, ctypes.c_int64, _P]),
     "bs_draft_verify_work_bytes": (_U64, [_U32, _U32]),
     "bs_draft_verify": (_INT, [_P, _P, _U64, _P, _P]),
 }

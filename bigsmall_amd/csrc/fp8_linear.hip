@@ -13,7 +13,9 @@
 // every code converted first.
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "bigsmall_fp8.h"
 #include "lds_limit.h"
@@ -60,6 +62,55 @@ __device__ __forceinline__ float quotient(float v, float a, float inv) {
   return __builtin_fmaf(__builtin_fmaf(-q, a, v), inv, q);
 }
 
+// Eight columns of a row, from column k on; 0 past the last one.
+struct Eight {
+  uint16_t v[8];
+};
+template <bool WIDE>
+__device__ __forceinline__ Eight load_eight(const uint16_t* row, uint32_t k, uint32_t cols) {
+  Eight e = {};
+  if (WIDE && k + 8 <= cols) {
+    *(uint4*)e.v = *(const uint4*)(row + k);
+  } else {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+      if (k + i < cols) e.v[i] = row[k + i];
+  }
+  return e;
+}
+
+// Sixteen lanes quantise a block, eight columns each: a lane's eight codes, and the scale.
+template <int TYPE>
+__device__ __forceinline__ uint2 quantise_block(const Eight& x, float& scale) {
+  float f[8], a = 0;
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    f[e] = load16<TYPE>(x.v[e]);
+    bad = bad || !(fabsf(f[e]) < INFINITY);
+    a = fmaxf(a, fabsf(f[e]));
+  }
+  a = bad ? INFINITY : a;
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
+  bad = a == INFINITY;
+  a = fmaxf(a, AMAX_LO);
+  // near the end of f32's range both sides are taken by 2^-16
+  const float down = a > 0x1p100f ? 0x1p-16f : 1.0f, b = a * down, inv = 1.0f / b;
+  uint32_t w[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = quotient(f[4 * p + e] * down * 448.0f, b, inv);
+    w[p] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    w[p] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)w[p], true);
+    w[p] = bad ? 0u : w[p];
+  }
+  scale = bad ? __uint_as_float(0x7FC00000u) : a / 448.0f;
+  return make_uint2(w[0], w[1]);
+}
+
 template <int TYPE, bool WIDE>
 __global__ __launch_bounds__(Q_THREADS) void quantise_kernel(const uint16_t* x, int64_t x_stride, bs_fp8_rows R) {
   const uint32_t lane = threadIdx.x % 16, blocks = R.code_stride / BLOCK;
@@ -67,49 +118,16 @@ __global__ __launch_bounds__(Q_THREADS) void quantise_kernel(const uint16_t* x, 
   if (t >= R.rows) return;
   const uint16_t* row = x + (int64_t)t * x_stride;
   const uint32_t j0 = blockIdx.x * Q_BLOCKS;
-  uint16_t v[Q_BLOCKS][8] = {};
+  Eight v[Q_BLOCKS];
 #pragma unroll
-  for (uint32_t i = 0; i < Q_BLOCKS; ++i) {
-    const uint32_t k = (j0 + i) * BLOCK + lane * 8;
-    if (WIDE && k + 8 <= R.cols) {
-      *(uint4*)v[i] = *(const uint4*)(row + k);
-    } else {
-#pragma unroll
-      for (uint32_t e = 0; e < 8; ++e)
-        if (k + e < R.cols) v[i][e] = row[k + e];
-    }
-  }
+  for (uint32_t i = 0; i < Q_BLOCKS; ++i) v[i] = load_eight<WIDE>(row, (j0 + i) * BLOCK + lane * 8, R.cols);
 #pragma unroll
   for (uint32_t i = 0; i < Q_BLOCKS; ++i) {
     const uint32_t j = j0 + i;
     if (j >= blocks) break;
-    float f[8], a = 0;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      f[e] = load16<TYPE>(v[i][e]);
-      bad = bad || !(fabsf(f[e]) < INFINITY);
-      a = fmaxf(a, fabsf(f[e]));
-    }
-    a = bad ? INFINITY : a;
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) a = fmaxf(a, __shfl_xor(a, d));
-    bad = a == INFINITY;
-    a = fmaxf(a, AMAX_LO);
-    // near the end of f32's range both sides are taken by 2^-16
-    const float down = a > 0x1p100f ? 0x1p-16f : 1.0f, b = a * down, inv = 1.0f / b;
-    uint32_t w[2];
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = quotient(f[4 * p + e] * down * 448.0f, b, inv);
-      w[p] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-      w[p] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], (int)w[p], true);
-      w[p] = bad ? 0u : w[p];
-    }
-    *(uint2*)(R.codes + t * R.code_stride + j * BLOCK + lane * 8) = make_uint2(w[0], w[1]);
-    if (lane == 0) R.scales[(uint64_t)j * R.scale_stride + t] = bad ? __uint_as_float(0x7FC00000u) : a / 448.0f;
+    float scale;
+    *(uint2*)(R.codes + t * R.code_stride + j * BLOCK + lane * 8) = quantise_block<TYPE>(v[i], scale);
+    if (lane == 0) R.scales[(uint64_t)j * R.scale_stride + t] = scale;
   }
 }
 
@@ -123,7 +141,11 @@ int quantise_launch(const void* x, int64_t stride, const bs_fp8_rows& R, hipStre
   return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
 }
 
-// ---- the product
+int quantise(const void* x, uint32_t type, int64_t stride, const bs_fp8_rows& R, hipStream_t s) {
+  return type == BS_FP8_BF16 ? quantise_launch<BS_FP8_BF16>(x, stride, R, s) : quantise_launch<BS_FP8_F16>(x, stride, R, s);
+}
+
+// ---- the product: what its kernels share
 
 __device__ __forceinline__ f32x4 product(i32x8 w, i32x8 x) {
   // (scales of 0 name the form without scales: e4m3 as it is)
@@ -135,20 +157,68 @@ __device__ __forceinline__ i32x8 load_operand(const uint8_t* p, const uint8_t* q
   return i32x8{lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 }
 
-// A workgroup's tile: WN by WT waves, each NT by TT results of 16 by 16. The rows of a wave lie in one block of the weight.
-template <int WN_, int WT_, int NT_, int TT_>
-struct Tile {
-  static constexpr uint32_t WN = WN_, WT = WT_, NT = NT_, TT = TT_;
-  static constexpr uint32_t WAVES = WN * WT, THREADS = WAVES * 64, N = WN * NT * 16, T = WT * TT * 16;
-  static constexpr uint32_t STAGE = (N + T) * BLOCK;           // bytes of LDS for one block of both operands
-  static constexpr uint32_t LOADS = (N + T) / 8 / WAVES;       // of a wave, 1 KiB each: eight rows
-  static_assert(NT * 16 <= BLOCK && (N + T) % (8 * WAVES) == 0 && BLOCK % (NT * 16) == 0, "");
-};
+// Sixteen rows of 128 bytes in LDS as an operand: chunk c of row r lies at place c ^ (r % 8), and a lane holds chunks g and g + 4 of its row.
+__device__ __forceinline__ i32x8 read_rows(const uint8_t* rows, uint32_t i) {
+  const uint32_t lane = threadIdx.x % 64, at = (lane % 16) * BLOCK + ((lane / 16) ^ (lane % 8)) * 16;
+  return load_operand(rows + i * 16 * BLOCK + at, rows + i * 16 * BLOCK + (at ^ 64));
+}
 
+// One block of NT by TT pairs of 16 rows in LDS, scaled by s and added to sum. Step k multiplies one pair and sums up the product
+// of step k - LAG, while rows for later steps are read; the barriers keep the compiler from putting each product next to its
+// sums again, where it waits for the matrix unit (8,192 rows through 14,336 x 4,096: 690 us that way, 445 this way).
+// also(k) is done in step k: loads of other blocks, so that they queue up beside the products and not before them.
+template <uint32_t NT, uint32_t TT, class F>
+__device__ __forceinline__ void multiply(const uint8_t* wrows, const uint8_t* xrows, const float (&s)[TT], f32x4 (&sum)[NT][TT], F&& also) {
+  constexpr uint32_t LAG = 3;
+  i32x8 b[TT], a[3];
+  f32x4 d[LAG + 1];
+  a[0] = read_rows(wrows, 0);
+#pragma unroll
+  for (uint32_t c = 0; c < TT; ++c) b[c] = read_rows(xrows, c);
+  if (NT > 1) a[1] = read_rows(wrows, 1);
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (uint32_t k = 0; k < NT * TT + LAG; ++k) {
+    const uint32_t i = k / TT, c = k % TT;
+    if (k < NT * TT) {
+      also(k);
+      d[k % (LAG + 1)] = product(a[i % 3], b[c]);
+    }
+    if (c == 0 && i + 2 < NT) a[(i + 2) % 3] = read_rows(wrows, i + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    if (k >= LAG) {
+      const uint32_t o = k - LAG;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[o / TT][o % TT][r] = __builtin_fmaf(s[o % TT], d[o % (LAG + 1)][r], sum[o / TT][o % TT][r]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+// 16 or 4 bytes a lane from base + from + at to LDS: base and at are the same in all lanes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)base, 0, 0xFFFFFFFFu, 0x00020000);
+}
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t base, uint32_t from, uint32_t at, uint8_t* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (LDS void*)to, 16, (int)from, (int)at, 0, 0);
+}
+__device__ __forceinline__ void load_lds4(__amdgpu_buffer_rsrc_t base, uint32_t from, uint32_t at, uint8_t* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(base, (LDS void*)to, 4, (int)from, (int)at, 0, 0);
+}
+
+// Wait until `left` of the wave's loads are under way.
+template <uint32_t left>
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt((left & 15) | (left >> 4) << 14 | 0x0F70);
+  asm volatile("" ::: "memory");
+}
+
+// A barrier for what the waves have read from LDS, or had brought there and waited for. (A fence would wait for all loads that are
+// on their way to LDS.)
 __device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  asm volatile("" ::: "memory");
 }
 
 // Consecutive workgroups go to the eight dies in turn. Each die gets a run of tiles, and walks them in strips of
@@ -162,146 +232,377 @@ __device__ __forceinline__ void tile_at(uint32_t wg, uint32_t tiles_n, uint32_t 
   n = in / wide;
 }
 
-constexpr uint32_t LAG = 3;
+// Four neighbouring results of a row, `count` of them there.
+template <int TYPE>
+__device__ __forceinline__ uint2 pack4(f32x4 v) {
+  uint16_t h[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) h[r] = store16<TYPE>(v[r]);
+  return make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+}
+__device__ __forceinline__ void store4(uint16_t* p, f32x4 v, uint32_t count, uint32_t type) {
+  const uint2 w = type == BS_FP8_BF16 ? pack4<BS_FP8_BF16>(v) : pack4<BS_FP8_F16>(v);
+  if (count >= 4 && ((uintptr_t)p & 7) == 0) {
+    *(uint2*)p = w;
+  } else {
+#pragma unroll
+    for (uint32_t r = 0; r < 4; ++r)
+      if (r < count) p[r] = (uint16_t)((r < 2 ? w.x : w.y) >> (r % 2 * 16));
+  }
+}
 
-// Both operands of a block of 128 columns go to LDS directly while the block before it is multiplied. The bound is the matrix unit: a
-// wave's step is an instruction of 32 cycles and four sums of four. 8,192 rows through 14,336 x 4,096: 445 us, 2.16 PFLOP/s, where the
-// library's product with one scale reaches 2.9.
-template <class S, int TYPE>
-__global__ __launch_bounds__(S::THREADS) void tile_kernel(bs_fp8_rows X, bs_fp8_weight W, uint16_t* y, int64_t y_stride, uint32_t tiles_n,
-                                                          uint32_t tiles_t) {
+struct Args {
+  bs_fp8_rows x;
+  bs_fp8_weight w;
+  uint16_t* y;
+  int64_t y_stride;
+  uint32_t type;  // y's
+  uint32_t tiles_n, tiles_t;
+};
+
+// ---- tiles: a workgroup's waves share each block
+
+// WN by WT waves, each NT by TT results of 16 by 16, STAGES blocks of both operands in LDS. The rows of a wave lie in one block of
+// the weight. The bound of the large one is LDS: reads and loads take its 128 bytes a clock for as long as the matrix unit is
+// busy, and a block's loads take about as long to come as the block before it to be multiplied. 8,192 rows through 14,336 x 4,096: 441
+// us, 2.18 PFLOP/s, where the library's product with a single scale reaches 2.9 (without the loads 306 us, without waiting for them
+// 394). x read into registers instead, in an order that suits it: 411 us and 17 to bring it there.
+template <int WN_, int WT_, int NT_, int TT_, int STAGES_>
+struct Tile {
+  static constexpr uint32_t WN = WN_, WT = WT_, NT = NT_, TT = TT_, STAGES = STAGES_;
+  static constexpr uint32_t WAVES = WN * WT, THREADS = WAVES * 64, N = WN * NT * 16, T = WT * TT * 16;
+  static constexpr uint32_t CODES = (N + T) * BLOCK, STAGE = CODES + WAVES * 256;  // bytes: codes, each wave's scales of x
+  static constexpr uint32_t LOADS = (N + T) / 8 / WAVES;       // of a wave, 1 KiB each: eight rows
+  static constexpr uint32_t OUT = WAVES * TT * 16 * NT * 32;   // bytes of the results on their way out
+  static constexpr uint32_t LDS_BYTES = STAGES * STAGE > OUT ? STAGES * STAGE : OUT;
+  static_assert(TT <= 4 && BLOCK % (NT * 16) == 0 && (N + T) % (8 * WAVES) == 0 && LDS_BYTES <= 160 * 1024, "");
+};
+
+// A wave's results out through LDS (its own part of it), so that a row's leave side by side: rows of NT * 32 bytes, 16 bytes q of row
+// t at place q ^ (t % (NT * 2)).
+template <uint32_t NT, uint32_t TT, int TYPE>
+__device__ __forceinline__ void store_tile(uint8_t* own, const f32x4 (&sum)[NT][TT], const Args& A, uint32_t t0, uint32_t n0) {
+  constexpr uint32_t ROW = NT * 32, QS = ROW / 16;
+  const uint32_t lane = threadIdx.x % 64;
+#pragma unroll
+  for (uint32_t c = 0; c < TT; ++c)
+#pragma unroll
+    for (uint32_t i = 0; i < NT; ++i) {
+      const uint32_t t = c * 16 + lane % 16, u = i * 4 + lane / 16;
+      *(uint2*)(own + t * ROW + ((u / 2) ^ (t % QS)) * 16 + u % 2 * 8) = pack4<TYPE>(sum[i][c]);
+    }
+  const bool wide = (((uintptr_t)A.y | (uint64_t)A.y_stride * 2) & 15) == 0;
+#pragma unroll 4
+  for (uint32_t k = lane; k < TT * 16 * QS; k += 64) {
+    const uint32_t t = k / QS, q = k % QS, n = n0 + q * 8;
+    const uint4 v = *(const uint4*)(own + t * ROW + (q ^ (t % QS)) * 16);
+    if (t0 + t >= A.x.rows) break;
+    uint16_t* row = A.y + (int64_t)(t0 + t) * A.y_stride;
+    if (wide && n + 8 <= A.w.outer) {
+      *(uint4*)(row + n) = v;
+    } else {
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (uint32_t r = 0; r < 8; ++r)
+        if (n + r < A.w.outer) row[n + r] = (uint16_t)(w[r / 2] >> (r % 2 * 16));
+    }
+  }
+}
+
+template <class S>
+__global__ __launch_bounds__(S::THREADS, 2) void tile_kernel(Args A) {
   BS_DYNAMIC_LDS(lds);
+  const bs_fp8_rows& X = A.x;
+  const bs_fp8_weight& W = A.w;
   const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t wn = wave / S::WT, wt = wave % S::WT;
   uint32_t tn, tt;
-  tile_at(blockIdx.x, tiles_n, tiles_t, tn, tt);
+  tile_at(blockIdx.x, A.tiles_n, A.tiles_t, tn, tt);
   const uint32_t n0 = tn * S::N, t0 = tt * S::T, blocks = X.code_stride / BLOCK;
 
-  // What a lane brings to LDS: of each eight rows, 16 bytes of one. Chunk c of row r goes to place c ^ (r % 8), so that the
-  // eight rows that a read touches at once lie in different banks; rows past the end repeat the last one.
+  // What a lane brings to LDS: of each eight rows, 16 bytes of one, chunk c of row r to place c ^ (r % 8): the eight rows that a
+  // read touches at once lie in different banks. Rows past the end repeat the last one. One load more brings the scales of
+  // the wave's rows of x.
   uint32_t from[S::LOADS];
 #pragma unroll
   for (uint32_t i = 0; i < S::LOADS; ++i) {
     const uint32_t r = (wave + i * S::WAVES) * 8 + lane / 8, c = ((lane % 8) ^ (lane / 8)) * 16;
     from[i] = r < S::N ? min(r, W.outer - 1 - n0) * W.stride + c : min(r - S::N, X.rows - 1 - t0) * X.code_stride + c;
   }
-  const uint8_t* wbase = W.codes + (uint64_t)n0 * W.stride;
-  const uint8_t* xbase = X.codes + (uint64_t)t0 * X.code_stride;
-  const auto fetch = [&](uint32_t j) {
-#pragma unroll
-    for (uint32_t i = 0; i < S::LOADS; ++i) {
-      const uint32_t piece = wave + i * S::WAVES;
-      const uint8_t* base = (piece * 8 < S::N ? wbase : xbase) + (uint64_t)j * BLOCK;
-      __builtin_amdgcn_global_load_lds((const GLB void*)(base + from[i]), (LDS void*)(lds + (j & 1) * S::STAGE + piece * 1024), 16, 0, 0);
-    }
+  const auto wbase = buffer(W.codes + (uint64_t)n0 * W.stride), xbase = buffer(X.codes + (uint64_t)t0 * X.code_stride);
+  const uint32_t scale_at = min(t0 + wt * S::TT * 16 + lane % (S::TT * 16), X.rows - 1) * 4;
+  const auto fetch = [&](uint32_t i, uint32_t j, uint32_t slot) {  // load i of block j
+    uint8_t* stage = lds + slot * S::STAGE;
+    const uint32_t piece = wave + i * S::WAVES;
+    if (i < S::LOADS)
+      load_lds16(piece * 8 < S::N ? wbase : xbase, from[i], j * BLOCK, stage + piece * 1024);
+    else
+      load_lds4(buffer(X.scales + (uint64_t)j * X.scale_stride), scale_at, 0, stage + S::CODES + wave * 256);
   };
-  uint32_t ts[S::TT];
-#pragma unroll
-  for (uint32_t c = 0; c < S::TT; ++c) ts[c] = min(t0 + (wt * S::TT + c) * 16 + lane % 16, X.rows - 1);
-  const uint32_t nb = min(n0 + wn * S::NT * 16, W.outer - 1) / BLOCK;
-  const float* ws = W.scales + (uint64_t)nb * W.scale_stride;
-  float xs[S::TT], wsj = ws[0];
-#pragma unroll
-  for (uint32_t c = 0; c < S::TT; ++c) xs[c] = X.scales[ts[c]];
+  const float* ws = W.scales + (uint64_t)(min(n0 + wn * S::NT * 16, W.outer - 1) / BLOCK) * W.scale_stride;
+  // the weight's scales, 64 blocks at a time, one a lane, and those after them
+  float ws64 = ws[min(lane, blocks - 1)], ws_next = ws[min(64 + lane, blocks - 1)];
 
   f32x4 sum[S::NT][S::TT] = {};
-  fetch(0);
-  // A fragment's two chunks of a lane, in its rows
-  const uint32_t at0 = (lane % 16) * BLOCK + (((lane / 16) * 2) ^ (lane % 8)) * 16, at1 = at0 ^ 16;
-  for (uint32_t j = 0; j < blocks; ++j) {
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this block's codes and scales
+  wait_loads<0>();
+#pragma unroll
+  for (uint32_t i = 0; i + 1 < S::STAGES; ++i)
+    if (i < blocks) {
+#pragma unroll
+      for (uint32_t k = 0; k <= S::LOADS; ++k) fetch(k, i, i);
+    }
+  uint32_t slot = 0;
+  const auto block = [&](uint32_t j, auto more) {
+    // this block's loads are done, the STAGES - 2 blocks' after it may go on
+    wait_loads<more ? (S::STAGES - 2) * (S::LOADS + 1) : 0>();
     lds_barrier();
+    const uint8_t* stage = lds + slot * S::STAGE;
+    const uint32_t ahead = slot == 0 ? S::STAGES - 1 : slot - 1;  // where the block before this one was
+    slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+    if (j != 0 && j % 64 == 0) ws64 = ws_next, ws_next = ws[min(j + 64 + lane, blocks - 1)];
+    const float wsj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ws64), j % 64));
     float s[S::TT];
 #pragma unroll
-    for (uint32_t c = 0; c < S::TT; ++c) s[c] = xs[c] * wsj;
-    if (j + 1 < blocks) {
-      wsj = ws[j + 1];
+    for (uint32_t c = 0; c < S::TT; ++c) s[c] = ((const float*)(stage + S::CODES + wave * 256))[c * 16 + lane % 16] * wsj;
+    multiply<S::NT, S::TT>(stage + wn * S::NT * 16 * BLOCK, stage + (S::N + wt * S::TT * 16) * BLOCK, s, sum, [&](uint32_t k) {
+      // With two stages the loads have to be back one block later, so they go out at once; else spread over the steps (128 by
+      // 128, four stages, 112 blocks: 79 us at once, 59 spread; two stages: 84 and 93).
+      constexpr uint32_t STEPS = S::STAGES == 2 ? 1 : S::NT * S::TT, ALL = S::LOADS + 1;
+      if constexpr (more) {
 #pragma unroll
-      for (uint32_t c = 0; c < S::TT; ++c) xs[c] = X.scales[(uint64_t)(j + 1) * X.scale_stride + ts[c]];
-      fetch(j + 1);
-    }
-    const uint8_t* stage = lds + (j & 1) * S::STAGE;
-    const uint8_t* wrows = stage + wn * S::NT * 16 * BLOCK;
-    const uint8_t* xrows = stage + (S::N + wt * S::TT * 16) * BLOCK;
-    // Step k multiplies one pair of 16 rows and sums up the product of step k - LAG, while the pair of rows for TT steps
-    // later is read; the barriers keep the compiler from putting each product next to its sums again.
-    const auto read = [&](const uint8_t* rows, uint32_t i) { return load_operand(rows + i * 16 * BLOCK + at0, rows + i * 16 * BLOCK + at1); };
-    i32x8 b[S::TT], a[2];
-    f32x4 d[LAG + 1];
-    a[0] = read(wrows, 0);
-    b[0] = read(xrows, 0);
-    b[1] = read(xrows, 1);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (uint32_t k = 0; k < S::NT * S::TT + LAG; ++k) {
-      const uint32_t i = k / S::TT, c = k % S::TT;
-      if (k < S::NT * S::TT) d[k % (LAG + 1)] = product(a[i % 2], b[c]);
-      if (k + 2 < S::TT) b[k + 2] = read(xrows, k + 2);
-      if (c == (S::TT > 2 ? S::TT - 2 : 0) && i + 1 < S::NT) a[(i + 1) % 2] = read(wrows, i + 1);
-      __builtin_amdgcn_sched_barrier(0);
-      if (k >= LAG) {
-        const uint32_t o = k - LAG;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum[o / S::TT][o % S::TT][r] = __builtin_fmaf(s[o % S::TT], d[o % (LAG + 1)][r], sum[o / S::TT][o % S::TT][r]);
-        __builtin_amdgcn_sched_barrier(0);
+        for (uint32_t i = k * ALL / STEPS; i < (k + 1) * ALL / STEPS && i < ALL; ++i) fetch(i, j + S::STAGES - 1, ahead);
       }
-    }
-  }
-  // Out through LDS, so that a row's results leave side by side: a wave's own part, rows of NT * 32 bytes, 16 bytes q of row t
-  // at place q ^ (t % 16).
-  constexpr uint32_t ROW = S::NT * 32, QS = ROW / 16;
+    });
+  };
+  uint32_t j = 0;
+  for (; j + S::STAGES - 1 < blocks; ++j) block(j, std::true_type());
+  for (; j < blocks; ++j) block(j, std::false_type());
   lds_barrier();
-  uint8_t* own = lds + wave * (S::TT * 16 * ROW);
+  uint8_t* own = lds + wave * (S::TT * 16 * S::NT * 32);
+  if (A.type == BS_FP8_BF16)
+    store_tile<S::NT, S::TT, BS_FP8_BF16>(own, sum, A, t0 + wt * S::TT * 16, n0 + wn * S::NT * 16);
+  else
+    store_tile<S::NT, S::TT, BS_FP8_F16>(own, sum, A, t0 + wt * S::TT * 16, n0 + wn * S::NT * 16);
+}
+
+// ---- streams: each wave has its own blocks
+
+// A workgroup: NT * 16 rows of the weight by TT * 16 of x. Each of its waves takes blocks in turn and brings them to LDS for itself
+// alone, STAGES deep, so waves wait for their own loads only and never for one another until their sums are joined, wave by
+// wave. (With waves that share each block, a barrier a block: 64 rows through 14,336 x 4,096 22 us, so 15.) The bound is memory, and
+// with few tiles how long a wave's loads take to come.
+template <int NT_, int TT_, int WAVES_, int STAGES_>
+struct Stream {
+  static constexpr uint32_t NT = NT_, TT = TT_, WAVES = WAVES_, STAGES = STAGES_, THREADS = WAVES * 64, N = NT * 16, T = TT * 16;
+  static constexpr uint32_t LOADS = (N + T) / 8, STAGE = (N + T) * BLOCK + 256;
+  static constexpr uint32_t LDS_BYTES = WAVES * (STAGES * STAGE > NT * TT * 1024 ? STAGES * STAGE : NT * TT * 1024);
+  static_assert(TT <= 4 && BLOCK % N == 0 && LDS_BYTES <= 160 * 1024 && (STAGES - 1) * (LOADS + 1) < 64, "");
+};
+
+// The waves' sums of a workgroup's tile, joined and stored.
+template <uint32_t NT, uint32_t TT, uint32_t WAVES>
+__device__ __forceinline__ void join_waves(uint8_t* lds, uint32_t wave, const f32x4 (&sum)[NT][TT], const Args& A, uint32_t n0, uint32_t t0) {
+  const uint32_t lane = threadIdx.x % 64;
+  f32x4* joined = (f32x4*)lds;  // [waves][NT * TT][64]
+  __syncthreads();
 #pragma unroll
-  for (uint32_t c = 0; c < S::TT; ++c)
+  for (uint32_t i = 0; i < NT; ++i)
 #pragma unroll
-    for (uint32_t i = 0; i < S::NT; ++i) {
-      const uint32_t t = c * 16 + lane % 16, u = i * 4 + lane / 16;
-      uint16_t h[4];
+    for (uint32_t c = 0; c < TT; ++c) joined[(wave * NT * TT + i * TT + c) * 64 + lane] = sum[i][c];
+  __syncthreads();
+  for (uint32_t u = wave; u < NT * TT; u += WAVES) {
+    const uint32_t n = n0 + u / TT * 16 + lane / 16 * 4, t = t0 + u % TT * 16 + lane % 16;
+    f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) h[r] = store16<TYPE>(sum[i][c][r]);
-      *(uint2*)(own + t * ROW + ((u / 2) ^ (t % QS)) * 16 + u % 2 * 8) = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-    }
-  const uint32_t tw = t0 + wt * S::TT * 16, nw = n0 + wn * S::NT * 16;
-  const bool wide = (((uintptr_t)y | (uint64_t)y_stride * 2) & 15) == 0;
-#pragma unroll 4
-  for (uint32_t k = lane; k < S::TT * 16 * QS; k += 64) {
-    const uint32_t t = k / QS, q = k % QS, n = nw + q * 8;
-    const uint4 v = *(const uint4*)(own + t * ROW + (q ^ (t % QS)) * 16);
-    if (tw + t >= X.rows) break;
-    uint16_t* row = y + (int64_t)(tw + t) * y_stride;
-    if (wide && n + 8 <= W.outer) {
-      *(uint4*)(row + n) = v;
-    } else {
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (uint32_t r = 0; r < 8; ++r)
-        if (n + r < W.outer) row[n + r] = (uint16_t)(w[r / 2] >> (r % 2 * 16));
-    }
+    for (uint32_t k = 0; k < WAVES; ++k) v += joined[(k * NT * TT + u) * 64 + lane];
+    if (t < A.x.rows && n < A.w.outer) store4(A.y + (int64_t)t * A.y_stride + n, v, A.w.outer - n, A.type);
   }
 }
 
-template <class S, int TYPE>
-int tile_launch(const bs_fp8_rows& X, const bs_fp8_weight& W, void* y, int64_t y_stride, hipStream_t s) {
+template <class S>
+__global__ __launch_bounds__(S::THREADS) void stream_kernel(Args A) {
+  BS_DYNAMIC_LDS(lds);
+  const bs_fp8_rows& X = A.x;
+  const bs_fp8_weight& W = A.w;
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  uint32_t tn, tt;
+  tile_at(blockIdx.x, A.tiles_n, A.tiles_t, tn, tt);
+  const uint32_t n0 = tn * S::N, t0 = tt * S::T, blocks = X.code_stride / BLOCK;
+  uint32_t from[S::LOADS];  // as in tile_kernel
+#pragma unroll
+  for (uint32_t i = 0; i < S::LOADS; ++i) {
+    const uint32_t r = i * 8 + lane / 8, c = ((lane % 8) ^ (lane / 8)) * 16;
+    from[i] = i * 8 < S::N ? min(r, W.outer - 1 - n0) * W.stride + c : min(r - S::N, X.rows - 1 - t0) * X.code_stride + c;
+  }
+  const auto wbase = buffer(W.codes + (uint64_t)n0 * W.stride), xbase = buffer(X.codes + (uint64_t)t0 * X.code_stride);
+  const uint32_t scale_at = min(t0 + lane % S::T, X.rows - 1) * 4;
+  uint8_t* own = lds + wave * S::STAGES * S::STAGE;
+  const auto fetch = [&](uint32_t j, uint32_t slot) {
+    uint8_t* stage = own + slot * S::STAGE;
+#pragma unroll
+    for (uint32_t i = 0; i < S::LOADS; ++i) load_lds16(i * 8 < S::N ? wbase : xbase, from[i], j * BLOCK, stage + i * 1024);
+    load_lds4(buffer(X.scales + (uint64_t)j * X.scale_stride), scale_at, 0, stage + (S::N + S::T) * BLOCK);
+  };
+  const float* ws = W.scales + (uint64_t)(n0 / BLOCK) * W.scale_stride;
+  uint32_t j = wave;
+  // the weight's scales, for 64 blocks of the wave at a time, one a lane, and those after them
+  float ws64 = ws[min(j + lane * S::WAVES, blocks - 1)], ws_next = ws[min(j + (64 + lane) * S::WAVES, blocks - 1)];
+  f32x4 sum[S::NT][S::TT] = {};
+  wait_loads<0>();
+#pragma unroll
+  for (uint32_t i = 0; i < S::STAGES; ++i)
+    if (j + i * S::WAVES < blocks) fetch(j + i * S::WAVES, i);
+  uint32_t n = 0, slot = 0;
+  const auto block = [&](auto more) {
+    // this block's loads are done, the STAGES - 1 blocks' after it may go on
+    wait_loads<more ? (S::STAGES - 1) * (S::LOADS + 1) : 0>();
+    if (n != 0 && n % 64 == 0) ws64 = ws_next, ws_next = ws[min(j + (64 + lane) * S::WAVES, blocks - 1)];
+    const float wsj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ws64), n % 64));
+    const uint8_t* stage = own + slot * S::STAGE;
+    float s[S::TT];
+#pragma unroll
+    for (uint32_t c = 0; c < S::TT; ++c) s[c] = ((const float*)(stage + (S::N + S::T) * BLOCK))[c * 16 + lane % 16] * wsj;
+    multiply<S::NT, S::TT>(stage, stage + S::N * BLOCK, s, sum, [](uint32_t) {});
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of the block has been read)
+    if constexpr (more) fetch(j + S::STAGES * S::WAVES, slot);
+    slot = slot + 1 == S::STAGES ? 0 : slot + 1;
+    j += S::WAVES, ++n;
+  };
+  while (j + S::STAGES * S::WAVES < blocks) block(std::true_type());
+  while (j < blocks) block(std::false_type());
+  join_waves<S::NT, S::TT, S::WAVES>(lds, wave, sum, A, n0, t0);
+}
+
+// ---- single rows, quantised on the way
+
+// A workgroup: 16 rows of the weight by up to 16 rows of x, which it quantises into LDS for itself while the weight's first blocks come:
+// one launch instead of two. Its eight waves take blocks in turn, DEPTH ahead in registers.
+constexpr uint32_t V_WAVES = 8, V_THREADS = V_WAVES * 64, V_DEPTH = 4;
+
+template <int TYPE>
+__global__ __launch_bounds__(V_THREADS) void values_kernel(Args A, const uint16_t* x, int64_t x_stride) {
+  BS_DYNAMIC_LDS(lds);
+  const bs_fp8_weight& W = A.w;
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), r = lane % 16, g = lane / 16;
+  const uint32_t n0 = blockIdx.x * 16, blocks = A.x.code_stride / BLOCK, t = min(r, A.x.rows - 1);
+  // Within a block a lane holds columns 16 g .. and 64 + 16 g .. of its row, of both operands: a load reads 64 bytes on end of each row.
+  const uint8_t* wp = W.codes + (uint64_t)min(n0 + r, W.outer - 1) * W.stride + g * 16;
+  const float* ws = W.scales + (uint64_t)(n0 / BLOCK) * W.scale_stride;
+  float* scales = (float*)(lds + A.x.rows * blocks * BLOCK);  // [rows][blocks]
+  i32x8 a[V_DEPTH];
+  float wsd[V_DEPTH];
+  const auto load = [&](int d, uint32_t j) {
+    j = min(j, blocks - 1);  // past the end the last block is read again, and not summed
+    a[d] = load_operand(wp + (uint64_t)j * BLOCK, wp + (uint64_t)j * BLOCK + 64);
+    wsd[d] = ws[j];
+  };
+  f32x4 sum[1][1] = {};
+  const auto add = [&](int d, uint32_t j) {
+    const uint32_t at = t * blocks + min(j, blocks - 1);
+    const uint8_t* row = lds + at * BLOCK;
+    const f32x4 p = product(a[d], load_operand(row + ((g ^ t) % 8) * 16, row + (((4 + g) ^ t) % 8) * 16));
+    const float s = j < blocks ? scales[at] * wsd[d] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum[0][0][e] = __builtin_fmaf(s, p[e], sum[0][0][e]);
+  };
+  uint32_t j = wave;
+  if (j < blocks) {
+#pragma unroll
+    for (uint32_t d = 0; d < V_DEPTH; ++d) load(d, j + d * V_WAVES);
+  }
+  const bool wide = (((uintptr_t)x | (uint64_t)x_stride * 2) & 15) == 0;
+  for (uint32_t u = threadIdx.x / 16; u < A.x.rows * blocks; u += V_THREADS / 16) {
+    const uint32_t row = u / blocks, k = u % blocks * BLOCK + lane % 16 * 8;
+    const uint16_t* p = x + (int64_t)row * x_stride;
+    const Eight v = wide ? load_eight<true>(p, k, A.x.cols) : load_eight<false>(p, k, A.x.cols);
+    float scale;
+    // 16 bytes c of a row's block lie at c ^ (row % 8): rows read at once lie in different banks
+    *(uint2*)(lds + u * BLOCK + ((lane % 16 / 2) ^ (row % 8)) * 16 + lane % 2 * 8) = quantise_block<TYPE>(v, scale);
+    if (lane % 16 == 0) scales[u] = scale;
+  }
+  __syncthreads();
+  if (j < blocks) {
+    for (; j + V_DEPTH * V_WAVES < blocks; j += V_DEPTH * V_WAVES) {
+#pragma unroll
+      for (uint32_t d = 0; d < V_DEPTH; ++d) {
+        add(d, j + d * V_WAVES);
+        load(d, j + (V_DEPTH + d) * V_WAVES);
+      }
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < V_DEPTH; ++d) add(d, j + d * V_WAVES);
+  }
+  join_waves<1, 1, V_WAVES>(lds, wave, sum, A, n0, 0);
+}
+
+// Up to this many blocks of x. One row through 4,096 x 4,096: 7.4 us, quantised by a kernel of its own 10.5; four (128
+// blocks) 9.6 and 10.5, eight 13.0 and 11.0; one row of 14,336 columns 15.7 and 16.
+constexpr uint32_t V_BLOCKS = 128;
+
+template <int TYPE>
+int values_launch(const Args& A, const void* x, int64_t x_stride, hipStream_t s) {
+  const uint32_t lds = std::max<uint32_t>(V_WAVES * 1024, A.x.rows * (A.x.code_stride / BLOCK) * (BLOCK + 4));
+  values_kernel<TYPE><<<(A.w.outer + 15) / 16, V_THREADS, lds, s>>>(A, (const uint16_t*)x, x_stride);
+  return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
+}
+static_assert(V_BLOCKS * (BLOCK + 4) <= 64 * 1024, "");
+
+// ---- which kernel
+
+template <class S>
+int tile_go(Args A, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  const uint32_t tiles_n = (W.outer + S::N - 1) / S::N, tiles_t = (X.rows + S::T - 1) / S::T;
-  bs_internal::ensure_lds_limit((const void*)tile_kernel<S, TYPE>, 2 * S::STAGE, done);
-  tile_kernel<S, TYPE><<<tiles_n * tiles_t, S::THREADS, 2 * S::STAGE, s>>>(X, W, (uint16_t*)y, y_stride, tiles_n, tiles_t);
+  A.tiles_n = (A.w.outer + S::N - 1) / S::N, A.tiles_t = (A.x.rows + S::T - 1) / S::T;
+  bs_internal::ensure_lds_limit((const void*)tile_kernel<S>, S::LDS_BYTES, done);
+  tile_kernel<S><<<A.tiles_n * A.tiles_t, S::THREADS, S::LDS_BYTES, s>>>(A);
   return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
 }
 
-template <int TYPE>
-int linear_launch(const bs_fp8_rows& X, const bs_fp8_weight& W, void* y, int64_t y_stride, hipStream_t s) {
-  // 256 by 256 reads each operand least often (8,192 rows through 14,336 x 4,096: 445 us, by 128 587) but wants a tile for
-  // each compute unit at least (777 through 1,000 x 1,400: 22.6 us, by 128 13.8).
-  if ((uint64_t)((W.outer + 255) / 256) * ((X.rows + 255) / 256) >= bs_internal::device_cus())
-    return tile_launch<Tile<2, 4, 8, 4>, TYPE>(X, W, y, y_stride, s);
-  return tile_launch<Tile<2, 2, 4, 4>, TYPE>(X, W, y, y_stride, s);
+template <class S>
+int stream_go(Args A, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  A.tiles_n = (A.w.outer + S::N - 1) / S::N, A.tiles_t = (A.x.rows + S::T - 1) / S::T;
+  bs_internal::ensure_lds_limit((const void*)stream_kernel<S>, S::LDS_BYTES, done);
+  stream_kernel<S><<<A.tiles_n * A.tiles_t, S::THREADS, S::LDS_BYTES, s>>>(A);
+  return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
+}
+
+// The shapes, and what they take, in us as measured: `fixed`, for each workgroup of a compute unit `start`, and `one` for each block
+// that it (a wave of a stream) goes through; start2 and two are for a pair of workgroups, side by side where LDS holds two. The smallest
+// estimate is taken. Over 1 to 4,096 rows through 512 x 14,336, 1,024 x 4,096, 2,048 x 1,024, 4,096 x 4,096, 4,096 x 14,336, 14,336 x 512 and
+// 14,336 x 4,096 that is at most a tenth slower than the fastest of them, mostly as fast.
+struct Shape {
+  uint32_t n, t, waves;
+  float fixed, start, one, start2, two;
+  int (*go)(Args, hipStream_t);
+};
+const Shape SHAPES[] = {
+    {32, 16, 8, 3.0f, 0.5f, 0.70f, 1.0f, 2.20f, stream_go<Stream<2, 1, 8, 2>>},  {64, 16, 4, 2.6f, 0.8f, 0.55f, 1.8f, 1.40f, stream_go<Stream<4, 1, 4, 3>>},
+    {32, 32, 8, 2.6f, 0.9f, 0.85f, 1.9f, 1.80f, stream_go<Stream<2, 2, 8, 2>>},  {64, 32, 4, 2.5f, 1.3f, 0.56f, 2.6f, 1.35f, stream_go<Stream<4, 2, 4, 3>>},
+    {64, 64, 4, 2.6f, 1.6f, 0.85f, 3.4f, 2.00f, stream_go<Stream<4, 4, 4, 2>>},  {64, 64, 1, 2.6f, 1.2f, 0.29f, 1.9f, 0.43f, tile_go<Tile<2, 2, 2, 2, 4>>},
+    {128, 128, 1, 2.3f, 3.2f, 0.55f, 6.4f, 1.10f, tile_go<Tile<2, 2, 4, 4, 4>>}, {128, 128, 1, 4.0f, 1.6f, 0.68f, 3.0f, 0.99f, tile_go<Tile<2, 2, 4, 4, 2>>},
+    {256, 256, 1, 2.6f, 4.6f, 1.45f, 9.2f, 3.30f, tile_go<Tile<2, 4, 8, 4, 2>>},
+};
+
+int linear(const Args& A, hipStream_t s) {
+  const uint32_t blocks = A.x.code_stride / BLOCK;
+  const uint64_t cus = std::min(bs_internal::device_cus(), 256u);
+  const Shape* best = nullptr;
+  float least = 0;
+  for (const Shape& c : SHAPES) {
+    const uint64_t tiles = (uint64_t)((A.w.outer + c.n - 1) / c.n) * ((A.x.rows + c.t - 1) / c.t);
+    if (tiles > 0x7FFFFFFFu) continue;
+    const uint64_t each = (tiles + cus - 1) / cus;  // workgroups of a compute unit
+    const float turns = (float)((blocks + c.waves - 1) / c.waves);
+    const float us = c.fixed + (float)(each / 2) * (c.start2 + turns * c.two) + (float)(each % 2) * (c.start + turns * c.one);
+    if (!best || us < least) best = &c, least = us;
+  }
+  return best->go(A, s);
 }
 
 bool aligned(const void* p) { return p && ((uintptr_t)p & 15) == 0; }
 
-// A grid has at most 65,535 workgroups in its second dimension, 16 rows each; offsets within 256 rows stay below 2^32.
+// Offsets within 256 rows stay below 2^32, a result's tiles below 2^31.
 constexpr uint32_t MOST_ROWS = 65535 * 16, MOST_COLS = 1u << 22, MOST_STRIDE = 1u << 23;
 
 bool rows_ok(const bs_fp8_rows* r) {
@@ -312,9 +613,14 @@ bool rows_ok(const bs_fp8_rows* r) {
 
 bool weight_ok(const bs_fp8_weight* w) {
   return w && w->outer > 0 && w->outer <= MOST_COLS && w->inner > 0 && w->inner <= MOST_COLS && w->stride % BLOCK == 0 &&
-         w->stride >= w->inner && w->stride <= MOST_STRIDE && w->scale_stride >= (w->inner + BLOCK - 1) / BLOCK && aligned(w->codes) && w->scales &&
-         ((uintptr_t)w->scales & 3) == 0;
+         w->stride >= w->inner && w->stride <= MOST_STRIDE && w->scale_stride >= (w->inner + BLOCK - 1) / BLOCK && aligned(w->codes) &&
+         w->scales && ((uintptr_t)w->scales & 3) == 0;
 }
+
+bool few_values(uint32_t rows, const bs_fp8_weight& w) { return rows <= 16 && rows * ((w.inner + BLOCK - 1) / BLOCK) <= V_BLOCKS; }
+
+// Codes and scales of values in the work area, scales first.
+uint64_t scale_bytes(uint32_t rows, const bs_fp8_weight& w) { return ((uint64_t)rows * ((w.inner + BLOCK - 1) / BLOCK) * 4 + 15) / 16 * 16; }
 
 }  // namespace
 
@@ -322,22 +628,35 @@ extern "C" int bs_fp8_quantise(const void* x, uint32_t type, int64_t x_stride, c
   if (!rows_ok(out) || type > BS_FP8_F16 || x_stride < 0) return BS_ERR_ARG;
   if (out->rows == 0) return BS_OK;
   if (!x || ((uintptr_t)x & 1)) return BS_ERR_ARG;
-  return type == BS_FP8_BF16 ? quantise_launch<BS_FP8_BF16>(x, x_stride, *out, (hipStream_t)stream)
-                             : quantise_launch<BS_FP8_F16>(x, x_stride, *out, (hipStream_t)stream);
+  return quantise(x, type, x_stride, *out, (hipStream_t)stream);
 }
 
-extern "C" uint64_t bs_fp8_linear_work_bytes(const bs_fp8_rows* x, const bs_fp8_weight* w) {
-  (void)x, (void)w;
-  return 0;
-}
-
-extern "C" int bs_fp8_linear(const bs_fp8_rows* x, const bs_fp8_weight* w, void* y, uint32_t type, int64_t y_stride, void* d_work,
-                             uint64_t work_bytes, void* stream) {
+extern "C" int bs_fp8_linear(const bs_fp8_rows* x, const bs_fp8_weight* w, void* y, uint32_t type, int64_t y_stride, void* stream) {
   if (!rows_ok(x) || !weight_ok(w) || type > BS_FP8_F16 || x->cols != w->inner || y_stride < (int64_t)w->outer) return BS_ERR_ARG;
   if (x->rows == 0) return BS_OK;
   if (!y || ((uintptr_t)y & 1)) return BS_ERR_ARG;
-  const uint64_t need = bs_fp8_linear_work_bytes(x, w);
+  return linear(Args{*x, *w, (uint16_t*)y, y_stride, type, 0, 0}, (hipStream_t)stream);
+}
+
+extern "C" uint64_t bs_fp8_linear_values_work_bytes(uint32_t rows, const bs_fp8_weight* w) {
+  if (!weight_ok(w) || rows > MOST_ROWS || few_values(rows, *w)) return 0;
+  return scale_bytes(rows, *w) + (uint64_t)rows * ((w->inner + BLOCK - 1) / BLOCK) * BLOCK;
+}
+
+extern "C" int bs_fp8_linear_values(const void* x, uint32_t x_type, int64_t x_stride, uint32_t rows, const bs_fp8_weight* w, void* y, uint32_t type,
+                                    int64_t y_stride, void* d_work, uint64_t work_bytes, void* stream) {
+  if (!weight_ok(w) || x_type > BS_FP8_F16 || type > BS_FP8_F16 || rows > MOST_ROWS || x_stride < 0 || y_stride < (int64_t)w->outer) return BS_ERR_ARG;
+  if (rows == 0) return BS_OK;
+  if (!x || !y || (((uintptr_t)x | (uintptr_t)y) & 1)) return BS_ERR_ARG;
+  const uint64_t need = bs_fp8_linear_values_work_bytes(rows, w);
   if (work_bytes < need || (need && !aligned(d_work))) return BS_ERR_CAP;
-  return type == BS_FP8_BF16 ? linear_launch<BS_FP8_BF16>(*x, *w, y, y_stride, (hipStream_t)stream)
-                             : linear_launch<BS_FP8_F16>(*x, *w, y, y_stride, (hipStream_t)stream);
+  const uint32_t wide = (w->inner + BLOCK - 1) / BLOCK * BLOCK;
+  hipStream_t s = (hipStream_t)stream;
+  Args A = {{(uint8_t*)d_work + scale_bytes(rows, *w), (float*)d_work, rows, w->inner, wide, rows}, *w, (uint16_t*)y, y_stride, type, 0, 0};
+  if (few_values(rows, *w)) {
+    A.x.codes = nullptr, A.x.scales = nullptr;
+    return x_type == BS_FP8_BF16 ? values_launch<BS_FP8_BF16>(A, x, x_stride, s) : values_launch<BS_FP8_F16>(A, x, x_stride, s);
+  }
+  const int rc = quantise(x, x_type, x_stride, A.x, s);
+  return rc != BS_OK ? rc : linear(A, s);
 }

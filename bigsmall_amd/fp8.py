@@ -99,6 +99,17 @@ class Fp8Rows:
         self.index, self.ref = codes.get_device(), ctypes.byref(c)
 
 
+def _matrix(x):
+    """x as rows whose columns are contiguous, their number and the columns'."""
+    k = x.shape[-1]
+    y = x if x.dim() == 2 else x.reshape(-1, k)
+    if y.stride(1) != 1 and k > 1:
+        y = y.contiguous()
+    if y.shape[0] > _MOST_ROWS:
+        raise ValueError(f"{y.shape[0]} rows: at most {_MOST_ROWS} at once")
+    return y, y.shape[0], k
+
+
 def fp8_quantise(x) -> Fp8Rows:
     """x [..., inner], bf16 or f16, in e4m3 with a scale for each 128 columns of a row: a = max |x| of the block
     (held to at least 2^-100), scale = a / 448, code = 448 x / a to nearest even, the exact quotient rounded once. A block
@@ -111,13 +122,8 @@ def fp8_quantise(x) -> Fp8Rows:
     _gpu(index, x)
     if x.requires_grad and _recording():
         _refuse_grad()
-    shape, k = x.shape[:-1], x.shape[-1]
-    y = x.reshape(-1, k)
-    if k > 1 and y.stride(1) != 1:
-        y = y.contiguous()
-    t = y.shape[0]
-    if t > _MOST_ROWS:
-        raise ValueError(f"{t} rows: at most {_MOST_ROWS} at once")
+    shape = x.shape[:-1]
+    y, t, k = _matrix(x)
     wide = _blocks(k) * BLOCK
     codes = torch.empty((t, wide), dtype=torch.float8_e4m3fn, device=x.device)
     scales = torch.empty((wide // BLOCK, t), dtype=torch.float32, device=x.device)
@@ -133,31 +139,38 @@ def fp8_linear(x, weight: Fp8Weight, dtype=None):
     fp8_quantise does, or what fp8_quantise returned. dtype: the result's, bf16 or f16; x's by default."""
     if not isinstance(weight, Fp8Weight):
         raise ValueError("weight must be an Fp8Weight")
+    index = weight.index
     if isinstance(x, Fp8Rows):
-        rows = x
-        if rows.c.cols != weight.inner:
-            raise ValueError(f"x has {rows.c.cols} columns, the weight {weight.inner}")
-        if rows.index != weight.index:
-            raise ValueError(f"x is on {rows.codes.device}, the weight on {weight.device}")
+        t, k, shape, rows = x.c.rows, x.c.cols, x.shape, x
+        if k != weight.inner:
+            raise ValueError(f"x has {k} columns, the weight {weight.inner}")
+        if x.index != index:
+            raise ValueError(f"x is on {x.codes.device}, the weight on {weight.device}")
     else:
         if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES:
             raise ValueError(f"x must be a bfloat16 or float16 tensor or Fp8Rows, got {getattr(x, 'dtype', type(x).__name__)}")
         if x.dim() < 1 or x.shape[-1] != weight.inner:
             raise ValueError(f"x has shape {tuple(x.shape)}, the weight has {weight.inner} columns")
-        if x.get_device() != weight.index:
+        if x.get_device() != index:
             raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-        rows = fp8_quantise(x)
-    dtype = rows.dtype if dtype is None else dtype
+        if x.requires_grad and _recording():
+            _refuse_grad()
+        shape, rows = x.shape[:-1], None
+        values, t, _ = _matrix(x)
+    dtype = x.dtype if dtype is None else dtype
     if dtype not in _TYPES:
         raise ValueError(f"the result is bfloat16 or float16, not {dtype}")
-    _gpu(weight.index, weight)
-    y = torch.empty((rows.c.rows, weight.outer), dtype=dtype, device=weight.device)
-    if rows.c.rows:
-        n = _native.lib().bs_fp8_linear_work_bytes(rows.ref, weight.ref)
-        work = torch.empty(n, dtype=torch.uint8, device=weight.device) if n else None
-        _call("bs_fp8_linear", weight.index, rows.ref, weight.ref, y.data_ptr(), _TYPES[dtype], weight.outer,
-              work.data_ptr() if n else 0, n)
-    return y.view(*rows.shape, weight.outer)
+    _gpu(index, weight)
+    y = torch.empty((*shape, weight.outer), dtype=dtype, device=weight.device)
+    if t:
+        if rows is not None:
+            _call("bs_fp8_linear", index, rows.ref, weight.ref, y.data_ptr(), _TYPES[dtype], weight.outer)
+        else:
+            n = _native.lib().bs_fp8_linear_values_work_bytes(t, weight.ref)
+            work = torch.empty(n, dtype=torch.uint8, device=weight.device) if n else None
+            _call("bs_fp8_linear_values", index, values.data_ptr(), _TYPES[x.dtype], values.stride(0), t, weight.ref, y.data_ptr(),
+                  _TYPES[dtype], weight.outer, work.data_ptr() if n else 0, n)
+    return y
 
 
 __all__ = ["BLOCK", "Fp8Weight", "Fp8Rows", "fp8_quantise", "fp8_linear"]

@@ -52,10 +52,14 @@ typedef struct {
 /* y[t][n] = sum over blocks j of x.scale[t][j] * w.scale[n / 128][j] * (codes of x . codes of w in j),
  * eight neighbouring products at a time cut off 13 bits below the largest one's first bit (as the matrix unit
  * adds them), all else in f32, rounded once to y's type. y: rows of `outer` values, y_stride
- * elements apart. d_work: bs_fp8_linear_work_bytes bytes of scratch, 16-byte aligned (0 may be NULL). */
-uint64_t bs_fp8_linear_work_bytes(const bs_fp8_rows *x, const bs_fp8_weight *w);
-int bs_fp8_linear(const bs_fp8_rows *x, const bs_fp8_weight *w, void *y, uint32_t type, int64_t y_stride, void *d_work,
-                  uint64_t work_bytes, void *stream);
+ * elements apart. */
+int bs_fp8_linear(const bs_fp8_rows *x, const bs_fp8_weight *w, void *y, uint32_t type, int64_t y_stride, void *stream);
+
+/* The same for rows of bf16 or f16 values, quantised on the way as bs_fp8_quantise does. d_work:
+ * bs_fp8_linear_values_work_bytes bytes of scratch, 16-byte aligned (0 bytes may be NULL). */
+uint64_t bs_fp8_linear_values_work_bytes(uint32_t rows, const bs_fp8_weight *w);
+int bs_fp8_linear_values(const void *x, uint32_t x_type, int64_t x_stride, uint32_t rows, const bs_fp8_weight *w, void *y,
+                         uint32_t type, int64_t y_stride, void *d_work, uint64_t work_bytes, void *stream);
 
 #ifdef __cplusplus
 }

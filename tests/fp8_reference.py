@@ -44,9 +44,12 @@ def linear(codes, scales, w, ws, dtype):
     x = torch.nn.functional.pad(codes * spread(scales, k, 1), (0, pad))
     y = torch.nn.functional.pad(w.float().double() * spread(spread(ws, n, 0), k, 1), (0, pad))
     out, size = x @ y.T, x.abs() @ y.abs().T
-    tops = torch.zeros_like(out)
-    for g in range(0, k + pad, 8):
-        tops += (x[:, None, g:g + 8] * y[None, :, g:g + 8]).abs().amax(2)
+    if out.numel() * k < 1 << 27:
+        tops = torch.zeros_like(out)
+        for g in range(0, k + pad, 8):
+            tops += (x[:, None, g:g + 8] * y[None, :, g:g + 8]).abs().amax(2)
+    else:                         # a group's largest product is no larger than the sum of their absolute values
+        tops = size
     tol = size * (18 + scales.shape[1]) * 2.0 ** -23 + tops * 7 * 2.0 ** -13
     info = torch.finfo(dtype)
     return out, tol + (out.abs() + tol) * (info.eps / 2) + info.smallest_normal * info.eps / 2

@@ -145,12 +145,22 @@ def test_c_entries_refuse_bad_arguments():
                                (rows(), at, 0, -1), (rows(rows=1 << 30, scale_stride=1 << 30), at, 0, 200)):
         assert L.bs_fp8_quantise(x, kind, stride, p(r), None) == ARG
     assert L.bs_fp8_quantise(at, 0, 200, None, None) == ARG
-    assert L.bs_fp8_linear(p(rows(rows=0)), p(weight()), at, 0, 8, None, 0, None) == 0
+    assert L.bs_fp8_linear(p(rows(rows=0)), p(weight()), at, 0, 8, None) == 0
     for r, w, y, kind, stride in ((rows(cols=201), weight(), at, 0, 8), (rows(), weight(stride=200), at, 0, 8), (rows(), weight(stride=128), at, 0, 8),
                                   (rows(), weight(codes=at + 4), at, 0, 8), (rows(), weight(scale_stride=1), at, 0, 8), (rows(), weight(outer=0), at, 0, 8),
                                   (rows(), weight(scales=0), at, 0, 8), (rows(), weight(), 0, 0, 8), (rows(), weight(), at, 0, 7), (rows(), weight(), at, 3, 8),
                                   (rows(), weight(), at + 1, 0, 8)):
-        assert L.bs_fp8_linear(p(r), p(w), y, kind, stride, at, 1 << 40, None) == ARG
+        assert L.bs_fp8_linear(p(r), p(w), y, kind, stride, None) == ARG
+    assert L.bs_fp8_linear_values(at, 0, 200, 0, p(weight()), at, 0, 8, None, 0, None) == 0
+    for x, xk, xs, n, w, y, kind, stride in ((0, 0, 200, 2, weight(), at, 0, 8), (at + 1, 0, 200, 2, weight(), at, 0, 8), (at, 2, 200, 2, weight(), at, 0, 8),
+                                             (at, 0, -1, 2, weight(), at, 0, 8), (at, 0, 200, 1 << 21, weight(), at, 0, 8), (at, 0, 200, 2, weight(inner=0), at, 0, 8),
+                                             (at, 0, 200, 2, weight(), 0, 0, 8), (at, 0, 200, 2, weight(), at, 2, 8), (at, 0, 200, 2, weight(), at, 0, 7)):
+        assert L.bs_fp8_linear_values(x, xk, xs, n, p(w), y, kind, stride, at, 1 << 40, None) == ARG
+    big = weight(outer=4096, inner=100, stride=128, scale_stride=1)
+    need = L.bs_fp8_linear_values_work_bytes(500, p(big))
+    assert need >= 500 * 132 and L.bs_fp8_linear_values_work_bytes(1, p(big)) == 0
+    assert L.bs_fp8_linear_values(at, 0, 100, 500, p(big), at, 0, 4096, at, need - 1, None) == CAP
+    assert L.bs_fp8_linear_values(at, 0, 100, 500, p(big), at, 0, 4096, at + 8, need, None) == CAP
 
     def batch(**c):
         f = dict(p=at, q=at, draft=at, accept=at, cu=at, pick=at, tokens=at, counts=at, p_stride=10, q_stride=10, type=0, n_rows=3, vocab=10, n_seqs=1,

@@ -83,9 +83,9 @@ def test_quantise_extremes(dtype):
     _same_rows(bs.fp8_quantise(x.cuda()), x)
 
 
-def _check(y, rows, w, ws, dtype):
-    want, tol = ref.linear(rows.codes.cpu().float().double(), rows.scales.cpu().double(), w, ws, dtype)
-    off = (y.cpu().double() - want).abs()
+def _check(y, rows, w, ws, dtype, device="cpu"):
+    want, tol = ref.linear(rows.codes.to(device).float().double(), rows.scales.to(device).double(), w.to(device), ws.to(device), dtype)
+    off = (y.to(device).double() - want).abs()
     worst = float((off / tol).max())
     assert worst <= 1, worst
 
@@ -111,6 +111,27 @@ def test_linear(t, n, k):
     z = bs.fp8_linear(rows, weight, dtype=other)              # quantised once, the other type out
     assert z.dtype == other
     _check(z, rows, w, ws, other)
+    assert t <= 16 or torch.equal(bs.fp8_linear(rows, weight), y)      # (few rows: another kernel, other sums)
+
+
+# Sizes for each way in which a product is cut up (tiles of 32 by 16 to 256 by 256, one to several turns), odd and even numbers of
+# blocks, and more than 64 blocks to a wave, whose scales come 64 at a time.
+LARGE = [(61, 4090, 4000), (64, 4097, 3000), (50, 8000, 1000), (64, 14000, 700), (250, 7001, 800), (129, 4097, 900), (500, 4100, 700), (900, 4000, 9000),
+         (1100, 3500, 1500), (1500, 4000, 256), (1300, 4500, 1000), (300, 14001, 400), (2300, 5000, 520), (3000, 4100, 200), (2100, 4609, 130),
+         (2050, 4999, 9000), (1300, 9000, 8500), (250, 7001, 8500), (2, 33, 70000), (5, 70, 40000), (20, 2000, 40000), (16, 14336, 33000), (300, 500, 34000)]
+
+
+@pytest.mark.parametrize("t,n,k", LARGE)
+def test_linear_large(t, n, k):
+    import bigsmall_amd as bs
+    g = _gen(t + n + k)
+    dtype = TYPES[(t + k) % 2]
+    x = _x(t, k, dtype, g).cuda()
+    w, ws = _w(n, k, g)
+    weight = bs.Fp8Weight(w.cuda(), ws.cuda())
+    y = bs.fp8_linear(x, weight)
+    rows = bs.fp8_quantise(x)
+    _check(y, rows, w, ws, dtype, "cuda")
     assert torch.equal(bs.fp8_linear(rows, weight), y)
 
 
