@@ -1,11 +1,12 @@
 // Verification of drafted tokens against the target's probabilities.
 //
-// parts_kernel: a workgroup per part of a sequence's vocabulary. Each finds the row at which the drafts end (a test a
-// lane; three dependent reads) and sums that row's weights over its part. pick_kernel: a workgroup per sequence finds
-// the part, the thread and the token at which the running sum passes the given share. Only that one row of p (and of
-// q where a draft was refused) is read. Sums are f64: with f32 the token drawn would hang on their order wherever the
-// share falls near a border, and a vocabulary has 100,000 of them. They are made in an order that depends on the
-// sizes alone, so the same numbers give the same tokens.
+// A sequence's vocabulary is cut into pieces, at most 256 and of 1,024 weights or a multiple. sums_kernel: each workgroup finds the row
+// at which the drafts end (a test a lane; three dependent reads), and each of its waves sums that row's weights over pieces
+// of its own. pick_kernel: a workgroup per sequence finds the piece, then the token at which the running sum passes the given
+// share; it is one wave, so nothing waits at a barrier. A small vocabulary is one workgroup's and one launch. Only that one row of p (and of q where a draft was refused)
+// is read, and one piece of it twice. Sums are f64: with f32 the token drawn would hang on their order wherever the share
+// falls near a border, and a vocabulary has 100,000 of them. They are made in an order that depends on the sizes alone, so
+// the same numbers give the same tokens.
 #include <float.h>
 
 #include <algorithm>
@@ -16,37 +17,71 @@
 namespace {
 
 constexpr uint32_t THREADS = 256, WAVES = THREADS / 64;
-constexpr uint32_t MOST_PARTS = THREADS, PART_MIN = 4096;
+constexpr uint32_t MOST_PIECES = THREADS, PIECE = 1024;
+constexpr uint32_t ALONE = 8;  // pieces that one workgroup sums and picks from in one launch
 
 struct Work {
-  double* sums;   // [n_seqs][parts]
-  int32_t* taken; // [n_seqs] drafts taken, -1: no rows
-  uint32_t parts, len;  // elements of a part
+  double* sums;          // [n_seqs][pieces]
+  int32_t* taken;        // [n_seqs] drafts taken, -1: no rows
+  uint32_t pieces, len;  // of a sequence; weights of a piece
+  uint32_t groups;       // workgroups of a sequence
 };
+
+template <int TYPE>
+__device__ __forceinline__ float of16(uint32_t bits) {
+  if constexpr (TYPE == BS_DRAFT_BF16) return __uint_as_float(bits << 16);
+  return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+}
 
 template <int TYPE>
 __device__ __forceinline__ float value(const void* p, uint64_t i) {
   if constexpr (TYPE == BS_DRAFT_F32) return ((const float*)p)[i];
-  if constexpr (TYPE == BS_DRAFT_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
-  if constexpr (TYPE == BS_DRAFT_F16) return (float)((const _Float16*)p)[i];
+  return of16<TYPE>(((const uint16_t*)p)[i]);
 }
 
+template <int TYPE>
+__device__ __forceinline__ void values4(const void* p, uint64_t i, float (&v)[4]) {
+  if constexpr (TYPE == BS_DRAFT_F32) {
+    *(float4*)v = *(const float4*)((const float*)p + i);
+  } else {
+    const uint2 u = *(const uint2*)((const uint16_t*)p + i);
+    v[0] = of16<TYPE>(u.x & 0xFFFFu), v[1] = of16<TYPE>(u.x >> 16), v[2] = of16<TYPE>(u.y & 0xFFFFu), v[3] = of16<TYPE>(u.y >> 16);
+  }
+}
+
+// (a difference with a NaN in it is not above 0; p = inf less q = inf is one)
 __device__ __forceinline__ double weight(double d) { return d > 0 ? (d < (double)FLT_MAX ? d : (double)FLT_MAX) : 0.0; }
 
-// The weights of a sequence's last row, w(j).
+// The weights of a sequence's last row.
 template <int TYPE>
 struct Row {
-  const bs_draft_batch& D;
-  uint64_t p, q;   // where the row begins
-  int64_t without; // the token left out, -1: none
-  bool minus;      // q is taken off
-  __device__ Row(const bs_draft_batch& batch, uint64_t row, bool refused)
-      : D(batch), p(row * (uint64_t)batch.p_stride), q(row * (uint64_t)batch.q_stride),
-        without(refused && !batch.q ? batch.draft[row] : -1), minus(refused && batch.q) {}
-  __device__ __forceinline__ double operator()(uint32_t j) const {
-    double d = (double)value<TYPE>(D.p, p + j);
-    if (minus) d -= (double)value<TYPE>(D.q, q + j);
-    return (int64_t)j == without ? 0.0 : weight(d);
+  const void *p, *q;  // the row; q NULL: not taken off
+  uint32_t vocab;
+  int64_t without;    // the token left out, -1: none
+  bool wide;          // four weights can be read at once
+  __device__ Row(const bs_draft_batch& D, uint64_t row, bool refused) : vocab(D.vocab), without(refused && !D.q ? D.draft[row] : -1) {
+    const uint32_t size = TYPE == BS_DRAFT_F32 ? 4 : 2;
+    p = (const uint8_t*)D.p + row * (uint64_t)D.p_stride * size;
+    q = refused && D.q ? (const uint8_t*)D.q + row * (uint64_t)D.q_stride * size : nullptr;
+    wide = (((uintptr_t)p | (uintptr_t)q) & (4 * size - 1)) == 0;
+  }
+  __device__ __forceinline__ double of(uint32_t j, float a, float b) const { return (int64_t)j == without ? 0.0 : weight((double)a - (double)b); }
+  // w(j) .. w(j + 3), 0 past the end
+  __device__ __forceinline__ void four(uint32_t j, double (&w)[4]) const {
+    float a[4] = {}, b[4] = {};
+    if (wide && j + 4 <= vocab) {
+      values4<TYPE>(p, j, a);
+      if (q) values4<TYPE>(q, j, b);
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e)
+        if (j + e < vocab) {
+          a[e] = value<TYPE>(p, j + e);
+          if (q) b[e] = value<TYPE>(q, j + e);
+        }
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) w[e] = of(j + e, a[e], b[e]);
   }
 };
 
@@ -85,132 +120,175 @@ __device__ __forceinline__ double wave_sum(double x) {
   return x;
 }
 
-// Sum of the threads' x up to and including one's own.
-__device__ double block_scan(double x, double* lds) {
+// The sum of a piece, by one wave: every lane has it.
+template <int TYPE>
+__device__ __forceinline__ double piece_sum(const Row<TYPE>& w, uint32_t piece, uint32_t len) {
+  const uint32_t lane = threadIdx.x % 64, lo = piece * len, hi = min(w.vocab, lo + len);
+  double sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (uint32_t j = lo + lane * 4; j < hi; j += 256) {
+    double x[4];
+    w.four(j, x);
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double up = __shfl_up(x, d);
-    if (threadIdx.x % 64 >= (uint32_t)d) x += up;
+    for (int e = 0; e < 4; ++e) sum[e] += x[e];
   }
-  __syncthreads();
-  if (threadIdx.x % 64 == 63) lds[threadIdx.x / 64] = x;
-  __syncthreads();
-  for (uint32_t w = 0; w < threadIdx.x / 64; ++w) x += lds[w];
-  return x;
+  return wave_sum((sum[0] + sum[1]) + (sum[2] + sum[3]));
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(THREADS) void parts_kernel(bs_draft_batch D, Work W, int32_t* status) {
-  __shared__ double sums[WAVES];
-  const uint32_t b = blockIdx.x / W.parts, part = blockIdx.x % W.parts;
-  const int32_t a = taken_drafts<TYPE>(D, b, part == 0 ? status : nullptr);
-  if (part == 0 && threadIdx.x == 0) W.taken[b] = a;
+__global__ __launch_bounds__(THREADS) void sums_kernel(bs_draft_batch D, Work W, int32_t* status) {
+  const uint32_t b = blockIdx.x / W.groups, group = blockIdx.x % W.groups;
+  const int32_t a = taken_drafts<TYPE>(D, b, group == 0 ? status : nullptr);
+  if (group == 0 && threadIdx.x == 0) W.taken[b] = a;
   if (a < 0) return;
   const int32_t row = D.cu[b] + a;
   const Row<TYPE> w(D, (uint64_t)row, row + 1 < D.cu[b + 1]);
-  const uint32_t end = min(D.vocab, (part + 1) * W.len);
-  double sum = 0;
-  for (uint32_t j = part * W.len + threadIdx.x; j < end; j += THREADS) sum += w(j);
-  sum = wave_sum(sum);
-  if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) W.sums[(uint64_t)b * W.parts + part] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-}
-
-// The first token in [lo, hi) at which `before` plus the weights up to it exceed `share`; if rounding leaves none, the
-// last one with a weight (0 if there is no such one either). Every thread gets it.
-template <int TYPE>
-__device__ uint32_t find(const Row<TYPE>& w, uint32_t lo, uint32_t hi, double before, double share, double* lds, uint32_t* lds_at) {
-  const uint32_t each = (hi - lo + THREADS - 1) / THREADS;
-  const uint32_t j0 = min(hi, lo + threadIdx.x * each), j1 = min(hi, j0 + each);
-  double own = 0;
-  for (uint32_t j = j0; j < j1; ++j) own += w(j);
-  const double upto = before + block_scan(own, lds);
-  if (threadIdx.x == 0) lds_at[0] = THREADS, lds_at[1] = 0;
-  __syncthreads();
-  if (own > 0 && upto > share) atomicMin(&lds_at[0], threadIdx.x);
-  if (own > 0) atomicMax(&lds_at[1], threadIdx.x);
-  __syncthreads();
-  if (threadIdx.x == (lds_at[0] < THREADS ? lds_at[0] : lds_at[1])) {
-    double sum = upto - own;
-    uint32_t last = 0;
-    for (uint32_t j = j0; j < j1; ++j) {
-      const double x = w(j);
-      sum += x;
-      if (x > 0) last = j;
-      if (x > 0 && sum > share) break;
-    }
-    lds_at[2] = last;
+  for (uint32_t piece = group * WAVES + threadIdx.x / 64; piece < W.pieces; piece += W.groups * WAVES) {
+    const double sum = piece_sum(w, piece, W.len);
+    if (threadIdx.x % 64 == 0) W.sums[(uint64_t)b * W.pieces + piece] = sum;
   }
-  __syncthreads();
-  return lds_at[2];
 }
 
+__device__ __forceinline__ double lane_of(double x, uint32_t lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// In a running sum over the lanes from `before` on, the lane whose x takes it past `share`; if rounding leaves none, the last one with an
+// x above 0. upto: the running sum with this lane's x.
+__device__ __forceinline__ uint32_t passing(double x, double before, double share, double& upto) {
+  upto = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double up = __shfl_up(upto, d);
+    if (threadIdx.x % 64 >= (uint32_t)d) upto += up;
+  }
+  upto += before;
+  const uint64_t some = __ballot(x > 0), past = __ballot(x > 0 && upto > share);
+  return past ? (uint32_t)__builtin_ctzll(past) : some ? 63u - (uint32_t)__builtin_clzll(some) : 0u;
+}
+
+// The same among a lane's own four numbers, which begin at `run`: `at` of them is where, `run` the sum before it.
+__device__ __forceinline__ void passing4(const double (&x)[4], double share, double& run, uint32_t& at, bool& done) {
+  double sum = run;
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) {
+    if (!done && x[e] > 0) at = e, run = sum, done = sum + x[e] > share;
+    sum += x[e];
+  }
+}
+
+// The token at which the running sum of a row's weights passes `part` of their whole sum, by one wave; false if the whole is 0. sums: of
+// the pieces.
 template <int TYPE>
-__global__ __launch_bounds__(THREADS) void pick_kernel(bs_draft_batch D, Work W, int32_t* status) {
-  __shared__ double lds[WAVES], total[2];
-  __shared__ uint32_t at[3];
-  const uint32_t b = blockIdx.x, tid = threadIdx.x;
-  const int32_t a = W.taken[b];
+__device__ bool pick(const Row<TYPE>& w, const Work& W, const double* sums, double part, uint32_t& token) {
+  const uint32_t lane = threadIdx.x % 64;
+  double s[4];
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) s[e] = lane * 4 + e < W.pieces ? sums[lane * 4 + e] : 0.0;
+  double own = (s[0] + s[1]) + (s[2] + s[3]);
+  const double total = wave_sum(own), share = part * total;
+  if (!(total > 0)) return false;
+  double upto, run;
+  uint32_t found = passing(own, 0.0, share, upto), at = 0;
+  bool done = false;
+  run = upto - own;
+  passing4(s, share, run, at, done);
+  const uint32_t piece = found * 4 + __builtin_amdgcn_readlane(at, found);
+  const double before = lane_of(run, found);
+  // the piece's weights, a run of them to each lane
+  const uint32_t each = W.len / 64, j0 = piece * W.len + lane * each;
+  own = 0;
+  for (uint32_t j = j0; j < j0 + each; j += 16) {
+    double x[4][4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) w.four(j + i * 4, x[i]);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) own += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
+  }
+  found = passing(own, before, share, upto);
+  run = upto - own, done = false;
+  uint32_t last = j0;
+  double sum = run;
+  for (uint32_t j = j0; j < j0 + each && !done; j += 4) {
+    double x[4];
+    w.four(j, x);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+      sum += x[e];
+      if (!done && x[e] > 0) last = j + e, done = sum > share;
+    }
+  }
+  token = __builtin_amdgcn_readlane(last, found);
+  return true;
+}
+
+// LONE: the pieces' sums are made here too, by four waves; else one wave.
+template <int TYPE, bool LONE>
+__global__ __launch_bounds__(LONE ? THREADS : 64) void pick_kernel(bs_draft_batch D, Work W, int32_t* status) {
+  __shared__ double sums[LONE ? ALONE : MOST_PIECES];
+  const uint32_t b = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int32_t a = LONE ? taken_drafts<TYPE>(D, b, wave == 0 ? status : nullptr) : W.taken[b];
+  const int32_t r0 = D.cu[b], row = r0 + a;
   int64_t* out = D.tokens + (uint64_t)b * (D.max_drafts + 1);
-  uint32_t token = 0;
-  if (a >= 0) {
-    const int32_t row = D.cu[b] + a;
-    const Row<TYPE> w(D, (uint64_t)row, row + 1 < D.cu[b + 1]);
-    const double own = tid < W.parts ? W.sums[(uint64_t)b * W.parts + tid] : 0.0;
-    const double upto = block_scan(own, lds);
-    if (tid == THREADS - 1) total[0] = upto;
-    if (tid == 0) at[0] = THREADS, at[1] = 0;
-    __syncthreads();
-    if (total[0] > 0) {
-      const double share = (double)D.pick[b] * total[0];
-      if (own > 0 && upto > share) atomicMin(&at[0], tid);
-      if (own > 0) atomicMax(&at[1], tid);
-      __syncthreads();
-      const uint32_t part = at[0] < THREADS ? at[0] : at[1];
-      if (tid == part) total[1] = upto - own;
-      __syncthreads();
-      token = find(w, part * W.len, min(D.vocab, (part + 1) * W.len), total[1], share, lds, at);
-    } else {
-      // nothing is left of the row (or it holds no probability): the target's own
-      const Row<TYPE> plain(D, (uint64_t)row, false);
-      double sum = 0;
-      for (uint32_t j = tid; j < D.vocab; j += THREADS) sum += plain(j);
-      sum = block_scan(sum, lds);
-      if (tid == THREADS - 1) total[1] = sum;
-      __syncthreads();
-      if (total[1] > 0)
-        token = find(plain, 0, D.vocab, 0.0, (double)D.pick[b] * total[1], lds, at);
-      else if (tid == 0 && status)
-        atomicOr(status, BS_DEV_ERR_COUNT);
-    }
+  if (wave == 0) {
+    for (uint32_t i = lane; i <= D.max_drafts; i += 64)
+      if ((int32_t)i != a) out[i] = (int32_t)i < a ? D.draft[r0 + (int32_t)i] : -1;
+    if (lane == 0) D.counts[b] = a + 1;
   }
-  for (uint32_t i = tid; i <= D.max_drafts; i += THREADS)
-    out[i] = (int32_t)i < a ? D.draft[D.cu[b] + (int32_t)i] : (int32_t)i == a ? (int64_t)token : -1;
-  if (tid == 0) D.counts[b] = a + 1;
+  if (a < 0) return;
+  const Row<TYPE> w(D, (uint64_t)row, row + 1 < D.cu[b + 1]);
+  if constexpr (LONE) {
+    for (uint32_t piece = wave; piece < W.pieces; piece += WAVES) {
+      const double sum = piece_sum(w, piece, W.len);
+      if (lane == 0) sums[piece] = sum;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+  }
+  uint32_t token = 0;
+  if (!pick(w, W, LONE ? sums : W.sums + (uint64_t)b * W.pieces, (double)D.pick[b], token)) {
+    // nothing is left of the row: once more with the target's own
+    const Row<TYPE> plain(D, (uint64_t)row, false);
+    for (uint32_t piece = 0; piece < W.pieces; ++piece) {
+      const double sum = piece_sum(plain, piece, W.len);
+      if (lane == 0) sums[piece] = sum;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (!pick(plain, W, sums, (double)D.pick[b], token) && lane == 0 && status) atomicOr(status, BS_DEV_ERR_COUNT);
+  }
+  if (lane == 0) out[a] = (int64_t)token;
 }
 
 Work layout(uint32_t n_seqs, uint32_t vocab, void* d_work) {
   Work w;
-  // enough workgroups to fill the card, parts of 4,096 elements at least
-  w.parts = std::max(1u, std::min({MOST_PARTS, 2048 / std::max(1u, n_seqs), (vocab + PART_MIN - 1) / PART_MIN}));
-  w.len = (vocab + w.parts - 1) / w.parts;
+  w.len = PIECE * ((vocab + MOST_PIECES * PIECE - 1) / (MOST_PIECES * PIECE));
+  w.pieces = (vocab + w.len - 1) / w.len;
+  // 2,048 workgroups fill the card; more of them would look for the drafts' end once more each
+  w.groups = std::max(1u, std::min((w.pieces + WAVES - 1) / WAVES, 2048 / std::max(1u, n_seqs)));
   w.sums = (double*)d_work;
-  w.taken = (int32_t*)(w.sums + (uint64_t)n_seqs * w.parts);
+  w.taken = (int32_t*)(w.sums + (uint64_t)n_seqs * w.pieces);
   return w;
 }
 
 template <int TYPE>
 int launch(const bs_draft_batch& D, const Work& w, int32_t* status, hipStream_t s) {
-  parts_kernel<TYPE><<<D.n_seqs * w.parts, THREADS, 0, s>>>(D, w, status);
-  pick_kernel<TYPE><<<D.n_seqs, THREADS, 0, s>>>(D, w, status);
+  if (w.pieces <= ALONE) {
+    pick_kernel<TYPE, true><<<D.n_seqs, THREADS, 0, s>>>(D, w, status);
+  } else {
+    sums_kernel<TYPE><<<D.n_seqs * w.groups, THREADS, 0, s>>>(D, w, status);
+    pick_kernel<TYPE, false><<<D.n_seqs, 64, 0, s>>>(D, w, status);
+  }
   return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP;
 }
 
 }  // namespace
 
 extern "C" uint64_t bs_draft_verify_work_bytes(uint32_t n_seqs, uint32_t vocab) {
-  return (uint64_t)n_seqs * (layout(n_seqs, vocab, nullptr).parts * 8ull + 4ull);
+  const uint32_t pieces = layout(n_seqs, vocab, nullptr).pieces;
+  return pieces <= ALONE ? 0 : (uint64_t)n_seqs * (pieces * 8ull + 4ull);
 }
 
 extern "C" int bs_draft_verify(const bs_draft_batch* D, void* d_work, uint64_t work_bytes, int32_t* d_status, void* stream) {
@@ -221,7 +299,8 @@ extern "C" int bs_draft_verify(const bs_draft_batch* D, void* d_work, uint64_t w
   if (!D->cu || !D->pick || !D->tokens || !D->counts || (D->n_rows && (!D->p || !D->draft || !D->accept))) return BS_ERR_ARG;
   const uintptr_t size = D->type == BS_DRAFT_F32 ? 3 : 1;
   if (((uintptr_t)D->p & size) || ((uintptr_t)D->q & size)) return BS_ERR_ARG;
-  if (!d_work || ((uintptr_t)d_work & 15) || work_bytes < bs_draft_verify_work_bytes(D->n_seqs, D->vocab)) return BS_ERR_CAP;
+  const uint64_t need = bs_draft_verify_work_bytes(D->n_seqs, D->vocab);
+  if (work_bytes < need || (need && (!d_work || ((uintptr_t)d_work & 15)))) return BS_ERR_CAP;
   const Work w = layout(D->n_seqs, D->vocab, d_work);
   hipStream_t s = (hipStream_t)stream;
   return D->type == BS_DRAFT_F32 ? launch<BS_DRAFT_F32>(*D, w, d_status, s)

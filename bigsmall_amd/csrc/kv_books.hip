@@ -5,8 +5,8 @@
 // own sequences: nothing passes between workgroups, so it is one launch, and the books stay as they were, so it can be
 // made again. The bound of the usual step is the launch and three dependent reads (place, length, page).
 //
-// keep_kernel enters a step into the books. drop is two launches: pages go onto the stack while lengths still stand,
-// then the places are emptied.
+// keep_kernel enters a step into the books. drop is one workgroup for a few places, else two launches: pages go onto the stack
+// while lengths still stand, then the places are emptied.
 #include <algorithm>
 
 #include "kv_common.h"
@@ -209,6 +209,58 @@ __global__ __launch_bounds__(THREADS) void empty_kernel(bs_kv_books K, const int
   if (threadIdx.x == 0) *K.n_free += (int32_t)total;
 }
 
+// Both in one launch, by one workgroup: a wave a place.
+constexpr uint32_t D_THREADS = 1024, D_PAGES = 16384;
+__global__ __launch_bounds__(D_THREADS) void drop_kernel(bs_kv_books K, const int32_t* seqs, uint32_t n_seqs, int32_t* status) {
+  __shared__ uint32_t seen[MOST_PLACES / 32];
+  __shared__ int32_t upto[D_THREADS / 64];
+  __shared__ int32_t pages[D_THREADS], to[D_THREADS];
+  __shared__ int any_bad;
+  const uint32_t tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  for (uint32_t i = tid; i < (K.n_places + 31) / 32; i += D_THREADS) seen[i] = 0;
+  if (tid == 0) any_bad = 0;
+  __syncthreads();
+  const int32_t n_free = *K.n_free;
+  const uint32_t place = tid < n_seqs ? (uint32_t)seqs[tid] : 0;
+  int32_t own = 0;
+  if (tid < n_seqs) {
+    bool bad = place >= K.n_places;
+    if (!bad) {
+      const uint32_t bit = 1u << (place % 32);
+      const int32_t length = K.length[place];
+      bad = (atomicOr(&seen[place / 32], bit) & bit) || length < 0 || length > (int32_t)(K.cols * PAGE);
+      own = bad ? 0 : length / (int32_t)PAGE;
+    }
+    if (bad) any_bad = 1;
+  }
+  int32_t before = own;  // pages up to and with this thread's
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int32_t up = __shfl_up(before, d);
+    if (lane >= (uint32_t)d) before += up;
+  }
+  if (lane == 63) upto[wave] = before;
+  __syncthreads();
+  int32_t total = 0;
+  for (uint32_t w = 0; w < D_THREADS / 64; ++w) {
+    if (w < wave) before += upto[w];
+    total += upto[w];
+  }
+  if (any_bad || n_free < 0 || (int64_t)total + n_free > (int64_t)K.n_pages) {
+    if (tid == 0) report(status, BS_DEV_ERR_BOUNDS);
+    return;
+  }
+  pages[tid] = own;
+  to[tid] = n_free + total - 1 - (before - own);
+  __syncthreads();
+  for (uint32_t b = wave; b < n_seqs; b += D_THREADS / 64) {
+    const int32_t* from = K.table + (size_t)(uint32_t)seqs[b] * K.cols;
+    for (int32_t c = (int32_t)lane; c < pages[b]; c += 64) K.free[to[b] - c] = from[c];
+  }
+  if (tid < n_seqs) K.length[place] = 0, K.which[place] = 0;
+  if (tid == 0) *K.n_free = n_free + total;
+}
+
 bool books_ok(const bs_kv_books* k) {
   return k && k->length && k->which && k->table && k->free && k->n_free && k->tails && k->n_places > 0 && k->n_places <= MOST_PLACES &&
          k->cols > 0 && k->cols < (1u << 24) && k->n_pages > 0 && k->n_pages < (1u << 30);
@@ -247,6 +299,10 @@ extern "C" int bs_kv_books_keep(const bs_kv_books* K, const bs_kv_tables* S, con
 extern "C" int bs_kv_books_drop(const bs_kv_books* K, const int32_t* d_seqs, uint32_t n_seqs, int32_t* d_status, void* stream) {
   if (!books_ok(K) || n_seqs > K->n_places || (n_seqs && !d_seqs)) return BS_ERR_ARG;
   if (n_seqs == 0) return BS_OK;
+  if (n_seqs <= D_THREADS && (uint64_t)n_seqs * K->cols <= D_PAGES) {  // 32 places of 256 pages at most: 4 us, in two launches 8
+    drop_kernel<<<1, D_THREADS, 0, (hipStream_t)stream>>>(*K, d_seqs, n_seqs, d_status);
+    return done();
+  }
   const uint32_t each = (n_seqs + MOST_GROUPS - 1) / MOST_GROUPS;
   push_kernel<<<(n_seqs + each - 1) / each, THREADS, 0, (hipStream_t)stream>>>(*K, d_seqs, n_seqs, each, d_status);
   empty_kernel<<<1, THREADS, 0, (hipStream_t)stream>>>(*K, d_seqs, n_seqs);

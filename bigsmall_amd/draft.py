@@ -22,24 +22,25 @@ _BATCH = struct.Struct("=8Q2q5I4x")
 _stream = torch._C._cuda_getCurrentRawStream
 
 
-def _vector(name, x, n, dtype, device):
-    if not isinstance(x, torch.Tensor) or x.dtype != dtype:
+def _vector(name, x, n, dtype, index):
+    """x as a contiguous vector of n numbers on device `index` (n None: any number)."""
+    if not isinstance(x, torch.Tensor) or x.dtype is not dtype:
         raise ValueError(f"{name} must be a {dtype} tensor, got {getattr(x, 'dtype', type(x).__name__)}")
-    if x.dim() != 1 or (n is not None and x.shape[0] != n):
-        raise ValueError(f"{name} has shape {tuple(x.shape)}, expected [{n if n is not None else 'sequences + 1'}]")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, p on {device}")
+    shape = x.shape
+    if len(shape) != 1 or (n is not None and shape[0] != n):
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected [{n if n is not None else 'sequences + 1'}]")
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, p is not")
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _rows(name, x, shape, dtype, device):
-    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES or (dtype is not None and x.dtype != dtype):
-        raise ValueError(f"{name} must be a {dtype or 'float32, bfloat16 or float16'} tensor, got {getattr(x, 'dtype', type(x).__name__)}")
-    if x.dim() != 2 or (shape is not None and x.shape != shape) or not 1 <= x.shape[1] <= 1 << 30:
-        raise ValueError(f"{name} has shape {tuple(x.shape)}, expected {tuple(shape) if shape is not None else '[rows, vocabulary]'}")
-    if device is not None and x.device != device:
-        raise ValueError(f"{name} is on {x.device}, p on {device}")
-    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+def _rows(name, x):
+    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES:
+        raise ValueError(f"{name} must be a float32, bfloat16 or float16 tensor, got {getattr(x, 'dtype', type(x).__name__)}")
+    shape = x.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= 1 << 30 or shape[0] > 1 << 30:
+        raise ValueError(f"{name} has shape {tuple(shape)}, expected [rows, vocabulary]")
+    return x if x.stride(1) == 1 or shape[1] == 1 else x.contiguous()
 
 
 def draft_verify(p, draft, cu, accept, pick, q=None, max_drafts=None, status=None):
@@ -62,36 +63,43 @@ def draft_verify(p, draft, cu, accept, pick, q=None, max_drafts=None, status=Non
     status: a device.StatusWord that gets BS_DEV_ERR_BOUNDS where rows do not exist or are more than max_drafts + 1 (the
     sequence gets no token) or a draft is no token (it is refused), and BS_DEV_ERR_COUNT where p's row has no
     probability at all (the token is 0)."""
-    p = _rows("p", p, None, None, None)
-    index, device, (t, vocab) = p.get_device(), p.device, p.shape
+    p = _rows("p", p)
+    index, (t, vocab) = p.get_device(), p.shape
+    qp = q_stride = 0
     if q is not None:
-        q = _rows("q", q, p.shape, p.dtype, device)
-    draft = _vector("draft", draft, t, torch.int64, device)
-    accept = _vector("accept", accept, t, torch.float32, device)
-    cu = _vector("cu", cu, None, torch.int32, device)
+        q = _rows("q", q)
+        if q.dtype is not p.dtype or q.shape != p.shape or q.get_device() != index:
+            raise ValueError(f"q is {q.dtype} {tuple(q.shape)} on {q.device}, p {p.dtype} {tuple(p.shape)} on {p.device}")
+        qp, q_stride = q.data_ptr(), q.stride(0)
+    draft = _vector("draft", draft, t, torch.int64, index)
+    accept = _vector("accept", accept, t, torch.float32, index)
+    cu = _vector("cu", cu, None, torch.int32, index)
     b = cu.shape[0] - 1
     if not 0 <= b <= 1 << 20:
         raise ValueError(f"cu has {b + 1} numbers, expected 1 to {(1 << 20) + 1}")
-    pick = _vector("pick", pick, b, torch.float32, device)
+    pick = _vector("pick", pick, b, torch.float32, index)
     if max_drafts is None:
         max_drafts = min(max(0, t - b), MOST_DRAFTS)
     if not 0 <= max_drafts <= MOST_DRAFTS:
         raise ValueError(f"max_drafts must be 0 to {MOST_DRAFTS}, got {max_drafts}")
-    if t > 1 << 30:
-        raise ValueError(f"{t} rows: at most {1 << 30}")
     if index < 0:
-        raise RuntimeError(f"draft_verify runs on an AMD GPU (MI355X); p is on {device}")
+        raise RuntimeError(f"draft_verify runs on an AMD GPU (MI355X); p is on {p.device}")
+    device = p.device
     tokens = torch.empty((b, max_drafts + 1), dtype=torch.int64, device=device)
-    counts = torch.empty((b,), dtype=torch.int32, device=device)
+    counts = torch.empty(b, dtype=torch.int32, device=device)
     if b:
         L = _native.lib()
         n = L.bs_draft_verify_work_bytes(b, vocab)
-        work = torch.empty(n, dtype=torch.uint8, device=device)
-        batch = _BATCH.pack(p.data_ptr(), q.data_ptr() if q is not None else 0, draft.data_ptr(), accept.data_ptr(), cu.data_ptr(),
-                            pick.data_ptr(), tokens.data_ptr(), counts.data_ptr(), p.stride(0), q.stride(0) if q is not None else 0,
+        work = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        batch = _BATCH.pack(p.data_ptr(), qp, draft.data_ptr(), accept.data_ptr(), cu.data_ptr(),
+                            pick.data_ptr(), tokens.data_ptr(), counts.data_ptr(), p.stride(0), q_stride,
                             _TYPES[p.dtype], t, vocab, b, max_drafts)
-        with torch.cuda.device(index):
-            rc = L.bs_draft_verify(batch, work.data_ptr(), n, status.ptr if status else None, _stream(index))
+        args = batch, work.data_ptr() if n else 0, n, status.ptr if status else None
+        if index == torch.cuda.current_device():
+            rc = L.bs_draft_verify(*args, _stream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = L.bs_draft_verify(*args, _stream(index))
         if rc:
             _native.check(rc, "bs_draft_verify")
     return tokens, counts

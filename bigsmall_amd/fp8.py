@@ -18,6 +18,7 @@ not synchronise; work areas come from torch's allocator for each call.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -40,6 +41,10 @@ def _gpu(index: int, what) -> None:
 def _refuse_grad() -> None:
     raise RuntimeError("fp8_linear has no backward pass: call it under torch.no_grad(), or detach its input")
 
+
+# bs_fp8_rows of include/bigsmall_fp8.h
+_ROWS = struct.Struct("=2Q4I")
+assert _ROWS.size == ctypes.sizeof(_native.BsFp8Rows)
 
 _stream = torch._C._cuda_getCurrentRawStream
 _recording = torch.is_grad_enabled
@@ -92,11 +97,20 @@ class Fp8Rows:
     """What fp8_quantise returns: codes [rows, inner] in e4m3, scales f32 [rows, inner / 128] (views of the
     kernels' own layout), and the leading shape and type of what was quantised."""
 
-    __slots__ = ("codes", "scales", "shape", "dtype", "index", "c", "ref")
+    __slots__ = ("shape", "dtype", "rows", "inner", "index", "ref", "_codes", "_scales")
 
-    def __init__(self, codes, scales, shape, dtype, c):
-        self.codes, self.scales, self.shape, self.dtype, self.c = codes, scales, shape, dtype, c
-        self.index, self.ref = codes.get_device(), ctypes.byref(c)
+    def __init__(self, codes, scales, rows, inner, shape, dtype, index):
+        self._codes, self._scales, self.rows, self.inner, self.shape, self.dtype, self.index = codes, scales, rows, inner, shape, dtype, index
+        self.ref = _ROWS.pack(codes.data_ptr(), scales.data_ptr(), rows, inner, codes.shape[1], rows)
+
+    @property
+    def codes(self):
+        c = self._codes
+        return c if c.shape[1] == self.inner else c.narrow(1, 0, self.inner)
+
+    @property
+    def scales(self):
+        return self._scales.t()
 
 
 def _matrix(x):
@@ -114,23 +128,24 @@ def fp8_quantise(x) -> Fp8Rows:
     """x [..., inner], bf16 or f16, in e4m3 with a scale for each 128 columns of a row: a = max |x| of the block
     (held to at least 2^-100), scale = a / 448, code = 448 x / a to nearest even, the exact quotient rounded once. A block
     that holds an infinity or a NaN has codes 0 and scale NaN, so the rows of a product with it are NaN."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES:
+    kind = _TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if kind is None:
         raise ValueError(f"x must be a bfloat16 or float16 tensor, got {getattr(x, 'dtype', type(x).__name__)}")
-    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > _MOST_COLS:
-        raise ValueError(f"x has shape {tuple(x.shape)}; its last dimension must hold 1 to {_MOST_COLS} columns")
+    shape = x.shape
+    if not shape or not 0 < shape[-1] <= _MOST_COLS:
+        raise ValueError(f"x has shape {tuple(shape)}; its last dimension must hold 1 to {_MOST_COLS} columns")
     index = x.get_device()
     _gpu(index, x)
     if x.requires_grad and _recording():
         _refuse_grad()
-    shape = x.shape[:-1]
     y, t, k = _matrix(x)
-    wide = _blocks(k) * BLOCK
-    codes = torch.empty((t, wide), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((wide // BLOCK, t), dtype=torch.float32, device=x.device)
-    c = _native.BsFp8Rows(codes.data_ptr(), scales.data_ptr(), t, k, wide, t)
-    rows = Fp8Rows(codes[:, :k], scales.T, shape, x.dtype, c)
+    blocks = (k + BLOCK - 1) // BLOCK
+    device = x.device
+    codes = torch.empty((t, blocks * BLOCK), dtype=torch.float8_e4m3fn, device=device)
+    scales = torch.empty((blocks, t), dtype=torch.float32, device=device)
+    rows = Fp8Rows(codes, scales, t, k, shape[:-1], x.dtype, index)
     if t:
-        _call("bs_fp8_quantise", index, y.data_ptr(), _TYPES[x.dtype], y.stride(0), rows.ref)
+        _call("bs_fp8_quantise", index, y.data_ptr(), kind, y.stride(0), rows.ref)
     return rows
 
 
@@ -141,9 +156,9 @@ def fp8_linear(x, weight: Fp8Weight, dtype=None):
         raise ValueError("weight must be an Fp8Weight")
     index = weight.index
     if isinstance(x, Fp8Rows):
-        t, k, shape, rows = x.c.rows, x.c.cols, x.shape, x
-        if k != weight.inner:
-            raise ValueError(f"x has {k} columns, the weight {weight.inner}")
+        t, shape, rows = x.rows, x.shape, x
+        if x.inner != weight.inner:
+            raise ValueError(f"x has {x.inner} columns, the weight {weight.inner}")
         if x.index != index:
             raise ValueError(f"x is on {x.codes.device}, the weight on {weight.device}")
     else:

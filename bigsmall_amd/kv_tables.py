@@ -16,6 +16,7 @@ books are one sequence of calls, so calls on several streams need the usual wait
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
@@ -24,6 +25,10 @@ from . import _native
 from .paged_kv import PAGE, KVBatch, _tensor
 
 MOST_PLACES = 65536
+
+# bs_kv_tables of include/bigsmall_kv.h
+_TABLES = struct.Struct("=8Q3I4x")
+assert _TABLES.size == ctypes.sizeof(_native.BsKvTables)
 
 _stream = torch._C._cuda_getCurrentRawStream
 
@@ -72,17 +77,22 @@ class KVTables:
         self._made, self._give_back = None, None
 
     def _vector(self, name, x, n=None):
-        if x.__class__ is not torch.Tensor and not isinstance(x, torch.Tensor):
-            raise ValueError(f"{name} must be an int32 tensor, got {type(x).__name__}")
-        if x.dtype != torch.int32 or x.dim() != 1 or (n is not None and x.shape[0] != n):
-            raise ValueError(f"{name} must be an int32 tensor [{n if n is not None else 'sequences'}], got {x.dtype} {tuple(x.shape)}")
+        if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32:
+            raise ValueError(f"{name} must be an int32 tensor, got {getattr(x, 'dtype', type(x).__name__)}")
+        shape = x.shape
+        if len(shape) != 1 or (n is not None and shape[0] != n):
+            raise ValueError(f"{name} has shape {tuple(shape)}, expected [{n if n is not None else 'sequences'}]")
         if x.get_device() != self.index:
             raise ValueError(f"{name} is on {x.device}, the tables are on {self.device}")
         return x if x.is_contiguous() else x.contiguous()
 
     def _call(self, name, *args):
-        with torch.cuda.device(self.index):
-            rc = getattr(_native.lib(), name)(self.ref, *args, _stream(self.index))
+        index = self.index
+        if index == torch.cuda.current_device():
+            rc = getattr(_native.lib(), name)(self.ref, *args, _stream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = getattr(_native.lib(), name)(self.ref, *args, _stream(index))
         if rc:
             _native.check(rc, name)
 
@@ -105,23 +115,27 @@ class KVTables:
         new = self._vector("new", new, b)
         if sure is not None:
             sure = self._vector("sure", sure, b)
-        if not 0 <= rows < 1 << 30:
-            raise ValueError(f"rows is {rows}")
+        max_new, max_len = rows if max_new is None else int(max_new), self.longest if max_len is None else int(max_len)
+        if not (0 <= rows < 1 << 30 and 0 <= max_new < 1 << 30 and 0 <= max_len < 1 << 30):
+            raise ValueError(f"rows {rows}, max_new {max_new} and max_len {max_len} must be 0 or more, below 2^30")
         cols = self.longest // PAGE
         small = 4 * b + 1 + b * cols
         # one allocation: slot first, which wants 8 bytes, then the tables, then owner and position
-        flat = torch.empty(2 * rows + small + 2 * rows, dtype=torch.int32, device=self.device)
-        slot, start, cu, tails, table, owner, position = flat.split([2 * rows, b, b + 1, 2 * b, b * cols, rows, rows])
-        slot, tails, table = slot.view(torch.int64), tails.view(b, 2), table.view(b, cols)
-        batch = KVBatch(start, cu, table, tails, rows if max_new is None else max_new, self.longest if max_len is None else max_len, rows)
+        flat = torch.empty(4 * rows + small, dtype=torch.int32, device=self.device)
+        slot, start, cu, tails, table, owner, position = flat.split_with_sizes((2 * rows, b, b + 1, 2 * b, b * cols, rows, rows))
         at = flat.data_ptr()
-        begin = at + 8 * rows
-        c = _native.BsKvTables(seqs.data_ptr(), begin, begin + 4 * b, begin + 4 * (2 * b + 1), begin + 4 * (4 * b + 1),
-                               begin + 4 * small, begin + 4 * (small + rows), at, b, rows, batch.max_new)
-        self._call("bs_kv_books_step", ctypes.byref(c), new.data_ptr(), sure.data_ptr() if sure is not None else 0,
-                   status.ptr if status else None)
+        start_at = at + 8 * rows
+        cu_at = start_at + 4 * b
+        tails_at = cu_at + 4 * (b + 1)
+        table_at = tails_at + 8 * b
+        owner_at = at + 8 * rows + 4 * small
+        batch = KVBatch.__new__(KVBatch)
+        batch._set(start, cu, table.view(b, cols), tails.view(b, 2), b, cols, cols, max_new, max_len, rows, self.index, start_at, cu_at,
+                   table_at, tails_at)
+        c = _TABLES.pack(seqs.data_ptr(), start_at, cu_at, tails_at, table_at, owner_at, owner_at + 4 * rows, at, b, rows, max_new)
+        self._call("bs_kv_books_step", c, new.data_ptr(), sure.data_ptr() if sure is not None else 0, status.ptr if status else None)
         self._made = (batch, c, seqs, sure)
-        return batch, StepRows(owner, position, slot)
+        return batch, StepRows(owner, position, slot.view(torch.int64))
 
     def keep(self, step: KVBatch, kept=None) -> None:
         """Enter the step that was made last into the books, once: of each sequence's new tokens the first kept[b]
@@ -131,7 +145,7 @@ class KVTables:
         _, c, _, sure = self._made
         if kept is not None:
             kept = self._vector("kept", kept, step.n_seqs)
-        self._call("bs_kv_books_keep", ctypes.byref(c), sure.data_ptr() if sure is not None else 0,
+        self._call("bs_kv_books_keep", c, sure.data_ptr() if sure is not None else 0,
                    kept.data_ptr() if kept is not None else 0)
         self._made = None
 

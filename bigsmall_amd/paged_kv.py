@@ -83,6 +83,11 @@ class KVPool:
         self.ref = ctypes.byref(self.c)
 
 
+# bs_kv_batch of include/bigsmall_kv.h around its n_rows, which each call says for itself
+_BATCH_HEAD, _BATCH_REST = struct.Struct("=4Q3I"), struct.Struct("=2I")
+assert _BATCH_HEAD.size == _native.BsKvBatch.n_rows.offset and _BATCH_HEAD.size + 4 + _BATCH_REST.size == ctypes.sizeof(_native.BsKvBatch)
+
+
 class KVBatch:
     """One step over a batch of sequences, device int32 tensors:
 
@@ -100,7 +105,7 @@ class KVBatch:
     only a status word tells.
     """
 
-    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "before", "c", "_head", "_rest")
+    __slots__ = ("start", "cu", "table", "tails", "index", "n_seqs", "max_new", "max_len", "total", "before", "_head", "_rest")
 
     def __init__(self, start, cu, table, tails, max_new: int, max_len: int, total: Optional[int] = None):
         _tensor("start", start, torch.int32)
@@ -117,14 +122,19 @@ class KVBatch:
             raise ValueError("KVBatch: start, cu and tails must be contiguous, table's rows apart")
         if b > 65535 or not 0 <= max_new < 1 << 30 or not 0 <= max_len < 1 << 30:
             raise ValueError("KVBatch: at most 65535 sequences, max_new and max_len below 2^30")
+        self._set(start, cu, table, tails, b, stride, table.shape[1], int(max_new), int(max_len), total, start.get_device(), start.data_ptr(),
+                  cu.data_ptr(), table.data_ptr(), tails.data_ptr())
+
+    def _set(self, start, cu, table, tails, b, stride, cols, max_new, max_len, total, index, *at):
+        """The fields, of what is known to fit; at: the four tensors' addresses."""
         self.start, self.cu, self.table, self.tails = start, cu, table, tails
-        self.n_seqs, self.max_new, self.max_len, self.total = b, int(max_new), int(max_len), total
+        self.n_seqs, self.max_new, self.max_len, self.total, self.index = b, max_new, max_len, total, index
         self.before = None           # of a PagedKVCache's step: how to take it back
-        self.c = _native.BsKvBatch(start.data_ptr(), cu.data_ptr(), table.data_ptr(), tails.data_ptr(), b, stride,
-                                   table.shape[1], 0, int(max_new), int(max_len))
-        self.index = start.get_device()
-        at = _native.BsKvBatch.n_rows.offset
-        self._head, self._rest = bytes(self.c)[:at], bytes(self.c)[at + 4:]
+        self._head, self._rest = _BATCH_HEAD.pack(*at, b, stride, cols), _BATCH_REST.pack(max_new, max_len)
+
+    @property
+    def c(self):
+        return _native.BsKvBatch.from_buffer_copy(self.with_rows(0))
 
     def with_rows(self, n: int) -> bytes:
         """The C structure of a call with n rows: a value of its own, since layers and threads share the batch."""

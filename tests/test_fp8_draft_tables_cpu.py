@@ -172,9 +172,10 @@ def test_c_entries_refuse_bad_arguments():
     for c in (dict(p=0), dict(draft=0), dict(accept=0), dict(cu=0), dict(pick=0), dict(tokens=0), dict(counts=0), dict(type=3), dict(vocab=0),
               dict(vocab=1 << 31), dict(max_drafts=1025), dict(n_seqs=1 << 21), dict(p=at + 2), dict(q=at + 1), dict(p_stride=-1), dict(n_rows=1 << 31)):
         assert L.bs_draft_verify(p(batch(**c)), at, 1 << 30, None, None) == ARG, c
-    need = L.bs_draft_verify_work_bytes(1, 10)
-    assert L.bs_draft_verify(p(batch()), at, need - 1, None, None) == CAP
-    assert L.bs_draft_verify(p(batch()), at + 4, need, None, None) == CAP and L.bs_draft_verify(p(batch()), None, need, None, None) == CAP
+    large = batch(vocab=100000, p_stride=100000, q_stride=100000)
+    need = L.bs_draft_verify_work_bytes(1, 100000)
+    assert need > 0 and L.bs_draft_verify(p(large), at, need - 1, None, None) == CAP
+    assert L.bs_draft_verify(p(large), at + 4, need, None, None) == CAP and L.bs_draft_verify(p(large), None, need, None, None) == CAP
 
     def books(**c):
         f = dict(length=at, which=at, table=at, free=at, n_free=at, tails=at, n_places=4, cols=2, n_pages=8)
@@ -219,8 +220,14 @@ def test_c_structures_match_their_headers(tmp_path):
         assert got[name] == (ctypes.sizeof(mirror),)
         for f in mirror._fields_:
             assert got[f"{name}.{f[0]}"] == (getattr(mirror, f[0]).offset, ctypes.sizeof(f[1])), (name, f[0])
-    values = list(range(1, 16))
-    assert draft._BATCH.pack(*values) == bytes(_native.BsDraftBatch(*values))
+    # packed by hand: each field's number where the C structure has it
+    for packer, mirror in ((draft._BATCH, _native.BsDraftBatch), (fp8._ROWS, _native.BsFp8Rows), (kv_tables._TABLES, _native.BsKvTables)):
+        values = [i + 1 for i in range(len(mirror._fields_))]
+        back = mirror.from_buffer_copy(packer.pack(*values))
+        assert packer.size == ctypes.sizeof(mirror) and [getattr(back, f[0]) for f in mirror._fields_] == values
+    from bigsmall_amd import paged_kv
+    b = _native.BsKvBatch.from_buffer_copy(paged_kv._BATCH_HEAD.pack(1, 2, 3, 4, 5, 6, 7) + (8).to_bytes(4, "little") + paged_kv._BATCH_REST.pack(9, 10))
+    assert [getattr(b, f[0]) for f in _native.BsKvBatch._fields_] == list(range(1, 11))
 
 
 def test_reference_quantiser_is_torchs_rounding():

@@ -86,8 +86,19 @@ def test_against_the_definition(seqs, drafts, vocab, dtype, model):
 def test_many_sequences_and_a_large_vocabulary():
     c, d = _case(700, 2, 300, torch.float32, True, 5)
     _same(_run(c, d), reference(**c, max_drafts=d))
-    c, d = _case(2, 2, 200001, torch.float32, True, 6, spread=3.0)
+    for seqs, vocab, dtype in ((2, 200001, torch.float32), (1, 262145, torch.float32), (1, 700004, torch.bfloat16)):
+        c, d = _case(seqs, 2, vocab, dtype, True, 6, spread=3.0)
+        _same(_run(c, d), reference(**c, max_drafts=d))
+
+
+@pytest.mark.parametrize("model", [True, False])
+@pytest.mark.parametrize("vocab", [4, 256, 1023, 1024, 1025, 8192, 8193, 9216, 20000])
+def test_borders_of_pieces(vocab, model):
+    c, d = _case(5, 3, vocab, TYPES[vocab % 3], model, vocab, spread=0.3)
     _same(_run(c, d), reference(**c, max_drafts=d))
+    for pick in (0.0, 1 - 2.0 ** -24):
+        t = dict(c, pick=torch.full((5,), pick))
+        _same(_run(t, d), reference(**t, max_drafts=d))
 
 
 def test_picks_at_both_ends_and_between_equal_weights():

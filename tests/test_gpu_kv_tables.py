@@ -122,11 +122,11 @@ def test_prompts_drafts_and_drops():
     assert int(t.n_free) == 200
 
 
-@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("seed", range(8))
 def test_random_walks(seed):
     import random
     rng = random.Random(seed)
-    t, b = _both(pages=rng.choice([30, 60, 400]), places=rng.choice([1, 5, 70]), longest=rng.choice([64, 300, 2000]), seed=seed)
+    t, b = _both(pages=rng.choice([30, 60, 400]), places=rng.choice([1, 5, 70]), longest=rng.choice([64, 300, 2000, 100000]), seed=seed)
     places = len(b.tails)
     for _ in range(30):
         seqs = rng.sample(range(places), rng.randint(1, places))
@@ -188,9 +188,10 @@ def test_all_or_nothing(seqs, new, sure, rows, bit):
     _step(t, b, [1], [5], None, 5)
 
 
-def test_drop_all_or_nothing():
+@pytest.mark.parametrize("longest", [1000, 200000])
+def test_drop_all_or_nothing(longest):
     from bigsmall_amd.device import StatusWord
-    t, b = _both()
+    t, b = _both(longest=longest)
     t.keep(_step(t, b, [0, 1], [700, 80], None, 780))
     b.keep()
     for seqs in ([0, 0], [0, 8], [-1], [1, 0, 1]):
@@ -199,6 +200,9 @@ def test_drop_all_or_nothing():
         assert int(status.t) == BOUNDS
         _same_state(t, b)
     t.drop(_i32([]))
+    _same_state(t, b)
+    t.drop(_i32([1, 5, 0]))
+    b.drop([1, 5, 0])
     _same_state(t, b)
 
 
