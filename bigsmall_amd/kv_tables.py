@@ -111,7 +111,7 @@ class KVTables:
         seqs = self._vector("seqs", seqs)
         b = seqs.shape[0]
         if not 0 < b <= min(self.places, 65535):
-            raise ValueError(f"a step of {b} sequences; the tables have {self.places} places")
+            raise ValueError(f"a step of {b} sequences; the tables have {self.places} places" + ("" if self.places else " (closed)"))
         new = self._vector("new", new, b)
         if sure is not None:
             sure = self._vector("sure", sure, b)
@@ -158,11 +158,22 @@ class KVTables:
         self._made = None
         self._call("bs_kv_books_drop", seqs.data_ptr(), seqs.shape[0], status.ptr if status else None)
 
+    def lent_by(self, give_back) -> None:
+        """give_back() is called by close()."""
+        self._give_back = give_back
+
     def close(self) -> None:
-        """Give pages and tails back to the cache that lent them; the tables are not to be used any more."""
+        """Give pages and tails back to the cache that lent them. Sequences in the tables end with it, and steps are refused."""
         give, self._give_back = self._give_back, None
+        self._made, self.places = None, 0
         if give is not None:
             give()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
 
 
 __all__ = ["MOST_PLACES", "KVTables", "StepRows"]

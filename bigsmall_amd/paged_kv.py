@@ -397,6 +397,19 @@ class PagedKVCache:
     def free_pages(self) -> int:
         return len(self._books.free)
 
+    def tables(self, sequences: int, longest: int, pages: Optional[int] = None):
+        """Books on the GPU (a KVTables) over `pages` of this cache's free pages (None: all of them) and places for as many
+        sequences, lent until its close(). Its steps are for append and attend like this cache's own."""
+        from .kv_tables import KVTables
+        numbers, tails, give_back = self._books.lend(sequences, pages)
+        try:
+            lent = KVTables(*(torch.tensor(x, dtype=torch.int32, device="cpu").to(self.device) for x in (numbers, tails)), longest)
+        except BaseException:
+            give_back()
+            raise
+        lent.lent_by(give_back)
+        return lent
+
     def step(self, new: dict) -> KVBatch:
         """A step that appends new[seq] tokens to each sequence, rows packed in the dict's order. Takes the
         pages it needs (RuntimeError, and nothing taken, if there are too few). Appending must follow for
@@ -461,6 +474,21 @@ class _Books:
         seq, self.next = self.next, self.next + 1
         self.seqs[seq] = [0, [], tail, tail + 1]
         return seq
+
+    def lend(self, sequences: int, pages) -> tuple:
+        """Page numbers and first tails taken for other books, and how to give them back."""
+        if not 0 < sequences <= len(self.free_tails):
+            raise RuntimeError(f"PagedKVCache: {sequences} sequences asked for, {len(self.free_tails)} are free")
+        pages = len(self.free) if pages is None else pages
+        if not 0 < pages <= len(self.free):
+            raise RuntimeError(f"PagedKVCache: {pages} pages asked for, {len(self.free)} are free")
+        numbers, tails = self.free[-pages:], self.free_tails[-sequences:]
+        del self.free[-pages:], self.free_tails[-sequences:]
+
+        def give_back():
+            self.free += numbers
+            self.free_tails += tails
+        return numbers, tails, give_back
 
     def drop(self, seq) -> None:
         _, pages, a, b = self._get(seq)

@@ -245,3 +245,52 @@ def test_exported():
     import bigsmall_amd as bs
     assert (bs.Fp8Weight, bs.fp8_quantise, bs.fp8_linear) == (fp8.Fp8Weight, fp8.fp8_quantise, fp8.fp8_linear)
     assert (bs.draft_verify, bs.KVTables, bs.StepRows) == (draft.draft_verify, kv_tables.KVTables, kv_tables.StepRows)
+
+
+class _Names:
+    """A loader's index."""
+
+    dtype = None
+
+    def __init__(self, layer=(), top=()):
+        from bigsmall_amd.paged_llama import _LAYER, _TOP
+        self.top, self.layer = list(_TOP) + list(top), [f"model.layers.0.{n}" for n in list(_LAYER) + list(layer)]
+
+    def layer_count(self):
+        return 1
+
+    def non_layer_tensor_names(self):
+        return self.top
+
+    def layer_tensor_names(self, i):
+        return self.layer
+
+
+def test_models_with_fp8_weights():
+    from types import SimpleNamespace
+
+    from bigsmall_amd.paged_llama import _SCALES, check_model
+    fp8_way = {"quant_method": "fp8", "weight_block_size": [128, 128], "activation_scheme": "dynamic"}
+
+    def config(q=None):
+        return SimpleNamespace(model_type="llama", num_hidden_layers=1, max_position_embeddings=64, quantization_config=q)
+
+    check_model(config(), _Names())
+    check_model(config(), _Names(_SCALES))
+    check_model(config(), _Names(["mlp.up_proj.weight_scale_inv"]))            # some of them in bf16
+    check_model(config(fp8_way), _Names(_SCALES))
+    check_model(config(SimpleNamespace(to_dict=lambda: fp8_way)), _Names(_SCALES))
+    for change in (dict(quant_method="awq"), dict(weight_block_size=[64, 128]), dict(weight_block_size=None), dict(activation_scheme="static")):
+        with pytest.raises(ValueError, match="quantised otherwise"):
+            check_model(config(dict(fp8_way, **change)), _Names(_SCALES))
+    check_model(config(dict(quant_method="awq")), _Names())                    # weights as they are, whatever they were made from
+    for names in (_Names(["input_layernorm.weight_scale_inv"]), _Names(["mlp.up_proj.input_scale"]), _Names(top=["lm_head.weight_scale_inv"])):
+        with pytest.raises(ValueError, match="does not use"):
+            check_model(config(), names)
+    loader = _Names(_SCALES)
+    loader.dtype = torch.bfloat16
+    with pytest.raises(ValueError, match="casts"):
+        check_model(config(), loader)
+    with pytest.raises(ValueError, match="scale_inv"):
+        from bigsmall_amd.paged_llama import PagedLlama
+        PagedLlama._project(torch.zeros(1, 128), {"a.weight": torch.zeros(128, 128).to(E4M3)}, "a")
