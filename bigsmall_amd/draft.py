@@ -53,7 +53,7 @@ def draft_verify(p, draft, cu, accept, pick, q=None, max_drafts=None, status=Non
                      accept and q are not read. A sequence without rows gets no token and count 0
     accept [T], pick [B] f32   random numbers in [0, 1)
     q [T, vocab]     the probabilities that the drafts were drawn from, of p's type; None: they were not drawn
-    max_drafts       the most that a sequence has (by default T - B, or 0)
+    max_drafts       the most that a sequence has, up to 1,024 (by default T - B, held to 0 and 1,024)
 
     Draft x is taken while accept * q[x] < p[x] (without q: accept < p[x]). Then one token is drawn: where a draft was
     refused from max(p - q, 0) of its row (without q: from p without the draft), after the last one from p. It is the first

@@ -105,7 +105,7 @@ class KVTables:
         sequence gets no more of them than complete no page (which is quantised once): its number of new tokens is the
         difference of the KVBatch's cu. max_new, max_len: as KVBatch takes them (rows and longest by default).
 
-        The books stay as they are until `keep`; another step made before it replaces this one. All or nothing: where
+        The books stay as they are until `keep`, which reads seqs and sure again; another step made before it replaces this one. All or nothing: where
         pages, rows or a place's length do not suffice (status, a device.StatusWord, gets BS_DEV_ERR_COUNT), or places do
         not exist or are named twice or numbers are negative (BS_DEV_ERR_BOUNDS), no sequence has a new token."""
         seqs = self._vector("seqs", seqs)

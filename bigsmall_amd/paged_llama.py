@@ -180,8 +180,10 @@ class PagedLlama:
 
     def _probabilities(self, logits, temperature):
         if temperature:
-            return torch.softmax(logits.float() / temperature, -1)
-        return torch.zeros(logits.shape, device=logits.device).scatter_(1, logits.argmax(-1, keepdim=True), 1.0)
+            x = logits.float()         # (the largest first taken off: no temperature makes it an infinity)
+            return torch.softmax((x - x.amax(-1, keepdim=True)) / max(temperature, 1e-30), -1)
+        one = torch.zeros(logits.shape, dtype=torch.float32, device=logits.device)
+        return one.scatter_(1, logits.argmax(-1, keepdim=True), 1.0)
 
     @torch.no_grad()
     def _generate_drafted(self, prompts, max_new_tokens, draft, drafts, temperature, generator):
@@ -193,6 +195,11 @@ class PagedLlama:
             return [torch.empty(0, dtype=torch.int64) for _ in prompts]
         b, dev = len(prompts), self.device
         ids = [torch.as_tensor(t).to(dev).long() for t in prompts]
+        if min(len(t) for t in ids) < 1:
+            raise ValueError("a prompt needs at least one token")
+        flat = torch.cat(ids)
+        if not 0 <= int(flat.min()) <= int(flat.max()) < self.embed.shape[0]:
+            raise ValueError("a prompt holds ids that are no tokens")
         longest = max(len(t) for t in ids) + max_new_tokens
         places = torch.arange(b, dtype=torch.int32, device=dev)
         status = StatusWord(dev)
@@ -201,7 +208,7 @@ class PagedLlama:
             return torch.tensor(x, dtype=torch.int32, device="cpu").to(dev)
 
         def rand(n):
-            return torch.rand(n, generator=generator, device=dev)
+            return torch.rand(n, generator=generator, dtype=torch.float32, device=dev)
 
         def run(tables, new, sure, rows, widest, reach):
             step, at = tables.step(places, new, sure, rows=rows, max_new=widest, max_len=reach, status=status)
@@ -213,10 +220,7 @@ class PagedLlama:
             tokens = torch.zeros(b, tables.longest + drafts + 1, dtype=torch.int64, device=dev)   # (room for what is cut off at the end)
             row = torch.arange(b, device=dev)
             lens = [len(t) for t in ids]
-            if min(lens) < 1:
-                raise ValueError("a prompt needs at least one token")
             step, at = run(tables, i32(lens), None, sum(lens), max(lens), max(lens))
-            flat = torch.cat(ids)
             tokens[at.owner, at.position] = flat
             x = self._hidden(step, flat)
             tables.keep(step)

@@ -152,7 +152,7 @@ int bs_kv_books_step(const bs_kv_books *books, const bs_kv_tables *step, const i
                      int32_t *d_status, void *stream);
 
 /* Enter the last step into the books: of sequence b's new tokens the first d_kept[b] stay (NULL: all), held to what is
- * certain and what there is. Once. */
+ * certain and what there is. Once. seqs, d_sure and the step's arrays are as they were for the step. */
 int bs_kv_books_keep(const bs_kv_books *books, const bs_kv_tables *step, const int32_t *d_sure, const int32_t *d_kept,
                      void *stream);
 

@@ -360,6 +360,48 @@ def test_refusals(model, fp8_model):  # noqa: F811
         PagedLlama(loader, config, pages=4, sequences=2)
 
 
+def test_prompts_are_tokens(model):  # noqa: F811
+    """(an id past the embedding is refused before anything reads it)"""
+    import bigsmall_amd
+    from bigsmall_amd.paged_llama import PagedLlama
+    path, config, _ = model
+    with bigsmall_amd.StreamingLoader(str(path), device="cuda") as loader:
+        m = PagedLlama(loader, config, pages=4, sequences=2)
+        for bad in (-1, config.vocab_size, 1 << 40):
+            with pytest.raises(ValueError, match="no tokens"):
+                m.generate([torch.arange(3), torch.tensor([1, bad])], 8, temperature=0.5)
+        assert m.cache.free_pages() == 4
+
+
+def test_low_temperatures_and_another_default_type(model):  # noqa: F811
+    """As the temperature goes to 0 what is drawn is the likeliest token; torch's default type changes nothing."""
+    import bigsmall_amd
+    from bigsmall_amd.paged_llama import PagedLlama
+    path, config, _ = model
+    prompts = [torch.arange(70) % config.vocab_size, torch.arange(3)]
+
+    def draft(tokens, lengths, n):
+        return tokens[torch.arange(2, device="cuda"), lengths.long() - 1][:, None].expand(2, n), None
+
+    with bigsmall_amd.StreamingLoader(str(path), device="cuda") as loader:
+        m = PagedLlama(loader, config, pages=8, sequences=2)
+        greedy = [o.tolist() for o in m.generate(prompts, 10, draft=draft)]
+
+        def drawn(temperature):
+            g = torch.Generator(device="cuda").manual_seed(3)
+            return [o.tolist() for o in m.generate(prompts, 10, draft=draft, temperature=temperature, generator=g)]
+
+        for temperature in (1e-45, 1e-38, 1e-20):
+            assert drawn(temperature) == greedy
+        before = torch.get_default_dtype()
+        try:
+            torch.set_default_dtype(torch.bfloat16)
+            assert [o.tolist() for o in m.generate(prompts, 10, draft=draft)] == greedy
+            assert drawn(1e-20) == greedy
+        finally:
+            torch.set_default_dtype(before)
+
+
 def test_example_runs(monkeypatch, capsys):
     monkeypatch.setattr(sys, "argv", ["draft_generate.py", "--layers", "2", "--tokens", "6", "--drafts", "3"])
     runpy.run_path(str(ROOT / "examples" / "draft_generate.py"), run_name="__main__")
