@@ -135,6 +135,27 @@ def test_linear_large(t, n, k):
     assert torch.equal(bs.fp8_linear(rows, weight), y)
 
 
+# More tiles of 256 by 256 than compute units, so that a workgroup has several: of one, two, three and more blocks; tiles that are
+# stored whole before ones that are not and after them (4,608 = 18 * 256; odd rows of y).
+MANY = [(4200, 4300, 128), (8192, 4096, 128), (4350, 4608, 384), (4200, 4300, 256), (9000, 4608, 130), (4608, 4611, 520), (8200, 4107, 70),
+        (4100, 4400, 8400)]
+
+
+@pytest.mark.parametrize("t,n,k", MANY)
+def test_linear_many_tiles(t, n, k):
+    import bigsmall_amd as bs
+    g = _gen(t + n + k)
+    dtype = TYPES[n % 2]
+    x = _x(t, k, dtype, g).cuda()
+    w, ws = _w(n, k, g)
+    weight = bs.Fp8Weight(w.cuda(), ws.cuda())
+    rows = bs.fp8_quantise(x)
+    y = bs.fp8_linear(rows, weight)
+    _check(y, rows, w, ws, dtype, "cuda")
+    for _ in range(3):
+        assert torch.equal(bs.fp8_linear(rows, weight), y)
+
+
 def test_each_block_has_its_scale():
     """Exact numbers: code 1 in one place each, so a result names the scales that made it."""
     import bigsmall_amd as bs
