@@ -3,10 +3,13 @@
 // A sequence's vocabulary is cut into pieces, at most 256 and of 1,024 weights or a multiple. sums_kernel: each workgroup finds the row
 // at which the drafts end (a test a lane; three dependent reads), and each of its waves sums that row's weights over pieces
 // of its own. pick_kernel: a workgroup per sequence finds the piece, then the token at which the running sum passes the given
-// share; it is one wave, so nothing waits at a barrier. A small vocabulary is one workgroup's and one launch. Only that one row of p (and of q where a draft was refused)
-// is read, and one piece of it twice. Sums are f64: with f32 the token drawn would hang on their order wherever the share
-// falls near a border, and a vocabulary has 100,000 of them. They are made in an order that depends on the sizes alone, so
-// the same numbers give the same tokens.
+// share; it is one wave, so nothing waits at a barrier. Small vocabularies and many sequences are one launch: a workgroup of
+// 16 waves for each sequence. Only that one row of p (and of q where a draft was refused) is read, and one piece of it twice. Sums
+// are f64: with f32 the token drawn would hang on their order wherever the share falls near a border, and a vocabulary has
+// 100,000 of them. They are made in an order that depends on the sizes alone, so the same numbers give the same tokens.
+//
+// The bound is memory once there is enough to read: 128 sequences of 128,256 weights, f32, p and q: 20 us for 131 MB, then 6 to pick. One
+// sequence: 4 and 5, a launch and dependent reads each.
 #include <float.h>
 
 #include <algorithm>
@@ -18,7 +21,10 @@ namespace {
 
 constexpr uint32_t THREADS = 256, WAVES = THREADS / 64;
 constexpr uint32_t MOST_PIECES = THREADS, PIECE = 1024;
-constexpr uint32_t ALONE = 8;  // pieces that one workgroup sums and picks from in one launch
+// One launch up to this many pieces, or from this many sequences on (one a compute unit). f32, one / two launches: 16,000 weights
+// 8.6 / 9.9 us for 8 sequences; 32,000 9.9 / 9.1 for 8, 11.9 / 12.9 for 128, and a call is 3 us less of the host's time; 128,256 21.7 / 9.1
+// for 8, 28.5 / 30.0 for 128, 39.7 / 47.9 for 256.
+constexpr uint32_t ALONE_PIECES = 32, ALONE_SEQS = 256, ALONE_THREADS = 1024;
 
 struct Work {
   double* sums;          // [n_seqs][pieces]
@@ -41,10 +47,12 @@ __device__ __forceinline__ float value(const void* p, uint64_t i) {
 
 template <int TYPE>
 __device__ __forceinline__ void values4(const void* p, uint64_t i, float (&v)[4]) {
+  // (rows start at any multiple of a weight's size; loads may too)
   if constexpr (TYPE == BS_DRAFT_F32) {
-    *(float4*)v = *(const float4*)((const float*)p + i);
+    __builtin_memcpy(v, (const float*)p + i, 16);
   } else {
-    const uint2 u = *(const uint2*)((const uint16_t*)p + i);
+    uint2 u;
+    __builtin_memcpy(&u, (const uint16_t*)p + i, 8);
     v[0] = of16<TYPE>(u.x & 0xFFFFu), v[1] = of16<TYPE>(u.x >> 16), v[2] = of16<TYPE>(u.y & 0xFFFFu), v[3] = of16<TYPE>(u.y >> 16);
   }
 }
@@ -58,18 +66,16 @@ struct Row {
   const void *p, *q;  // the row; q NULL: not taken off
   uint32_t vocab;
   int64_t without;    // the token left out, -1: none
-  bool wide;          // four weights can be read at once
   __device__ Row(const bs_draft_batch& D, uint64_t row, bool refused) : vocab(D.vocab), without(refused && !D.q ? D.draft[row] : -1) {
     const uint32_t size = TYPE == BS_DRAFT_F32 ? 4 : 2;
     p = (const uint8_t*)D.p + row * (uint64_t)D.p_stride * size;
     q = refused && D.q ? (const uint8_t*)D.q + row * (uint64_t)D.q_stride * size : nullptr;
-    wide = (((uintptr_t)p | (uintptr_t)q) & (4 * size - 1)) == 0;
   }
   __device__ __forceinline__ double of(uint32_t j, float a, float b) const { return (int64_t)j == without ? 0.0 : weight((double)a - (double)b); }
   // w(j) .. w(j + 3), 0 past the end
   __device__ __forceinline__ void four(uint32_t j, double (&w)[4]) const {
     float a[4] = {}, b[4] = {};
-    if (wide && j + 4 <= vocab) {
+    if (j + 4 <= vocab) {
       values4<TYPE>(p, j, a);
       if (q) values4<TYPE>(q, j, b);
     } else {
@@ -224,10 +230,10 @@ __device__ bool pick(const Row<TYPE>& w, const Work& W, const double* sums, doub
   return true;
 }
 
-// LONE: the pieces' sums are made here too, by four waves; else one wave.
+// LONE: the pieces' sums are made here too, by all waves; else there is one.
 template <int TYPE, bool LONE>
-__global__ __launch_bounds__(LONE ? THREADS : 64) void pick_kernel(bs_draft_batch D, Work W, int32_t* status) {
-  __shared__ double sums[LONE ? ALONE : MOST_PIECES];
+__global__ __launch_bounds__(LONE ? ALONE_THREADS : 64) void pick_kernel(bs_draft_batch D, Work W, int32_t* status) {
+  __shared__ double sums[MOST_PIECES];
   const uint32_t b = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int32_t a = LONE ? taken_drafts<TYPE>(D, b, wave == 0 ? status : nullptr) : W.taken[b];
   const int32_t r0 = D.cu[b], row = r0 + a;
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(LONE ? THREADS : 64) void pick_kernel(bs_draft_batc
   if (a < 0) return;
   const Row<TYPE> w(D, (uint64_t)row, row + 1 < D.cu[b + 1]);
   if constexpr (LONE) {
-    for (uint32_t piece = wave; piece < W.pieces; piece += WAVES) {
+    for (uint32_t piece = wave; piece < W.pieces; piece += ALONE_THREADS / 64) {
       const double sum = piece_sum(w, piece, W.len);
       if (lane == 0) sums[piece] = sum;
     }
@@ -273,10 +279,12 @@ Work layout(uint32_t n_seqs, uint32_t vocab, void* d_work) {
   return w;
 }
 
+bool alone(uint32_t n_seqs, uint32_t pieces) { return pieces <= ALONE_PIECES || n_seqs >= ALONE_SEQS; }
+
 template <int TYPE>
 int launch(const bs_draft_batch& D, const Work& w, int32_t* status, hipStream_t s) {
-  if (w.pieces <= ALONE) {
-    pick_kernel<TYPE, true><<<D.n_seqs, THREADS, 0, s>>>(D, w, status);
+  if (alone(D.n_seqs, w.pieces)) {
+    pick_kernel<TYPE, true><<<D.n_seqs, ALONE_THREADS, 0, s>>>(D, w, status);
   } else {
     sums_kernel<TYPE><<<D.n_seqs * w.groups, THREADS, 0, s>>>(D, w, status);
     pick_kernel<TYPE, false><<<D.n_seqs, 64, 0, s>>>(D, w, status);
@@ -288,7 +296,7 @@ int launch(const bs_draft_batch& D, const Work& w, int32_t* status, hipStream_t 
 
 extern "C" uint64_t bs_draft_verify_work_bytes(uint32_t n_seqs, uint32_t vocab) {
   const uint32_t pieces = layout(n_seqs, vocab, nullptr).pieces;
-  return pieces <= ALONE ? 0 : (uint64_t)n_seqs * (pieces * 8ull + 4ull);
+  return alone(n_seqs, pieces) ? 0 : (uint64_t)n_seqs * (pieces * 8ull + 4ull);
 }
 
 extern "C" int bs_draft_verify(const bs_draft_batch* D, void* d_work, uint64_t work_bytes, int32_t* d_status, void* stream) {

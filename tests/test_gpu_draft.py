@@ -101,6 +101,25 @@ def test_borders_of_pieces(vocab, model):
         _same(_run(t, d), reference(**t, max_drafts=d))
 
 
+@pytest.mark.parametrize("seqs,vocab", [(3, 32767), (3, 32768), (4, 32769), (3, 33793), (5, 33794), (4, 33795), (255, 32801), (256, 32801), (300, 34000), (258, 1030)])
+def test_one_launch_or_two(seqs, vocab):
+    """Sizes on both sides of where one workgroup takes a sequence by itself; rows that start anywhere; alone as beside others."""
+    import bigsmall_amd as bs
+    dtype = TYPES[seqs % 3]
+    c, d = _case(seqs, 1, vocab, dtype, True, seqs + vocab, spread=1.0)
+    got = _run(c, d)
+    _same(got, reference(**c, max_drafts=d))
+    off = {k: torch.empty(c[k].numel() + 3, dtype=dtype, device="cuda")[i:].narrow(0, 0, c[k].numel()).view(c[k].shape) for k, i in (("p", 1), ("q", 3))}
+    for k in off:
+        off[k].copy_(c[k])
+    rest = {k: v.cuda() for k, v in c.items() if k not in "pq"}
+    _same(bs.draft_verify(p=off["p"], q=off["q"], max_drafts=d, **rest), [x.cpu() for x in got])
+    lo, hi = int(c["cu"][1]), int(c["cu"][2])
+    one = dict({k: v[lo:hi] for k, v in c.items() if k not in ("cu", "pick")}, cu=torch.tensor([0, hi - lo], dtype=torch.int32), pick=c["pick"][1:2])
+    tokens, counts = _run(one, d)
+    assert torch.equal(tokens[0], got[0][1]) and int(counts[0]) == int(got[1][1])
+
+
 def test_picks_at_both_ends_and_between_equal_weights():
     """Dyadic weights: all sums are exact, so borders are hit exactly; a border belongs to the token after it."""
     vocab = 9000
