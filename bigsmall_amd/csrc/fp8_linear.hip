@@ -621,6 +621,7 @@ __global__ __launch_bounds__(Large::THREADS, 2) void large_kernel(Args A) {
       for (uint32_t c = 0; c < S::TT; ++c) sum[i][c] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (uint32_t i = 0; i <= S::LAG; ++i) d[i] = f32x4{0, 0, 0, 0};
+    s[3] = 0;  // (of the products before: it may be no number)
   }
   wait_loads<0>();
 }

@@ -191,6 +191,24 @@ def test_what_is_not_finite_stays_in_its_row(t):
     assert float(bs.fp8_linear(torch.zeros(t, 500, dtype=torch.float16).cuda(), weight).abs().max()) == 0
 
 
+@pytest.mark.parametrize("t,n,k", [(8192, 4096, 128), (4350, 4608, 384), (1300, 4700, 300), (1300, 4700, 600)])
+def test_what_is_not_finite_stays_in_its_tile(t, n, k):
+    """Rows that are no numbers in every group of 16 of some tiles; workgroups that go on with another tile leave them behind."""
+    import bigsmall_amd as bs
+    g = _gen(t + k)
+    x = _x(t, k, torch.bfloat16, g)
+    w, ws = _w(n, k, g)
+    weight = bs.Fp8Weight(w.cuda(), ws.cuda())
+    want = bs.fp8_linear(x.cuda(), weight)
+    bad = torch.zeros(t, dtype=torch.bool)
+    for first in (0, 256, 1024, t - 40):
+        bad[first:first + 256:5] = True
+    x[bad, k - 1] = math.inf
+    x[bad & (torch.arange(t) % 2 == 0), 0] = math.nan
+    y = bs.fp8_linear(x.cuda(), weight).cpu()
+    assert bool(y[bad].isnan().all()) and torch.equal(y[~bad], want.cpu()[~bad])
+
+
 @pytest.mark.parametrize("t", [1, 20, 150])
 def test_strides_and_shapes(t):
     import bigsmall_amd as bs
