@@ -2,8 +2,7 @@
 //
 // bs_fp8_quantise: sixteen lanes hold a block of 128 columns, eight each; the largest
 // |x| goes round among them and gives the scale. The bound is memory: two bytes in, one out: 8,192 rows of 4,096 in 20 us, 5.1 TB/s,
-// as a large copy; a few rows 4 to 5, a launch and one read. (A workgroup has 16 rows by 4 blocks, so that all of a lane's reads
-// are under way before the first maximum.)
+// as a large copy; 64 rows 2.8, a launch and one read. (A lane with four blocks, read together: 4.2 for 64 rows, the same for 8,192.)
 //
 // bs_fp8_linear: one matrix instruction multiplies 16 rows of the weight by 16 rows of x over
 // a whole block of 128 columns, so its result is scaled in registers (the row's scale times the
@@ -50,7 +49,7 @@ __device__ __forceinline__ uint16_t store16(float x) {
 
 // ---- quantising
 
-constexpr uint32_t Q_THREADS = 256, Q_ROWS = Q_THREADS / 16, Q_BLOCKS = 4;  // of one workgroup
+constexpr uint32_t Q_THREADS = 256, Q_ROWS = Q_THREADS / 16;  // of one workgroup: a block of 16 rows
 
 // Blocks with an |x| below this are scaled as if they had it: scales and their inverses stay normal f32 numbers.
 constexpr float AMAX_LO = 0x1p-100f;
@@ -115,27 +114,17 @@ __device__ __forceinline__ uint2 quantise_block(const Eight& x, float& scale) {
 
 template <int TYPE, bool WIDE>
 __global__ __launch_bounds__(Q_THREADS) void quantise_kernel(const uint16_t* x, int64_t x_stride, bs_fp8_rows R) {
-  const uint32_t lane = threadIdx.x % 16, blocks = R.code_stride / BLOCK;
+  const uint32_t lane = threadIdx.x % 16, j = blockIdx.x, k = j * BLOCK + lane * 8;
   const uint64_t t = (uint64_t)blockIdx.y * Q_ROWS + threadIdx.x / 16;
   if (t >= R.rows) return;
-  const uint16_t* row = x + (int64_t)t * x_stride;
-  const uint32_t j0 = blockIdx.x * Q_BLOCKS;
-  Eight v[Q_BLOCKS];
-#pragma unroll
-  for (uint32_t i = 0; i < Q_BLOCKS; ++i) v[i] = load_eight<WIDE>(row, (j0 + i) * BLOCK + lane * 8, R.cols);
-#pragma unroll
-  for (uint32_t i = 0; i < Q_BLOCKS; ++i) {
-    const uint32_t j = j0 + i;
-    if (j >= blocks) break;
-    float scale;
-    *(uint2*)(R.codes + t * R.code_stride + j * BLOCK + lane * 8) = quantise_block<TYPE>(v[i], scale);
-    if (lane == 0) R.scales[(uint64_t)j * R.scale_stride + t] = scale;
-  }
+  float scale;
+  *(uint2*)(R.codes + t * R.code_stride + k) = quantise_block<TYPE>(load_eight<WIDE>(x + (int64_t)t * x_stride, k, R.cols), scale);
+  if (lane == 0) R.scales[(uint64_t)j * R.scale_stride + t] = scale;
 }
 
 template <int TYPE>
 int quantise_launch(const void* x, int64_t stride, const bs_fp8_rows& R, hipStream_t s) {
-  const dim3 grid((R.code_stride / BLOCK + Q_BLOCKS - 1) / Q_BLOCKS, (R.rows + Q_ROWS - 1) / Q_ROWS);
+  const dim3 grid(R.code_stride / BLOCK, (R.rows + Q_ROWS - 1) / Q_ROWS);
   if (((uintptr_t)x & 15) == 0 && stride % 8 == 0)
     quantise_kernel<TYPE, true><<<grid, Q_THREADS, 0, s>>>((const uint16_t*)x, stride, R);
   else
