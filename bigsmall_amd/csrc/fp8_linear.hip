@@ -1,7 +1,7 @@
 // Products of e4m3 weights with a scale for each block of 128.
 //
 // bs_fp8_quantise: sixteen lanes hold a block of 128 columns, eight each; the largest
-// |x| goes round among them and gives the scale. The bound is memory: two bytes in, one out: 8,192 rows of 4,096 in 20 us, 5.1 TB/s,
+// |x| goes round among them and gives the scale. The bound is memory: two bytes in, one out: 8,192 rows of 4,096 in 18 to 20 us, 5.2 TB/s,
 // as a large copy; 64 rows 2.8, a launch and one read. (A lane with four blocks, read together: 4.2 for 64 rows, the same for 8,192.)
 //
 // bs_fp8_linear: one matrix instruction multiplies 16 rows of the weight by 16 rows of x over
@@ -765,9 +765,10 @@ __global__ __launch_bounds__(V_THREADS) void values_kernel(Args A, const uint16_
   join_waves<1, 1, V_WAVES>(lds, wave, sum, A, n0, 0);
 }
 
-// Up to this many blocks of x. One row through 4,096 x 4,096: 7.4 us, quantised by a kernel of its own 10.5; four (128
-// blocks) 9.6 and 10.5, eight 13.0 and 11.0; one row of 14,336 columns 15.7 and 16.
-constexpr uint32_t V_BLOCKS = 128;
+// Up to this many blocks of x and rows of the weight (a workgroup a compute unit). One row through 4,096 x 4,096: 6.5 us, quantised
+// by a kernel of its own 8.3; three (96 blocks) 7.9 and 8.5, four 8.9 and 8.4; one row of 14,336 columns 15.3 and 14.0; one through
+// 14,336 x 4,096 13.1 and 13.8, through 16,384 x 2,048 12.0 and 10.7.
+constexpr uint32_t V_BLOCKS = 96, V_OUTER = 4096;
 
 template <int TYPE>
 int values_launch(const Args& A, const void* x, int64_t x_stride, hipStream_t s) {
@@ -856,7 +857,7 @@ bool weight_ok(const bs_fp8_weight* w) {
          w->scales && ((uintptr_t)w->scales & 3) == 0;
 }
 
-bool few_values(uint32_t rows, const bs_fp8_weight& w) { return rows <= 16 && rows * ((w.inner + BLOCK - 1) / BLOCK) <= V_BLOCKS; }
+bool few_values(uint32_t rows, const bs_fp8_weight& w) { return rows <= 16 && w.outer <= V_OUTER && rows * ((w.inner + BLOCK - 1) / BLOCK) <= V_BLOCKS; }
 
 // Codes and scales of values in the work area, scales first.
 uint64_t scale_bytes(uint32_t rows, const bs_fp8_weight& w) { return ((uint64_t)rows * ((w.inner + BLOCK - 1) / BLOCK) * 4 + 15) / 16 * 16; }

@@ -130,8 +130,7 @@ class PagedLlama:
             if w.dtype == torch.float8_e4m3fn:
                 if name + ".weight_scale_inv" not in layer:
                     raise ValueError(f"PagedLlama: {name} is held in fp8 without {name}.weight_scale_inv")
-                # few rows are quantised on the way
-                rows = (x if len(names) == 1 or x.shape[0] <= 4 else fp8_quantise(x)) if rows is None else rows
+                rows = (x if len(names) == 1 else fp8_quantise(x)) if rows is None else rows
                 out.append(fp8_linear(rows, Fp8Weight(w, layer[name + ".weight_scale_inv"])))
             else:
                 out.append(linear(x, w))
