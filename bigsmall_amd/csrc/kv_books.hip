@@ -4,7 +4,8 @@
 // of those before its own, and of all, since a step is made whole or not at all) and then writes what belongs to its
 // own sequences: nothing passes between workgroups, so it is one launch, and the books stay as they were, so it can be
 // made again. The bound of the usual step is the launch and three dependent reads (place, length, page): 128 sequences of
-// up to 16,383 tokens, 5 new ones each, 6 us for 131 KB of tables; 32 prompts of up to 8,192 tokens 7 us for 2 MB of rows.
+// up to 16,383 tokens, 5 new ones each, 5 us for 131 KB of tables; 32 prompts of up to 8,192 tokens 6 us for 2 MB of rows.
+// (The counts one after another over the workgroup, and a sequence looked up again for its tables: 6 and 7.)
 //
 // keep_kernel enters a step into the books: 3 us, a launch and two dependent reads. drop is one workgroup for a few places, else two
 // launches: pages go onto the stack while lengths still stand, then the places are emptied.
@@ -17,22 +18,39 @@ namespace {
 using namespace bs_kv;
 
 constexpr uint32_t THREADS = 256, WAVES = THREADS / 64, MOST_PLACES = 65536;
+// Workgroups count all sequences each, so beyond 512 of them they take several sequences.
+constexpr uint32_t MOST_GROUPS = 512;
 
-__device__ __forceinline__ int64_t wave_total(int64_t x) {
+// Sums of N numbers over the workgroup, side by side, and the bits of `bits` that any thread has.
+template <int N>
+struct Totals {
+  int64_t sum[WAVES][N];
+  int bits[WAVES];
+};
+template <int N>
+__device__ int totals(int64_t (&x)[N], int bits, Totals<N>& lds) {
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
-  return x;
-}
-
-// The sum over the workgroup.
-__device__ int64_t block_total(int64_t x, int64_t* lds) {
-  x = wave_total(x);
+  for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] += __shfl_xor(x[i], d);
+  const int any = (__ballot(bits & BS_DEV_ERR_BOUNDS) ? BS_DEV_ERR_BOUNDS : 0) | (__ballot(bits & BS_DEV_ERR_COUNT) ? BS_DEV_ERR_COUNT : 0);
+  const uint32_t wave = threadIdx.x / 64;
+  if (threadIdx.x % 64 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) lds.sum[wave][i] = x[i];
+    lds.bits[wave] = any;
+  }
   __syncthreads();
-  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = x;
-  __syncthreads();
-  int64_t sum = 0;
-  for (uint32_t w = 0; w < WAVES; ++w) sum += lds[w];
-  return sum;
+  int all = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = 0;
+#pragma unroll
+  for (uint32_t w = 0; w < WAVES; ++w) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] += lds.sum[w][i];
+    all |= lds.bits[w];
+  }
+  return all;
 }
 
 // What a step wants of one sequence.
@@ -73,26 +91,27 @@ __device__ Want want(const bs_kv_books& K, const bs_kv_tables& S, const int32_t*
 __global__ __launch_bounds__(THREADS) void step_kernel(bs_kv_books K, bs_kv_tables S, const int32_t* d_new, const int32_t* d_sure,
                                                        uint32_t each, int32_t* status) {
   __shared__ uint32_t seen[MOST_PLACES / 32];
-  __shared__ int64_t lds[WAVES];
+  __shared__ Totals<4> lds;
+  __shared__ Want own[MOST_PLACES / MOST_GROUPS];
   const uint32_t tid = threadIdx.x, first = blockIdx.x * each, last = min(S.n_seqs, first + each);
   for (uint32_t i = tid; i < (K.n_places + 31) / 32; i += THREADS) seen[i] = 0;
   __syncthreads();
-  int64_t rows = 0, pages = 0, rows_before = 0, pages_before = 0;
+  int64_t sums[4] = {0, 0, 0, 0};  // rows and pages, and those of the sequences before this workgroup's
+  const int32_t n_free = *K.n_free;
   int bad = 0;
   for (uint32_t b = tid; b < S.n_seqs; b += THREADS) {
     const Want w = want(K, S, d_new, d_sure, b);
     bad |= w.bad;
-    rows += w.n, pages += w.pages;
-    if (b < first) rows_before += w.n, pages_before += w.pages;
+    sums[0] += w.n, sums[1] += w.pages;
+    if (b < first) sums[2] += w.n, sums[3] += w.pages;
+    if (b >= first && b < last) own[b - first] = w;
     if (!(w.bad & BS_DEV_ERR_BOUNDS)) {
       const uint32_t bit = 1u << (w.place % 32);
       if (atomicOr(&seen[w.place / 32], bit) & bit) bad |= BS_DEV_ERR_BOUNDS;
     }
   }
-  const int32_t n_free = *K.n_free;
-  rows = block_total(rows, lds), pages = block_total(pages, lds);
-  rows_before = block_total(rows_before, lds), pages_before = block_total(pages_before, lds);
-  bad = (block_total(bad & BS_DEV_ERR_BOUNDS, lds) ? BS_DEV_ERR_BOUNDS : 0) | (block_total(bad & BS_DEV_ERR_COUNT, lds) ? BS_DEV_ERR_COUNT : 0);
+  bad = totals(sums, bad, lds);
+  int64_t rows = sums[0], pages = sums[1], rows_before = sums[2], pages_before = sums[3];
   if (n_free < 0 || n_free > (int32_t)K.n_pages) bad |= BS_DEV_ERR_BOUNDS;
   if (rows > (int64_t)S.n_rows || pages > (int64_t)n_free) bad |= BS_DEV_ERR_COUNT;
   if (bad && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) report(status, bad);
@@ -102,7 +121,7 @@ __global__ __launch_bounds__(THREADS) void step_kernel(bs_kv_books K, bs_kv_tabl
   const uint32_t strip = blockIdx.y * THREADS + tid, strips = gridDim.y * THREADS;
   int32_t at = (int32_t)rows_before, from = n_free - 1 - (int32_t)pages_before;
   for (uint32_t b = first; b < last; ++b) {
-    const Want w = want(K, S, d_new, d_sure, b);
+    const Want w = own[b - first];
     const int32_t n = bad ? 0 : w.n, taken = bad ? 0 : w.pages, held = w.start / (int32_t)PAGE;
     const bool place = (uint32_t)w.place < K.n_places;
     if (strip == 0) {
@@ -112,10 +131,10 @@ __global__ __launch_bounds__(THREADS) void step_kernel(bs_kv_books K, bs_kv_tabl
       S.tails[2 * (size_t)b] = tail + which;
       S.tails[2 * (size_t)b + 1] = tail + (taken ? which ^ 1 : which);
     }
-    const int32_t* own = K.table + (size_t)(place ? w.place : 0) * K.cols;
+    const int32_t* held_pages = K.table + (size_t)(place ? w.place : 0) * K.cols;
     int32_t* row = S.table + (size_t)b * K.cols;
     for (int32_t c = (int32_t)strip; c < (int32_t)K.cols; c += (int32_t)strips)
-      row[c] = c < held ? own[c] : c < held + taken ? K.free[from - (c - held)] : 0;
+      row[c] = c < held ? held_pages[c] : c < held + taken ? K.free[from - (c - held)] : 0;
     for (int32_t i = (int32_t)strip; i < n; i += (int32_t)strips) {
       S.owner[at + i] = (int32_t)b;
       S.position[at + i] = w.start + i;
@@ -129,16 +148,16 @@ __global__ __launch_bounds__(THREADS) void step_kernel(bs_kv_books K, bs_kv_tabl
 }
 
 __global__ __launch_bounds__(THREADS) void keep_kernel(bs_kv_books K, bs_kv_tables S, const int32_t* d_sure, const int32_t* d_kept) {
-  __shared__ int64_t lds[WAVES];
+  __shared__ Totals<1> lds;
   const uint32_t tid = threadIdx.x;
   if (blockIdx.x == S.n_seqs) {  // one more workgroup for the stack
-    int64_t pages = 0;
+    int64_t pages[1] = {0};
     for (uint32_t b = tid; b < S.n_seqs; b += THREADS) {
       const int32_t start = S.start[b], end = start + S.cu[b + 1] - S.cu[b];
-      pages += end / (int32_t)PAGE - start / (int32_t)PAGE;
+      pages[0] += end / (int32_t)PAGE - start / (int32_t)PAGE;
     }
-    pages = block_total(pages, lds);
-    if (tid == 0) *K.n_free -= (int32_t)pages;
+    totals(pages, 0, lds);
+    if (tid == 0) *K.n_free -= (int32_t)pages[0];
     return;
   }
   const uint32_t b = blockIdx.x;
@@ -157,36 +176,36 @@ __global__ __launch_bounds__(THREADS) void keep_kernel(bs_kv_books K, bs_kv_tabl
 
 // Pages of the places before `first`, and of all; 0 and an error's bit if the places are not to be dropped together.
 __device__ int count_pages(const bs_kv_books& K, const int32_t* seqs, uint32_t n_seqs, uint32_t first, int64_t& before, int64_t& total,
-                           uint32_t* seen, int64_t* lds) {
+                           uint32_t* seen, Totals<2>& lds) {
   const uint32_t tid = threadIdx.x;
   for (uint32_t i = tid; i < (K.n_places + 31) / 32; i += THREADS) seen[i] = 0;
   __syncthreads();
   int bad = 0;
-  before = total = 0;
+  int64_t sums[2] = {0, 0};
+  const int32_t n_free = *K.n_free;
   for (uint32_t b = tid; b < n_seqs; b += THREADS) {
     const uint32_t place = (uint32_t)seqs[b];
     if (place >= K.n_places) {
-      bad = 1;
+      bad = BS_DEV_ERR_BOUNDS;
       continue;
     }
     const uint32_t bit = 1u << (place % 32);
     const int32_t length = K.length[place];
     if ((atomicOr(&seen[place / 32], bit) & bit) || length < 0 || length > (int32_t)(K.cols * PAGE)) {
-      bad = 1;
+      bad = BS_DEV_ERR_BOUNDS;
       continue;
     }
-    total += length / (int32_t)PAGE;
-    if (b < first) before += length / (int32_t)PAGE;
+    sums[0] += length / (int32_t)PAGE;
+    if (b < first) sums[1] += length / (int32_t)PAGE;
   }
-  before = block_total(before, lds), total = block_total(total, lds);
-  const int32_t n_free = *K.n_free;
-  if (n_free < 0 || total + n_free > (int64_t)K.n_pages) bad = 1;
-  return block_total(bad, lds) ? BS_DEV_ERR_BOUNDS : 0;
+  bad = totals(sums, bad, lds);
+  total = sums[0], before = sums[1];
+  return n_free < 0 || total + n_free > (int64_t)K.n_pages ? BS_DEV_ERR_BOUNDS : bad;
 }
 
 __global__ __launch_bounds__(THREADS) void push_kernel(bs_kv_books K, const int32_t* seqs, uint32_t n_seqs, uint32_t each, int32_t* status) {
   __shared__ uint32_t seen[MOST_PLACES / 32];
-  __shared__ int64_t lds[WAVES];
+  __shared__ Totals<2> lds;
   const uint32_t first = blockIdx.x * each, last = min(n_seqs, first + each);
   int64_t before, total;
   if (const int bad = count_pages(K, seqs, n_seqs, first, before, total, seen, lds)) {
@@ -203,7 +222,7 @@ __global__ __launch_bounds__(THREADS) void push_kernel(bs_kv_books K, const int3
 
 __global__ __launch_bounds__(THREADS) void empty_kernel(bs_kv_books K, const int32_t* seqs, uint32_t n_seqs) {
   __shared__ uint32_t seen[MOST_PLACES / 32];
-  __shared__ int64_t lds[WAVES];
+  __shared__ Totals<2> lds;
   int64_t before, total;
   if (count_pages(K, seqs, n_seqs, 0, before, total, seen, lds)) return;
   for (uint32_t b = threadIdx.x; b < n_seqs; b += THREADS) K.length[seqs[b]] = 0, K.which[seqs[b]] = 0;
@@ -272,9 +291,6 @@ bool step_ok(const bs_kv_books* k, const bs_kv_tables* s) {
          (s->n_seqs == 0 || (s->seqs && s->start && s->cu && s->tails && s->table)) &&
          (s->n_rows == 0 || (s->owner && s->position && s->slot && ((uintptr_t)s->slot & 7) == 0));
 }
-
-// Workgroups count all sequences each, so beyond 512 of them they take several sequences.
-constexpr uint32_t MOST_GROUPS = 512;
 
 int done() { return hipGetLastError() == hipSuccess ? BS_OK : BS_ERR_HIP; }
 
