@@ -8,8 +8,8 @@
 // are f64: with f32 the token drawn would hang on their order wherever the share falls near a border, and a vocabulary has
 // 100,000 of them. They are made in an order that depends on the sizes alone, so the same numbers give the same tokens.
 //
-// The bound is memory once there is enough to read: 128 sequences of 128,256 weights, f32, p and q: 20 us for 131 MB, then 6 to pick. One
-// sequence: 4 and 5, a launch and dependent reads each.
+// The bound is memory once there is enough to read: 128 sequences of 128,256 weights, f32, p and q: 18 us for up to 131 MB, then 5 to pick. One
+// sequence: 4 and 4, a launch and dependent reads each.
 #include <float.h>
 
 #include <algorithm>
@@ -161,16 +161,18 @@ __device__ __forceinline__ double lane_of(double x, uint32_t lane) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// In a running sum over the lanes from `before` on, the lane whose x takes it past `share`; if rounding leaves none, the last one with an
-// x above 0. upto: the running sum with this lane's x.
-__device__ __forceinline__ uint32_t passing(double x, double before, double share, double& upto) {
-  upto = x;
+// The running sum over the lanes, with this one's x.
+__device__ __forceinline__ double running(double x) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const double up = __shfl_up(upto, d);
-    if (threadIdx.x % 64 >= (uint32_t)d) upto += up;
+    const double up = __shfl_up(x, d);
+    if (threadIdx.x % 64 >= (uint32_t)d) x += up;
   }
-  upto += before;
+  return x;
+}
+
+// The lane whose x takes the running sum `upto` past `share`; if rounding leaves none, the last one with an x above 0.
+__device__ __forceinline__ uint32_t passing(double x, double upto, double share) {
   const uint64_t some = __ballot(x > 0), past = __ballot(x > 0 && upto > share);
   return past ? (uint32_t)__builtin_ctzll(past) : some ? 63u - (uint32_t)__builtin_clzll(some) : 0u;
 }
@@ -194,12 +196,12 @@ __device__ bool pick(const Row<TYPE>& w, const Work& W, const double* sums, doub
 #pragma unroll
   for (uint32_t e = 0; e < 4; ++e) s[e] = lane * 4 + e < W.pieces ? sums[lane * 4 + e] : 0.0;
   double own = (s[0] + s[1]) + (s[2] + s[3]);
-  const double total = wave_sum(own), share = part * total;
+  double upto = running(own);
+  const double total = lane_of(upto, 63), share = part * total;
   if (!(total > 0)) return false;
-  double upto, run;
-  uint32_t found = passing(own, 0.0, share, upto), at = 0;
+  uint32_t found = passing(own, upto, share), at = 0;
   bool done = false;
-  run = upto - own;
+  double run = upto - own;
   passing4(s, share, run, at, done);
   const uint32_t piece = found * 4 + __builtin_amdgcn_readlane(at, found);
   const double before = lane_of(run, found);
@@ -213,7 +215,8 @@ __device__ bool pick(const Row<TYPE>& w, const Work& W, const double* sums, doub
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) own += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
   }
-  found = passing(own, before, share, upto);
+  upto = running(own) + before;
+  found = passing(own, upto, share);
   run = upto - own, done = false;
   uint32_t last = j0;
   double sum = run;
@@ -238,12 +241,17 @@ __global__ __launch_bounds__(LONE ? ALONE_THREADS : 64) void pick_kernel(bs_draf
   const int32_t a = LONE ? taken_drafts<TYPE>(D, b, wave == 0 ? status : nullptr) : W.taken[b];
   const int32_t r0 = D.cu[b], row = r0 + a;
   int64_t* out = D.tokens + (uint64_t)b * (D.max_drafts + 1);
-  if (wave == 0) {
-    for (uint32_t i = lane; i <= D.max_drafts; i += 64)
-      if ((int32_t)i != a) out[i] = (int32_t)i < a ? D.draft[r0 + (int32_t)i] : -1;
+  // the first drafts are read now and written with the token: waiting for them here would hold up the sums
+  const int64_t early = wave == 0 && (int32_t)lane < a ? D.draft[r0 + (int32_t)lane] : -1;
+  const auto write = [&](uint32_t token) {
+    if (lane <= D.max_drafts) out[lane] = (int32_t)lane == a ? (int64_t)token : early;
+    for (uint32_t i = lane + 64; i <= D.max_drafts; i += 64) out[i] = (int32_t)i < a ? D.draft[r0 + (int32_t)i] : (int32_t)i == a ? (int64_t)token : -1;
     if (lane == 0) D.counts[b] = a + 1;
+  };
+  if (a < 0) {
+    if (wave == 0) write(0);
+    return;
   }
-  if (a < 0) return;
   const Row<TYPE> w(D, (uint64_t)row, row + 1 < D.cu[b + 1]);
   if constexpr (LONE) {
     for (uint32_t piece = wave; piece < W.pieces; piece += ALONE_THREADS / 64) {
@@ -265,7 +273,7 @@ __global__ __launch_bounds__(LONE ? ALONE_THREADS : 64) void pick_kernel(bs_draf
     __builtin_amdgcn_wave_barrier();
     if (!pick(plain, W, sums, (double)D.pick[b], token) && lane == 0 && status) atomicOr(status, BS_DEV_ERR_COUNT);
   }
-  if (lane == 0) out[a] = (int64_t)token;
+  write(token);
 }
 
 Work layout(uint32_t n_seqs, uint32_t vocab, void* d_work) {
