@@ -109,6 +109,16 @@ class StatusWord:
             raise DecodeError(f"{what}: device integrity check failed ({', '.join(names)}; status=0x{v:x})")
 
 
+def status_ptr(status, index: int):
+    """The address of a status word for a C entry on GPU `index`, None for none. ValueError for a word elsewhere (a StatusWord
+    made without a device lies on the host): the kernel would write to an address that is not its GPU's."""
+    if status is None:
+        return None
+    if status.t.get_device() != index:
+        raise ValueError(f"the status word is on {status.t.device}, the call runs on cuda:{index}")
+    return status.t.data_ptr()
+
+
 @dataclass
 class ChunkJob:
     """One BSCK blob to decode: device blob address/length, output address, counts."""

@@ -14,6 +14,7 @@ import struct
 import torch
 
 from . import _native
+from .device import status_ptr
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MOST_DRAFTS = 1024
@@ -82,6 +83,7 @@ def draft_verify(p, draft, cu, accept, pick, q=None, max_drafts=None, status=Non
         max_drafts = min(max(0, t - b), MOST_DRAFTS)
     if not 0 <= max_drafts <= MOST_DRAFTS:
         raise ValueError(f"max_drafts must be 0 to {MOST_DRAFTS}, got {max_drafts}")
+    word = status_ptr(status, index)
     if index < 0:
         raise RuntimeError(f"draft_verify runs on an AMD GPU (MI355X); p is on {p.device}")
     device = p.device
@@ -94,7 +96,7 @@ def draft_verify(p, draft, cu, accept, pick, q=None, max_drafts=None, status=Non
         batch = _BATCH.pack(p.data_ptr(), qp, draft.data_ptr(), accept.data_ptr(), cu.data_ptr(),
                             pick.data_ptr(), tokens.data_ptr(), counts.data_ptr(), p.stride(0), q_stride,
                             _TYPES[p.dtype], t, vocab, b, max_drafts)
-        args = batch, work.data_ptr() if n else 0, n, status.ptr if status else None
+        args = batch, work.data_ptr() if n else 0, n, word
         if index == torch.cuda.current_device():
             rc = L.bs_draft_verify(*args, _stream(index))
         else:

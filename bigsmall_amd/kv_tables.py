@@ -22,6 +22,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
+from .device import status_ptr
 from .paged_kv import PAGE, KVBatch, _tensor
 
 MOST_PLACES = 65536
@@ -133,7 +134,7 @@ class KVTables:
         batch._set(start, cu, table.view(b, cols), tails.view(b, 2), b, cols, cols, max_new, max_len, rows, self.index, start_at, cu_at,
                    table_at, tails_at)
         c = _TABLES.pack(seqs.data_ptr(), start_at, cu_at, tails_at, table_at, owner_at, owner_at + 4 * rows, at, b, rows, max_new)
-        self._call("bs_kv_books_step", c, new.data_ptr(), sure.data_ptr() if sure is not None else 0, status.ptr if status else None)
+        self._call("bs_kv_books_step", c, new.data_ptr(), sure.data_ptr() if sure is not None else 0, status_ptr(status, self.index))
         self._made = (batch, c, seqs, sure)
         return batch, StepRows(owner, position, slot.view(torch.int64))
 
@@ -155,8 +156,9 @@ class KVTables:
         seqs = self._vector("seqs", seqs)
         if seqs.shape[0] > self.places:
             raise ValueError(f"{seqs.shape[0]} places; the tables have {self.places}")
+        word = status_ptr(status, self.index)
         self._made = None
-        self._call("bs_kv_books_drop", seqs.data_ptr(), seqs.shape[0], status.ptr if status else None)
+        self._call("bs_kv_books_drop", seqs.data_ptr(), seqs.shape[0], word)
 
     def lent_by(self, give_back) -> None:
         """give_back() is called by close()."""

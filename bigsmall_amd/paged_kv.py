@@ -33,6 +33,7 @@ from typing import Optional
 import torch
 
 from . import _native
+from .device import status_ptr
 
 PAGE = 64
 HEAD_DIMS = (64, 80, 96, 128, 256)
@@ -277,7 +278,7 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
         _refuse_grad()
     if t:
         _call("bs_kv_append", pool, batch.with_rows(t), _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
-              status.ptr if status else None)
+              status_ptr(status, pool.index))
     return result
 
 
@@ -311,14 +312,14 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((t, heads), dtype=torch.float32, device=q.device) if return_lse else None
     if t:
-        step = batch.with_rows(t)
+        step, word = batch.with_rows(t), status_ptr(status, pool.index)
         n = _native.lib().bs_kv_attend_work_bytes(pool.ref, step, heads)
         work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         if softcap:               # (what f32 can hold; the library takes what lies outside for these)
             softcap = min(max(softcap, 2.0 ** -60), 2.0 ** 60)
         query = _QUERY.pack(qp, out.data_ptr(), lse.data_ptr() if return_lse else 0, sp, pp, fp, q0, q1, heads, window,
                             pool.head_dim ** -0.5 if scale is None else scale, softcap)
-        _call("bs_kv_attend", pool, step, query, work.data_ptr() if n else 0, n, status.ptr if status else None)
+        _call("bs_kv_attend", pool, step, query, work.data_ptr() if n else 0, n, word)
     return (out, lse) if return_lse else out
 
 
@@ -342,7 +343,7 @@ def kv_read(pool: KVPool, pages, n: int, tail, status=None):
         raise ValueError(f"kv_read: {n} tokens need {n // PAGE} full pages, {shape[0]} given")
     k = torch.empty((pool.n_kv_heads, n, pool.head_dim), dtype=torch.bfloat16, device=pool.device)
     v = torch.empty_like(k)
-    _call("bs_kv_read", pool, pages.data_ptr(), shape[0], tail.data_ptr(), n, k.data_ptr(), v.data_ptr(), status.ptr if status else None)
+    _call("bs_kv_read", pool, pages.data_ptr(), shape[0], tail.data_ptr(), n, k.data_ptr(), v.data_ptr(), status_ptr(status, pool.index))
     return k, v
 
 
