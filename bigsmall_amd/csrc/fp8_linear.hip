@@ -289,6 +289,9 @@ __device__ __forceinline__ void store_tile(uint8_t* own, const f32x4 (&sum)[NT][
       const uint32_t t = c * 16 + lane % 16, u = i * 4 + lane / 16;
       *(uint2*)(own + t * ROW + ((u / 2) ^ (t % QS)) * 16 + u % 2 * 8) = pack4<TYPE>(sum[i][c]);
     }
+  // other lanes of the wave read it: LDS keeps a wave's order, and this the compiler's
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
   const bool wide = (((uintptr_t)A.y | (uint64_t)A.y_stride * 2) & 15) == 0;
 #pragma unroll 4
   for (uint32_t k = lane; k < TT * 16 * QS; k += 64) {
