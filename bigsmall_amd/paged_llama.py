@@ -160,7 +160,8 @@ class PagedLlama:
         tokens int64 [sequences, ...], of which row i begins with the lengths[i] (int32) tokens so far; ids int64
         [sequences, n], and the probabilities [sequences, n, vocab] (f32) that they were drawn from, or None if they were
         not drawn. Up to `drafts` of them are computed in one step; what comes out is distributed as without drafts (greedy:
-        the same tokens, as far as steps of more rows round alike)."""
+        the same tokens, as far as steps of more rows round alike). RuntimeError where a row that a token is drawn from has no
+        probability at all."""
         if draft is not None or temperature:
             return self._generate_drafted(prompts, max_new_tokens, draft, drafts, temperature, generator)
         seqs = []
@@ -201,7 +202,7 @@ class PagedLlama:
             raise ValueError("a prompt holds ids that are no tokens")
         longest = max(len(t) for t in ids) + max_new_tokens
         places = torch.arange(b, dtype=torch.int32, device=dev)
-        status = StatusWord(dev)
+        status, drawn = StatusWord(dev), StatusWord(dev)
 
         def i32(x):
             return torch.tensor(x, dtype=torch.int32, device="cpu").to(dev)
@@ -215,6 +216,12 @@ class PagedLlama:
                 raise RuntimeError(f"PagedLlama.generate: {tables.free.shape[0]} pages do not hold {b} sequences of up to {longest} tokens")
             return step, at
 
+        def numbers(counts):
+            *n, nothing = torch.cat([counts, drawn.t]).tolist()
+            if nothing:
+                raise RuntimeError("PagedLlama.generate: the model's logits leave no probability to draw from (they hold a NaN or an infinity)")
+            return n
+
         with self.cache.tables(b, longest) as tables:
             tokens = torch.zeros(b, tables.longest + drafts + 1, dtype=torch.int64, device=dev)   # (room for what is cut off at the end)
             row = torch.arange(b, device=dev)
@@ -225,11 +232,11 @@ class PagedLlama:
             tables.keep(step)
             p = self._probabilities(self._logits(x[step.cu[1:].long() - 1]), temperature)
             every = torch.arange(b + 1, dtype=torch.int32, device=dev)
-            new, _ = draft_verify(p, torch.zeros(b, dtype=torch.int64, device=dev), every, rand(b), rand(b), max_drafts=0)
+            new, counts = draft_verify(p, torch.zeros(b, dtype=torch.int64, device=dev), every, rand(b), rand(b), max_drafts=0, status=drawn)
             lengths = i32(lens)                         # tokens so far, the last of which is not in the cache yet
             tokens[row, lengths.long()] = new[:, 0]
             lengths = lengths + 1
-            made = [1] * b
+            made = numbers(counts)
             while min(made) < max_new_tokens:
                 left = [max_new_tokens - m for m in made]
                 n = min(drafts, max(left) - 1)
@@ -250,13 +257,13 @@ class PagedLlama:
                 x = self._hidden(step, given[owner, place])
                 p = self._probabilities(self._logits(x), temperature)
                 q = q[owner, place.clamp(max=n - 1)].float() if q is not None else None
-                new, counts = draft_verify(p, given[owner, place + 1], step.cu, rand(len(owner)), rand(b), q=q, max_drafts=n)
+                new, counts = draft_verify(p, given[owner, place + 1], step.cu, rand(len(owner)), rand(b), q=q, max_drafts=n, status=drawn)
                 tables.keep(step, counts)               # the last token and the drafts that were taken
                 to = lengths[:, None].long() + torch.arange(1 + n, device=dev)
                 kept = torch.arange(1 + n, device=dev) < counts[:, None]
                 tokens[row[:, None].expand_as(to)[kept], to[kept]] = new[kept]
                 lengths = lengths + counts
-                made = [min(max_new_tokens, m + c) for m, c in zip(made, counts.tolist())]
+                made = [min(max_new_tokens, m + c) for m, c in zip(made, numbers(counts))]
             return [tokens[i, k:k + max_new_tokens].clone() for i, k in enumerate(lens)]
 
     def park(self, seq: int, store) -> None:
