@@ -24,7 +24,7 @@ import torch
 from torch.nn.functional import linear, silu
 
 from .device import StatusWord
-from .draft import draft_verify
+from .draft import MOST_DRAFTS, draft_verify
 from .fp8 import BLOCK, Fp8Weight, fp8_linear, fp8_quantise
 from .paged_kv import PagedKVCache, Rope
 
@@ -159,7 +159,7 @@ class PagedLlama:
         draft: a callable (tokens, lengths, n) -> (ids, probabilities) that guesses the next n tokens of each sequence from
         tokens int64 [sequences, ...], of which row i begins with the lengths[i] (int32) tokens so far; ids int64
         [sequences, n], and the probabilities [sequences, n, vocab] (f32) that they were drawn from, or None if they were
-        not drawn. Up to `drafts` of them are computed in one step; what comes out is distributed as without drafts (greedy:
+        not drawn. Up to `drafts` of them, and 1,024, are computed in one step; what comes out is distributed as without drafts (greedy:
         the same tokens, as far as steps of more rows round alike). RuntimeError where a row that a token is drawn from has no
         probability at all."""
         if draft is not None or temperature:
@@ -191,6 +191,7 @@ class PagedLlama:
             drafts = 0
         if drafts < 0 or not 0.0 <= temperature < float("inf"):
             raise ValueError(f"drafts {drafts} and temperature {temperature} must not be negative or infinite")
+        drafts = min(drafts, MOST_DRAFTS)
         if not prompts or max_new_tokens < 1:
             return [torch.empty(0, dtype=torch.int64) for _ in prompts]
         b, dev = len(prompts), self.device

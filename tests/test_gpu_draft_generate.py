@@ -45,3 +45,26 @@ def test_rows_without_any_probability_are_an_error(loaded, draft, at, value):
     with pytest.raises(RuntimeError, match="no probability"):
         m.generate(prompts, 10, temperature=0.7, draft=draft, generator=torch.Generator(device="cuda").manual_seed(1))
     assert len(calls) == at + 1 and m.cache.free_pages() == 8
+
+
+class _Enough(Exception):
+    pass
+
+
+@pytest.mark.parametrize("drafts", [1025, 1 << 40])
+def test_more_drafts_than_a_step_takes(loaded, drafts):
+    """As many are asked for as one verification takes, and room is made for no more."""
+    m = loaded(pages=24, sequences=1)
+    asked = []
+
+    def draft(tokens, lengths, n):
+        asked.append((n, tokens.shape[1]))
+        raise _Enough
+
+    with pytest.raises(_Enough):
+        m.generate([torch.arange(30)], 1200, draft=draft, drafts=drafts)
+    assert asked[0][0] == 1024 and asked[0][1] <= 30 + 1200 + 63 + 1025
+    asked.clear()
+    with pytest.raises(_Enough):
+        m.generate([torch.arange(30)], 8, draft=draft, drafts=drafts)
+    assert asked[0][0] == 6           # of 8 tokens the prompt gave the first, and a step draws its last one itself
