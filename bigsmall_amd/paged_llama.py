@@ -26,7 +26,7 @@ from torch.nn.functional import linear, silu
 from .device import StatusWord
 from .draft import MOST_DRAFTS, draft_verify
 from .fp8 import BLOCK, Fp8Weight, fp8_linear, fp8_quantise
-from .paged_kv import PagedKVCache, Rope
+from .paged_kv import PAGE, PagedKVCache, Rope
 
 
 _TOP = {"model.embed_tokens.weight", "model.norm.weight", "lm_head.weight"}
@@ -161,7 +161,7 @@ class PagedLlama:
         [sequences, n], and the probabilities [sequences, n, vocab] (f32) that they were drawn from, or None if they were
         not drawn. Up to `drafts` of them, and 1,024, are computed in one step; what comes out is distributed as without drafts (greedy:
         the same tokens, as far as steps of more rows round alike). RuntimeError where a row that a token is drawn from has no
-        probability at all."""
+        probability at all, or the cache has too few pages free; what the sequences do not need stays free meanwhile."""
         if draft is not None or temperature:
             return self._generate_drafted(prompts, max_new_tokens, draft, drafts, temperature, generator)
         seqs = []
@@ -202,6 +202,8 @@ class PagedLlama:
         if not 0 <= int(flat.min()) <= int(flat.max()) < self.embed.shape[0]:
             raise ValueError("a prompt holds ids that are no tokens")
         longest = max(len(t) for t in ids) + max_new_tokens
+        # the last token is not cached, and drafts that are taken back complete no page: the rest of the pages stays with the cache
+        pages = max(1, sum((len(t) + max_new_tokens - 1) // PAGE for t in ids))
         places = torch.arange(b, dtype=torch.int32, device=dev)
         status, drawn = StatusWord(dev), StatusWord(dev)
 
@@ -223,7 +225,7 @@ class PagedLlama:
                 raise RuntimeError("PagedLlama.generate: the model's logits leave no probability to draw from (they hold a NaN or an infinity)")
             return n
 
-        with self.cache.tables(b, longest) as tables:
+        with self.cache.tables(b, longest, pages) as tables:
             tokens = torch.zeros(b, tables.longest + drafts + 1, dtype=torch.int64, device=dev)   # (room for what is cut off at the end)
             row = torch.arange(b, device=dev)
             lens = [len(t) for t in ids]

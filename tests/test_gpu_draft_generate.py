@@ -68,3 +68,31 @@ def test_more_drafts_than_a_step_takes(loaded, drafts):
     with pytest.raises(_Enough):
         m.generate([torch.arange(30)], 8, draft=draft, drafts=drafts)
     assert asked[0][0] == 6           # of 8 tokens the prompt gave the first, and a step draws its last one itself
+
+
+@pytest.mark.parametrize("lens,new,need", [((60, 3), 4, 0), ((60, 3), 5, 1), ((60, 124), 6, 3), ((128, 1, 63), 1, 2)])
+def test_pages_that_the_sequences_do_not_need_stay_free(loaded, lens, new, need):
+    """Other sequences of the cache go on while drafts are asked for; what is needed is enough, to the page."""
+    prompts = [torch.arange(n) % 500 for n in lens]
+    m = loaded(pages=max(1, need) + 2, sequences=len(lens) + 1)
+    free = []
+
+    def draft(tokens, lengths, n):
+        free.append(m.cache.free_pages())
+        if len(free) == 1:                           # a sequence of somebody else's
+            m.forward({m.cache.add(): torch.arange(130)})
+        return _same_again(tokens, lengths, n)
+
+    out = m.generate(prompts, new, draft=draft)
+    assert [len(o) for o in out] == [new] * len(lens)
+    if new > 2:
+        assert free[0] == 2 and m.cache.free_pages() == max(1, need)
+    plain = m.generate(prompts, new)                 # (each of its tokens is the likeliest; so is each of those with drafts)
+    assert [len(o) for o in plain] == [new] * len(lens)
+    if need:
+        short = loaded(pages=need, sequences=len(lens))
+        taken = short.cache.step({short.cache.add(): 64}) if need > 1 else None
+        if taken is not None:
+            with pytest.raises(RuntimeError, match="free"):
+                short.generate(prompts, new, draft=_same_again)
+            assert short.cache.free_pages() == need - 1
