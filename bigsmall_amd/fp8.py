@@ -39,7 +39,7 @@ def _gpu(index: int, what) -> None:
 
 
 def _refuse_grad() -> None:
-    raise RuntimeError("fp8_linear has no backward pass: call it under torch.no_grad(), or detach its input")
+    raise RuntimeError("fp8_linear has no backward pass: call it under torch.no_grad(), or detach its inputs")
 
 
 # bs_fp8_rows of include/bigsmall_fp8.h
@@ -63,7 +63,7 @@ def _call(name: str, index: int, *args) -> None:
 
 class Fp8Weight:
     """A weight [outer, inner]: e4m3 codes and one f32 scale for each block of 128 by 128 (the last ones may be
-    smaller). The codes are used in place where their rows start at multiples of 128 bytes from a 16-byte
+    smaller), neither of which may require a gradient while gradients are recorded. The codes are used in place where their rows start at multiples of 128 bytes from a 16-byte
     aligned base, as a contiguous tensor's of a multiple of 128 columns do; else they are copied once, here, into rows
     that end in zeros."""
 
@@ -78,6 +78,8 @@ class Fp8Weight:
         if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or tuple(scales.shape) != (_blocks(n), _blocks(k)):
             raise ValueError(f"Fp8Weight: scales must be a float32 tensor [{_blocks(n)}, {_blocks(k)}], got "
                              f"{getattr(scales, 'dtype', type(scales).__name__)} {tuple(getattr(scales, 'shape', ()))}")
+        if _recording() and (codes.requires_grad or scales.requires_grad):
+            _refuse_grad()
         if scales.device != codes.device:
             raise ValueError(f"Fp8Weight: scales are on {scales.device}, codes on {codes.device}")
         stride = codes.stride(0) if n > 1 else _blocks(k) * BLOCK
