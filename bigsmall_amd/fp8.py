@@ -12,8 +12,9 @@ A value is its code times its block's scale, as in checkpoints that hold a
 13 bits below the largest one's first bit, then f32), the result is rounded once.
 
 Inference only: inputs that require a gradient are refused while gradients are
-recorded. All calls run on the current torch stream of the weight's device and do
-not synchronise; work areas come from torch's allocator for each call.
+recorded, and dual tensors of forward-mode differentiation always. All calls run on
+the current torch stream of the weight's device and do not synchronise; work areas come
+from torch's allocator for each call.
 """
 from __future__ import annotations
 
@@ -21,8 +22,10 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
+from ._gradients import recording, tangents
 
 BLOCK = 128
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
@@ -39,7 +42,8 @@ def _gpu(index: int, what) -> None:
 
 
 def _refuse_grad() -> None:
-    raise RuntimeError("fp8_linear has no backward pass: call it under torch.no_grad(), or detach its inputs")
+    raise RuntimeError("fp8_linear has no backward pass, and no derivative forwards: call it under torch.no_grad(), or detach its inputs (of a "
+                       "dual tensor, take the primal)")
 
 
 # bs_fp8_rows of include/bigsmall_fp8.h
@@ -47,7 +51,6 @@ _ROWS = struct.Struct("=2Q4I")
 assert _ROWS.size == ctypes.sizeof(_native.BsFp8Rows)
 
 _stream = torch._C._cuda_getCurrentRawStream
-_recording = torch.is_grad_enabled
 
 
 def _call(name: str, index: int, *args) -> None:
@@ -78,7 +81,7 @@ class Fp8Weight:
         if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or tuple(scales.shape) != (_blocks(n), _blocks(k)):
             raise ValueError(f"Fp8Weight: scales must be a float32 tensor [{_blocks(n)}, {_blocks(k)}], got "
                              f"{getattr(scales, 'dtype', type(scales).__name__)} {tuple(getattr(scales, 'shape', ()))}")
-        if _recording() and (codes.requires_grad or scales.requires_grad):
+        if (recording() and (codes.requires_grad or scales.requires_grad)) or (forward_ad._current_level >= 0 and tangents(codes, scales)):
             _refuse_grad()
         if scales.device != codes.device:
             raise ValueError(f"Fp8Weight: scales are on {scales.device}, codes on {codes.device}")
@@ -138,7 +141,7 @@ def fp8_quantise(x) -> Fp8Rows:
         raise ValueError(f"x has shape {tuple(shape)}; its last dimension must hold 1 to {_MOST_COLS} columns")
     index = x.get_device()
     _gpu(index, x)
-    if x.requires_grad and _recording():
+    if (x.requires_grad and recording()) or (forward_ad._current_level >= 0 and tangents(x)):
         _refuse_grad()
     y, t, k = _matrix(x)
     blocks = (k + BLOCK - 1) // BLOCK
@@ -170,7 +173,7 @@ def fp8_linear(x, weight: Fp8Weight, dtype=None):
             raise ValueError(f"x has shape {tuple(x.shape)}, the weight has {weight.inner} columns")
         if x.get_device() != index:
             raise ValueError(f"x is on {x.device}, the weight on {weight.device}")
-        if x.requires_grad and _recording():
+        if (x.requires_grad and recording()) or (forward_ad._current_level >= 0 and tangents(x)):
             _refuse_grad()
         shape, rows = x.shape[:-1], None
         values, t, _ = _matrix(x)

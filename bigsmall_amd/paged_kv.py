@@ -20,9 +20,10 @@ PagedKVCache keeps the pools of all layers and does the bookkeeping: sequences,
 pages, tails, steps.
 
 Inference only: inputs that require a gradient are refused while gradients are
-recorded. All calls run on the current torch stream of the pool's device and do not
-synchronise. Work areas come from torch's allocator for each call. Tensors of
-another stream need the usual wait and record_stream by the caller.
+recorded, and dual tensors of forward-mode differentiation always. All calls run on
+the current torch stream of the pool's device and do not synchronise. Work areas come
+from torch's allocator for each call. Tensors of another stream need the usual wait and
+record_stream by the caller.
 """
 from __future__ import annotations
 
@@ -31,8 +32,10 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
+from ._gradients import recording, tangents
 from .device import status_ptr
 
 PAGE = 64
@@ -200,7 +203,8 @@ def _gpu(pool: KVPool) -> None:
 
 
 def _refuse_grad() -> None:
-    raise RuntimeError("the paged KV cache has no backward pass: call it under torch.no_grad(), or detach q, k and v")
+    raise RuntimeError("the paged KV cache has no backward pass, and no derivative forwards: call it under torch.no_grad(), or detach q, k and v "
+                       "(of a dual tensor, take the primal)")
 
 
 def _refuse_total(batch: KVBatch, n: int) -> None:
@@ -216,7 +220,6 @@ def _check_batch(pool: KVPool, batch: KVBatch) -> None:
 # The current stream's handle of a device, without the Stream object that torch.cuda.current_stream makes (2 us of a
 # call that takes 10).
 _stream = torch._C._cuda_getCurrentRawStream
-_recording = torch.is_grad_enabled
 
 # bs_kv_rows and bs_kv_query of include/bigsmall_kv.h, packed: a ctypes structure of as many fields takes 1 us more to fill
 _ROWS = struct.Struct("=6Q6q4I")
@@ -274,7 +277,7 @@ def kv_append(pool: KVPool, batch: KVBatch, q, k, v, rope: Optional[Rope] = None
             result = out
         else:
             qp = 0
-    if _recording() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad)):
+    if (recording() and (k.requires_grad or v.requires_grad or (q is not None and q.requires_grad))) or (forward_ad._current_level >= 0 and tangents(q, k, v)):
         _refuse_grad()
     if t:
         _call("bs_kv_append", pool, batch.with_rows(t), _ROWS.pack(qp, kp, vp, op, cos, sin, q0, q1, k0, k1, v0, v1, heads, rot, inter, n_pos),
@@ -300,7 +303,7 @@ def kv_attend(pool: KVPool, batch: KVBatch, q, scale: Optional[float] = None, so
     _check_heads(heads, pool)
     if not 0 <= window < 1 << 31 or not 0.0 <= softcap < float("inf"):
         raise ValueError("window and softcap must not be negative or infinite")
-    if _recording() and (q.requires_grad or (slopes is not None and slopes.requires_grad)):
+    if (recording() and (q.requires_grad or (slopes is not None and slopes.requires_grad))) or (forward_ad._current_level >= 0 and tangents(q, slopes)):
         _refuse_grad()
     sp = pp = fp = 0
     if slopes is not None:
