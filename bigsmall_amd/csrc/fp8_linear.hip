@@ -397,7 +397,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void tile_kernel(Args A) {
 //  - Operands are read at least six products ahead, one or two of them every four products: the first half of a block
 //    goes through the weight's tiles, each of which then gives its registers to one of the second half, and the second half
 //    through x's, each of which gives way to the next block's.
-// 8,192 rows through 14,336 x 4,096: 404 us, 2.38 PFLOP/s, where the library's product with a single scale takes 328. (As a Tile of these sizes
+// 8,192 rows through 14,336 x 4,096: 398 to 404 us, 2.4 PFLOP/s, where the library's product with a single scale takes 328. (As a Tile of these sizes
 // 433, its operands read at once and each tile by itself; in halves but read at once 443; read in turn 418. Without waiting for loads
 // it takes as long.) The clock sinks with the load: with x and weight 0 it takes 312, the library 250. Matrix units are busy 70 % of the clocks,
 // the vector units' additions of scaled products take 35 %.
@@ -469,8 +469,8 @@ __global__ __launch_bounds__(Large::THREADS, 2) void large_kernel(Args A) {
 
   // The blocks of all the workgroup's tiles come as one row of blocks. This is where loading stands in it: two blocks ahead of the products,
   // and at the end on the last one, which is loaded again and not read. As in tile_kernel a load is eight rows: 8 w, 64 + 8 w (B),
-  // 128 + 8 w, 192 + 8 w (B) of the weight, all four of x (A); one more brings the scales of the wave's rows of x, and at a
-  // tile's first block and each 64th after it one the next 64 of the weight.
+  // 128 + 8 w, 192 + 8 w (B) of the weight, all four of x (A); one more (A) brings a block's scales: waves 0 to 3 those of 64
+  // rows of x each, waves 4 to 7 one of the weight's two, the same in all lanes.
   uint32_t wfrom[4], xfrom[4], scale_at, next = blockIdx.x, at = 0, slot = 0;
   __amdgpu_buffer_rsrc_t wbase, xbase;
   const float* scale_base;
@@ -622,8 +622,8 @@ __global__ __launch_bounds__(Large::THREADS, 2) void large_kernel(Args A) {
 
 // A workgroup: NT * 16 rows of the weight by TT * 16 of x. Each of its waves takes blocks in turn and brings them to LDS for itself
 // alone, STAGES deep, so waves wait for their own loads only and never for one another until their sums are joined, wave by
-// wave. (With waves that share each block, a barrier a block: 64 rows through 14,336 x 4,096 22 us, so 15.) The bound is memory, and
-// with few tiles how long a wave's loads take to come.
+// wave. (With waves that share each block, a barrier a block: 64 rows through 14,336 x 4,096 22 us, so 14; a weight that no cache holds
+// 18, 3.3 TB/s.) The bound is memory, and with few tiles how long a wave's loads take to come: 224 workgroups of 256 compute units there.
 template <int NT_, int TT_, int WAVES_, int STAGES_>
 struct Stream {
   static constexpr uint32_t NT = NT_, TT = TT_, WAVES = WAVES_, STAGES = STAGES_, THREADS = WAVES * 64, N = NT * 16, T = TT * 16;
@@ -770,7 +770,7 @@ __global__ __launch_bounds__(V_THREADS) void values_kernel(Args A, const uint16_
 
 // Up to this many blocks of x and rows of the weight (a workgroup a compute unit). One row through 4,096 x 4,096: 6.5 us, quantised
 // by a kernel of its own 8.3; three (96 blocks) 7.9 and 8.5, four 8.9 and 8.4; one row of 14,336 columns 15.3 and 14.0; one through
-// 14,336 x 4,096 13.1 and 13.8, through 16,384 x 2,048 12.0 and 10.7.
+// 14,336 x 4,096 13.1 and 13.8, through 16,384 x 2,048 12.0 and 10.7: beyond a workgroup a compute unit it goes either way.
 constexpr uint32_t V_BLOCKS = 96, V_OUTER = 4096;
 
 template <int TYPE>
@@ -812,8 +812,9 @@ int stream_go(Args A, hipStream_t s) {
 
 // The shapes, and what they take, in us as measured: `fixed`, for each workgroup of a compute unit `start`, and `one` for each block
 // that it (a wave of a stream) goes through; start2 and two are for a pair of workgroups, side by side where LDS holds two. The smallest
-// estimate is taken. Over 1 to 4,096 rows through 512 x 14,336, 1,024 x 4,096, 2,048 x 1,024, 4,096 x 4,096, 4,096 x 14,336, 14,336 x 512 and
-// 14,336 x 4,096 that is at most a seventh slower than the fastest of them, mostly as fast.
+// estimate is taken. Over 1 to 8,192 rows through 512 x 14,336, 1,024 x 4,096, 2,048 x 1,024, 1,000 x 1,400, 4,096 x 4,096, 4,096 x 14,336,
+// 14,336 x 512 and 14,336 x 4,096 that is at most a tenth slower than the fastest of them, mostly as fast. (The estimates are of
+// weights that a cache holds: one that comes from memory takes longer by any shape.)
 struct Shape {
   uint32_t n, t, waves;
   float fixed, start, one, start2, two;

@@ -48,13 +48,15 @@ def draft_verify(p, draft, cu, accept, pick, q=None, max_drafts=None, status=Non
     """Which drafted tokens stay, and the token after them. Returns tokens int64 [B, max_drafts + 1] (the drafts
     taken, the token drawn, then -1) and counts int32 [B] (how many tokens those are).
 
-    p [T, vocab]     the target's probabilities after each row's token (f32, bf16 or f16; they need not add up to 1)
+    p [T, vocab]     the target's probabilities after each row's token (f32, bf16 or f16). The draw does not depend on a row's sum,
+                     taking a draft does: tokens follow p only if its rows, and q's, add up to 1
     draft [T] int64  the token proposed to follow each row
     cu [B + 1] int32 sequence b has the rows cu[b] .. cu[b + 1] - 1, one more than drafts; its last row's draft,
                      accept and q are not read. A sequence without rows gets no token and count 0
     accept [T], pick [B] f32   random numbers in [0, 1)
     q [T, vocab]     the probabilities that the drafts were drawn from, of p's type; None: they were not drawn
-    max_drafts       the most that a sequence has, up to 1,024 (by default T - B, held to 0 and 1,024)
+    max_drafts       the most that a sequence has, up to 1,024 (by default T - B, held to 0 and 1,024: enough where every sequence
+                     has a row; say it where some have none)
 
     Draft x is taken while accept * q[x] < p[x] (without q: accept < p[x]). Then one token is drawn: where a draft was
     refused from max(p - q, 0) of its row (without q: from p without the draft), after the last one from p. It is the first

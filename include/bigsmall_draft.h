@@ -24,8 +24,9 @@ extern "C" {
 #define BS_DRAFT_MOST 1024 /* drafts of a sequence */
 
 /* Row r of p is the target's distribution after row r's token, row r of q the
- * draft model's, draft[r] the token proposed to follow it. Sequence b has rows
- * cu[b] .. cu[b + 1] - 1, one more than drafts (its last row of q, draft and
+ * draft model's, draft[r] the token proposed to follow it. Drafts are taken by p
+ * and q as they are: tokens follow p only if their rows add up to 1. Sequence b has
+ * rows cu[b] .. cu[b + 1] - 1, one more than drafts (its last row of q, draft and
  * accept is not read); one without rows takes no part. */
 typedef struct {
     const void *p, *q;     /* [n_rows][vocab], rows p_stride and q_stride elements apart; q may be NULL */

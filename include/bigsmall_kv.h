@@ -156,7 +156,7 @@ int bs_kv_books_step(const bs_kv_books *books, const bs_kv_tables *step, const i
 int bs_kv_books_keep(const bs_kv_books *books, const bs_kv_tables *step, const int32_t *d_sure, const int32_t *d_kept,
                      void *stream);
 
-/* Empty places: their pages become free, the first sequence's first page the last to be taken. All or nothing, as above. */
+/* Empty places: their pages become free, the first sequence's first page on top, the next to be taken. All or nothing, as above. */
 int bs_kv_books_drop(const bs_kv_books *books, const int32_t *d_seqs, uint32_t n_seqs, int32_t *d_status, void *stream);
 
 #ifdef __cplusplus
